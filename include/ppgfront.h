@@ -335,6 +335,120 @@ int ppg_extend_map_matches(ppg_ctx* ctx, float nnratio, float th, const ppg_mapg
                            const int32_t* conn_off, const uint32_t* conn_idx,
                            uint8_t* tracked, int32_t* frame_mp, int32_t* frame_me, int* n_matches);
 
+/* ---- attention between descriptor sets ----
+ * What a learned matcher behind the front-end is made of: rows of one set against rows of another as in ppg_match_nn, with
+ * a softmax in the place of the argmin.  No counterpart in the reference (its matchers take the nearest neighbour,
+ * matching/src/Matcher.cpp:57-82).  All tensors are in device memory of the context's GPU; offsets and the argument
+ * structures are host memory, read before the call returns.  Nothing is allocated, so every call can be captured into a
+ * graph; memory a call needs between its kernels is the caller's (`work`), and calls that may run at the same time (two
+ * streams, two captured graphs) need a `work` each.
+ *
+ * A SET is what one frame or one local map contributes; a call takes n_sets of them, concatenated: set s owns the rows
+ * q_off[s] .. q_off[s+1]-1 of the queries and k_off[s] .. k_off[s+1]-1 of the keys (both ascending from >= 0, lengths of
+ * zero allowed).  Rows outside every set are neither read nor written.
+ * A ROW is `heads` vectors of head_dim components; component c of head h of row r is p[r * row + h * head + c].  row and
+ * head are strides in components, >= 0 (0: the same vector for all; not for outputs), byte strides and addresses
+ * multiples of 16.  A frame's own descriptors ([n][256] floats) are 4 heads of 64, 8 of 32 or 2 of 128.
+ * With more query heads than key heads, group = heads / kv_heads consecutive query heads share a key head.
+ * An output shares no component with an input, except where that is said.
+ * stream: as in ppg_match_nn_noalloc (NULL: the context's own stream, and the call returns when the results are in place;
+ * else a hipStream_t to enqueue on without waiting); PPG_STREAM_DEFAULT is HIP's default stream. */
+#define PPG_STREAM_DEFAULT ((void*)1)
+#define PPG_F32 0
+#define PPG_BF16 1
+#define PPG_F16 2
+#define PPG_ATTN_MAX_SETS 128     /* sets per call (PPG_ECAP beyond) */
+#define PPG_ATTN_MAX_SEL 64       /* blocks that one query may select (PPG_ECAP beyond) */
+typedef struct ppg_rows {
+    void* p;
+    int heads;
+    long long row, head;
+} ppg_rows;
+
+/* The descriptors ([n][256] fp32) and undistorted positions ([n][2] fp32) of frame `frame` of the batch that the last
+ * ppg_extract* / ppg_wait_batch on this context handed out, where they lie on the GPU: inputs for the calls below without
+ * a trip over the host.  They are complete, and stay as they are until the next of those calls or the second
+ * ppg_submit_batch* (the ring of slots behind ppg_frame_out). */
+int ppg_resident_frame(ppg_ctx* ctx, int frame, const float** d_desc, const float** d_pos, int* n);
+
+/* Rotary positions.  Of every vector, the first rot_dim components are rot_dim/2 pairs; pair j is turned by the angle
+ * pos[r][axis] * freq[j] (64-bit product and reduction, so far positions keep their angle), the others are copied:
+ *   (x, y) -> (x cos - y sin, x sin + y cos);  inverse != 0: the opposite angle (which is also the gradient's turn).
+ * layout: PPG_ROTARY_INTERLEAVED pairs components (2j, 2j+1), PPG_ROTARY_HALF (j, j + rot_dim/2).
+ * n_axes 1: one coordinate per row; 2 (rot_dim a multiple of 4): pairs below rot_dim/4 turn with the first coordinate,
+ * the rest with the second.  Two tensors (queries and keys) per call, the second optional (n_rows[1] = 0); dst may be
+ * src (same address and strides).  A position that is not finite gives NaN in that row's rotated components. */
+#define PPG_ROTARY_INTERLEAVED 0
+#define PPG_ROTARY_HALF 1
+typedef struct ppg_rotary_args {
+    int dtype, head_dim, rot_dim, layout, inverse, n_axes;
+    int n_rows[2];
+    const float* pos[2];      /* [n_rows][n_axes] */
+    const double* freq;       /* [rot_dim/2], radians per unit of position */
+    ppg_rows src[2], dst[2];
+} ppg_rotary_args;
+int ppg_rotary(ppg_ctx* ctx, const ppg_rotary_args* args, void* stream);
+/* The usual frequencies (host): freq[j] = base^(-j/n) for j < n.  scale > 1 stretches them for positions up to scale times
+ * the `extent` a model was trained on: a pair that turns at least `high` times over the extent keeps its frequency, one
+ * that turns at most `low` times is divided by scale, in between linearly in the number of turns.  scale = 1: plain. */
+int ppg_rotary_frequencies(int n, double base, double scale, double extent, double low, double high, double* freq);
+
+/* Keys in blocks of `block` (32, 64 or 128) consecutive rows, counted from the start of each set; the last one of a set may
+ * be short.  Set s has ceil(len / block) of them and their records follow those of set s-1.
+ * mean [blocks][kv_heads][head_dim]: the mean of a block's keys, summed in 64 bits and rounded once (0 for a block without
+ * keys); count [blocks]: its keys.  skip (optional): keys with skip[row] != 0 are left out. */
+typedef struct ppg_block_means_args {
+    int dtype, head_dim, block, n_sets;
+    const int32_t* k_off;
+    ppg_rows k;
+    const uint8_t* skip;
+    float* mean;
+    int32_t* count;
+} ppg_block_means_args;
+int ppg_block_means(ppg_ctx* ctx, const ppg_block_means_args* args, void* stream);
+
+/* The n_sel blocks of its set whose means have the largest product with the (summed) query of a group, for every query
+ * row and key head: sel [rows of q][kv_heads][n_sel], block numbers within the set, ascending, -1 behind them when the set
+ * has fewer blocks with count > 0.  Products are evaluated in 64 bits; equal ones go to the lower block, NaN ranks below
+ * every number. */
+typedef struct ppg_block_select_args {
+    int dtype, head_dim, block, n_sets;
+    const int32_t *q_off, *k_off;
+    ppg_rows q;
+    int kv_heads;
+    const float* mean;
+    const int32_t* count;
+    int n_sel;
+    int32_t* sel;
+} ppg_block_select_args;
+int ppg_block_select(ppg_ctx* ctx, const ppg_block_select_args* args, void* stream);
+
+/* Attention: out = sum_j p_j v_j with p = softmax over j of scale * q . k_j, over the keys of the row's set.
+ * skip (optional): keys with skip[row] != 0 are left out whatever their values (also NaN or infinite ones).
+ * sel (optional, with block and n_sel): only the listed blocks of the set, [rows of q][kv_heads][n_sel] as
+ * ppg_block_select writes them; numbers that name no block of the set are passed over, and a block listed twice counts
+ * twice.  A row with nothing to attend to (or whose products are all -inf) gives 0, and -inf in lse.
+ * lse (optional, [rows of q][heads]): log sum_j exp(scale * q . k_j).
+ * Products and sums are held in 32 bits; with 16-bit inputs the softmax's weights are rounded to that type before they
+ * meet the values, as the inputs of the matrix unit are. */
+typedef struct ppg_attention_args {
+    int dtype, head_dim;
+    float scale;              /* > 0 */
+    int n_sets;
+    const int32_t *q_off, *k_off;
+    ppg_rows q, k, v, out;
+    const uint8_t* skip;
+    float* lse;
+    int block, n_sel;
+    const int32_t* sel;
+    void* work;               /* ppg_attention_work() bytes, 256-byte aligned; may be NULL when that is 0 */
+    size_t work_bytes;
+} ppg_attention_args;
+/* Bytes of `work` a call with these arguments needs (by its sizes; no pointer but q_off and k_off is read); 0 also for
+ * arguments that the call would refuse. */
+size_t ppg_attention_work(const ppg_attention_args* args);
+int ppg_attention(ppg_ctx* ctx, const ppg_attention_args* args, void* stream);
+
 /* HIP stream the context launches on (as a void* hipStream_t). */
 void* ppg_stream(ppg_ctx* ctx);
 

@@ -20,6 +20,10 @@ PPG_OK, PPG_EINVAL, PPG_EHIP, PPG_EIO, PPG_ENOMEM, PPG_ECAP, PPG_ERANGE, PPG_ECO
 SHUTTER_ID_BYTES = 128
 T_FEAT, T_JUNC, T_HEAT_RAW, T_DESCMAP, T_SCORE, T_HEAT, T_HEAT_REFINED, T_HEAT_REMAPPED = range(8)
 MATCH_PLAIN, MATCH_INIT = 0, 1
+F32, BF16, F16 = 0, 1, 2
+ROTARY_INTERLEAVED, ROTARY_HALF = 0, 1
+STREAM_DEFAULT = 1
+ATTN_MAX_SETS, ATTN_MAX_SEL = 128, 64
 
 
 class Config(C.Structure):
@@ -43,6 +47,70 @@ class MapGraph(C.Structure):
     _fields_ = [("m", C.c_int), ("desc", C.c_void_p), ("proj", C.c_void_p), ("viewcos", C.c_void_p),
                 ("in_view", C.c_void_p), ("bad", C.c_void_p), ("nobs", C.c_void_p), ("edge_off", C.c_void_p),
                 ("edge_id", C.c_void_p), ("edge_other", C.c_void_p), ("edge_ok", C.c_void_p)]
+
+
+class Rows(C.Structure):
+    """ppg_rows: a device address, heads per row, and the strides of a row and of a head in components."""
+    _fields_ = [("p", C.c_void_p), ("heads", C.c_int), ("row", C.c_longlong), ("head", C.c_longlong)]
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("head_dim", C.c_int), ("rot_dim", C.c_int), ("layout", C.c_int), ("inverse", C.c_int),
+                ("n_axes", C.c_int), ("n_rows", C.c_int * 2), ("pos", C.c_void_p * 2), ("freq", C.c_void_p),
+                ("src", Rows * 2), ("dst", Rows * 2)]
+
+
+class BlockMeansArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("head_dim", C.c_int), ("block", C.c_int), ("n_sets", C.c_int), ("k_off", C.c_void_p),
+                ("k", Rows), ("skip", C.c_void_p), ("mean", C.c_void_p), ("count", C.c_void_p)]
+
+
+class BlockSelectArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("head_dim", C.c_int), ("block", C.c_int), ("n_sets", C.c_int), ("q_off", C.c_void_p),
+                ("k_off", C.c_void_p), ("q", Rows), ("kv_heads", C.c_int), ("mean", C.c_void_p), ("count", C.c_void_p),
+                ("n_sel", C.c_int), ("sel", C.c_void_p)]
+
+
+class AttentionArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("head_dim", C.c_int), ("scale", C.c_float), ("n_sets", C.c_int), ("q_off", C.c_void_p),
+                ("k_off", C.c_void_p), ("q", Rows), ("k", Rows), ("v", Rows), ("out", Rows), ("skip", C.c_void_p),
+                ("lse", C.c_void_p), ("block", C.c_int), ("n_sel", C.c_int), ("sel", C.c_void_p), ("work", C.c_void_p),
+                ("work_bytes", C.c_size_t)]
+
+
+def offsets(values):
+    """Set offsets as the argument structures take them (n_sets + 1 host integers)."""
+    return np.ascontiguousarray(values, np.int32)
+
+
+def _args(kind, q_off, k_off, fields):
+    a = kind(**fields)
+    a._keep = (q_off, k_off)   # the structure holds addresses only
+    for name, off in (("q_off", q_off), ("k_off", k_off)):
+        if off is not None:
+            setattr(a, name, off.ctypes.data)
+            a.n_sets = len(off) - 1
+    return a
+
+
+def rotary_args(n_rows, pos, src, dst, **fields):
+    """ppg_rotary_args; n_rows, pos, src and dst are pairs (queries, keys) or one-element tuples."""
+    a = RotaryArgs(**fields)
+    for i in range(len(n_rows)):
+        a.n_rows[i], a.pos[i], a.src[i], a.dst[i] = n_rows[i], pos[i], src[i], dst[i]
+    return a
+
+
+def block_means_args(k_off, **fields):
+    return _args(BlockMeansArgs, None, k_off, fields)
+
+
+def block_select_args(q_off, k_off, **fields):
+    return _args(BlockSelectArgs, q_off, k_off, fields)
+
+
+def attention_args(q_off, k_off, **fields):
+    return _args(AttentionArgs, q_off, k_off, fields)
 
 
 _lib = None
@@ -156,6 +224,14 @@ def lib():
         L.ppg_profile.argtypes = [C.c_void_p, C.c_int]
         L.ppg_profile_read.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p]
         L.ppg_profile_flops.argtypes = [C.c_void_p, C.c_void_p]
+        L.ppg_resident_frame.argtypes = [C.c_void_p, C.c_int, C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_int)]
+        L.ppg_rotary.argtypes = [C.c_void_p, C.POINTER(RotaryArgs), C.c_void_p]
+        L.ppg_rotary_frequencies.argtypes = [C.c_int] + [C.c_double] * 5 + [C.c_void_p]
+        L.ppg_block_means.argtypes = [C.c_void_p, C.POINTER(BlockMeansArgs), C.c_void_p]
+        L.ppg_block_select.argtypes = [C.c_void_p, C.POINTER(BlockSelectArgs), C.c_void_p]
+        L.ppg_attention.argtypes = [C.c_void_p, C.POINTER(AttentionArgs), C.c_void_p]
+        L.ppg_attention_work.argtypes = [C.POINTER(AttentionArgs)]
+        L.ppg_attention_work.restype = C.c_size_t
         _lib = L
     return _lib
 
@@ -176,6 +252,15 @@ def default_config(width, height, max_batch=1, max_num=500, weights=DEFAULT_WEIG
     cfg._weights_keepalive = os.path.abspath(weights).encode()
     cfg.weights_path = cfg._weights_keepalive
     return cfg
+
+
+def rotary_frequencies(n, base=10000.0, scale=1.0, extent=1.0, low=1.0, high=32.0):
+    """ppg_rotary_frequencies (host): n doubles."""
+    f = np.zeros(max(n, 1), np.float64)
+    rc = lib().ppg_rotary_frequencies(n, base, scale, extent, low, high, f.ctypes.data)
+    if rc:
+        raise PPGError(f"ppg_rotary_frequencies failed ({rc}): " + lib().ppg_last_error(None).decode())
+    return f[:n]
 
 
 class PPGError(RuntimeError):
@@ -351,6 +436,28 @@ class Context:
         return self.L.ppg_match_nn_noalloc(C.c_void_p(self.h), C.c_void_p(dA), nA, C.c_void_p(dB), nB, dim, C.c_float(th),
                                            C.c_float(ratio), mode, C.c_void_p(d_match12), C.c_void_p(d_best),
                                            C.c_void_p(d_second), C.c_void_p(d_count), C.c_void_p(stream))
+
+    # ---- attention between descriptor sets (device tensors; stream as in match_nn_noalloc, STREAM_DEFAULT: HIP's default) ----
+    def resident_frame(self, frame=0):
+        """(device address of the descriptors, of the undistorted positions, rows) of a frame of the last batch."""
+        d, p, n = C.c_void_p(), C.c_void_p(), C.c_int(0)
+        self._chk(self.L.ppg_resident_frame(self.h, frame, C.byref(d), C.byref(p), C.byref(n)))
+        return d.value, p.value, n.value
+
+    def rotary(self, args, stream=None):
+        self._chk(self.L.ppg_rotary(self.h, args, stream))
+
+    def block_means(self, args, stream=None):
+        self._chk(self.L.ppg_block_means(self.h, args, stream))
+
+    def block_select(self, args, stream=None):
+        self._chk(self.L.ppg_block_select(self.h, args, stream))
+
+    def attention_work(self, args):
+        return self.L.ppg_attention_work(args)
+
+    def attention(self, args, stream=None):
+        self._chk(self.L.ppg_attention(self.h, args, stream))
 
     def last_error(self):
         return self.L.ppg_last_error(C.c_void_p(self.h)).decode()

@@ -1,0 +1,58 @@
+// Launch interface of the attention kernels (attn_kernels.hip) towards ppg_attn.cpp.  Everything was checked on the host
+// before it gets here: types, sizes, strides, alignments, the offsets' order.
+#pragma once
+#include "../../include/ppgfront.h"
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace ppg {
+
+// The sets of a call travel with the launch (kernel arguments): no copy to the device, nothing that a later call could
+// overwrite, and a captured graph keeps its own.
+struct AttnSets {
+    int n;
+    int q_off[PPG_ATTN_MAX_SETS + 1], k_off[PPG_ATTN_MAX_SETS + 1];
+    int tile[PPG_ATTN_MAX_SETS + 1];   // first work-group tile of a set (what a tile is depends on the kernel)
+    int blk[PPG_ATTN_MAX_SETS + 1];    // first key block of a set
+};
+
+struct RotaryLaunch {
+    int head_dim, rot_dim, layout, inverse, n_axes;
+    int n_rows[2];
+    const float* pos[2];
+    const double* freq;
+    ppg_rows src[2], dst[2];
+};
+hipError_t launch_rotary(int dtype, const RotaryLaunch& a, hipStream_t s);
+
+struct BlockMeansLaunch {
+    int block;
+    ppg_rows k;
+    const uint8_t* skip;
+    float* mean;
+    int32_t* count;
+};
+hipError_t launch_block_means(int dtype, int head_dim, const BlockMeansLaunch& a, AttnSets& sets, hipStream_t s);
+
+struct BlockSelectLaunch {
+    int block, kv_heads, n_sel;
+    ppg_rows q;
+    const float* mean;
+    const int32_t* count;
+    int32_t* sel;
+};
+hipError_t launch_block_select(int dtype, int head_dim, const BlockSelectLaunch& a, AttnSets& sets, hipStream_t s);
+
+struct AttentionLaunch {
+    float scale;
+    ppg_rows q, k, v, out;
+    const uint8_t* skip;
+    float* lse;
+    int block, n_sel;
+    const int32_t* sel;
+    void* work;
+};
+size_t attention_work(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets);
+hipError_t launch_attention(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets, hipStream_t s);
+
+}  // namespace ppg

@@ -1,7 +1,7 @@
 // Attention between descriptor sets on gfx950: rotary positions, block means, block selection, attention over whole sets
 // or over selected blocks.  Sums, softmax statistics and means are held in 32 bits or more; what is stored in fewer bits is
 // rounded once, to nearest even.
-#include "attn_kernels.h"
+#include "attn_tile.h"
 #include "wave_util.h"
 
 #include <algorithm>
@@ -11,17 +11,6 @@ namespace ppg {
 // ---- element types ----
 template <class T> __device__ __forceinline__ float to_float(T v) { return (float)v; }
 template <class T> struct alignas(16) Vec16 { T v[16 / sizeof(T)]; };
-
-// the set whose [first, next) range of `off` holds x; off ascends, off[0] <= x < off[n]
-__device__ __forceinline__ int find_set(const int* off, int n, int x) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (off[mid] <= x) lo = mid;
-        else hi = mid;
-    }
-    return lo;
-}
 
 // cos and sin of `turns` full turns: the reduction is exact in 64 bits (the distance to the nearest quarter turn), the rest,
 // at most an eighth of a turn, goes through the Taylor sums of sine and cosine, whose first terms left out are below 2^-29
@@ -275,9 +264,10 @@ hipError_t launch_block_select(int dtype, int head_dim, const BlockSelectLaunch&
     return hipGetLastError();
 }
 
-size_t attention_work(int, int, const AttentionLaunch&, AttnSets&) { return 0; }
+size_t attention_work(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets) { return a.n_sel ? 0 : dense_work(dtype, head_dim, a, sets); }
 
 hipError_t launch_attention(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets, hipStream_t s) {
+    if (!a.sel) return launch_dense(dtype, head_dim, a, sets, s);
     const long long units = ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads;
     if (!units) return hipSuccess;
     BY_TYPE(dtype, BY_DIM(head_dim, (attention_row_kernel<T, D><<<(unsigned)((units + 3) / 4), 256, 0, s>>>(a, sets))));

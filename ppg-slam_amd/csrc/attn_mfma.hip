@@ -1,0 +1,375 @@
+// Attention over whole sets on the matrix cores (layouts and softmax in attn_tile.h).
+//
+// Rows: the queries of the `group` heads that share a key head are one long list, row r = query r / group, head r % group.
+//   attention_wide_kernel  four waves of 32 rows each share the key and value tiles in LDS (two stages: the next tile's
+//                          loads are in flight in registers while this one is multiplied);
+//   attention_split_kernel 32 rows per work-group, its four waves (and, where rows are few, several work-groups) share out the
+//                          keys; sums meet in LDS, and those of several work-groups in attention_join_kernel.
+#include "attn_tile.h"
+
+#include <algorithm>
+
+namespace ppg {
+
+// where row r of key head g lives; rows behind the last are the last one (computed, not stored)
+struct RowPlace {
+    long long q;
+    int head;
+};
+__device__ __forceinline__ RowPlace row_place(int r, int rows, int group, int g, int q0) {
+    r = min(r, rows - 1);
+    const int q = group == 1 ? r : r / group;
+    return {(long long)(q0 + q), g * group + (group == 1 ? 0 : r - q * group)};
+}
+
+template <class T, int D, int NF = Shape<T, D>::NF>
+__device__ __forceinline__ void load_query(u32x4 (&f)[NF], const ppg_rows& q, const RowPlace& p, int h) {
+    const T* x = (const T*)q.p + p.q * q.row + p.head * q.head;
+#pragma unroll
+    for (int i = 0; i < Shape<T, D>::NF; i++) f[i] = *(const u32x4*)(x + Shape<T, D>::chunk(i, h) * Shape<T, D>::N);
+}
+
+// this lane's components of its query: 4 consecutive ones per register group
+template <class T, int D> __device__ __forceinline__ void store_out(const ppg_rows& out, const RowPlace& p, const f32x16 (&o)[D / 32], float inv, int h) {
+    T* y = (T*)out.p + p.q * out.row + p.head * out.head;
+#pragma unroll
+    for (int t = 0; t < D / 32; t++)
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            T w[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = (T)(inv == 0.f ? 0.f : o[t][b * 4 + e] * inv);
+            if constexpr (IsF32<T>::v) *(f32x4*)(y + t * 32 + 8 * b + 4 * h) = __builtin_bit_cast(f32x4, w);
+            else *(s16x4*)(y + t * 32 + 8 * b + 4 * h) = __builtin_bit_cast(s16x4, w);
+        }
+}
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }
+__device__ __forceinline__ float log_sum(float m, float l, float c) { return l == 0.f ? -INFINITY : fmaf(m, c, __log2f(l)) * kLn2; }
+
+template <class T, int D, int BN>
+__global__ __launch_bounds__(256, 2) void attention_wide_kernel(AttentionLaunch a, AttnSets sets) {
+    using S = Shape<T, D>;
+    constexpr int SUB = BN / 32, CH = BN * S::CPR / 256, ROWB = D * (int)sizeof(T), TILE = BN * ROWB;
+    static_assert(BN * S::CPR % 256 == 0, "tile loads are whole rounds of the work-group");
+    __shared__ alignas(16) char lds_k[2][TILE], lds_v[2][TILE];
+    __shared__ unsigned char lds_dead[2][BN];
+    const int unit = xcd_unit(blockIdx.x, sets.tile[sets.n]);
+    if (unit >= sets.tile[sets.n]) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    const int s = find_set(sets.tile, sets.n, unit);
+    const int q0 = sets.q_off[s], k0 = sets.k_off[s], nk = sets.k_off[s + 1] - k0, kvh = a.k.heads, group = a.q.heads / kvh;
+    const int rows = (sets.q_off[s + 1] - q0) * group, tiles = (rows + 127) / 128;
+    const int g = (unit - sets.tile[s]) / tiles, row = ((unit - sets.tile[s]) % tiles) * 128 + wave * 32 + (lane & 31);
+    const RowPlace place = row_place(row, rows, group, g, q0);
+    u32x4 qf[S::NF];
+    load_query<T, D>(qf, a.q, place, h);
+    const float c = a.scale * kLog2e, slack = 8.f / c;
+    Running<T, D> run;
+    run.clear();
+
+    // tile loads: thread -> (row, chunk); rows behind the set are its last one with zero values
+    const T* kp = (const T*)a.k.p + g * a.k.head + (long long)k0 * a.k.row;
+    const T* vp = (const T*)a.v.p + g * a.v.head + (long long)k0 * a.v.row;
+    u32x4 rk[CH], rv[CH];
+    bool dead[CH];
+    auto load = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            const int x = tid + 256 * i, j = t * BN + x / S::CPR, ch = x % S::CPR, jj = min(j, nk - 1);
+            rk[i] = *(const u32x4*)(kp + (long long)jj * a.k.row + ch * S::N);
+            rv[i] = *(const u32x4*)(vp + (long long)jj * a.v.row + ch * S::N);
+            dead[i] = j >= nk || (a.skip && a.skip[k0 + jj]);
+        }
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            const int x = tid + 256 * i, r = x / S::CPR, ch = x % S::CPR;
+            *(u32x4*)(lds_k[buf] + r * ROWB + ((ch ^ S::swz_k(r)) << 4)) = rk[i];
+            *(u32x4*)(lds_v[buf] + r * ROWB + ((ch ^ S::swz_v(r)) << 4)) = dead[i] ? u32x4{0, 0, 0, 0} : rv[i];
+            if (ch == 0) lds_dead[buf][r] = dead[i];
+        }
+    };
+    const int nt = (nk + BN - 1) / BN;
+    if (nt) {
+        load(0);
+        store(0);
+    }
+    __syncthreads();
+    for (int t = 0; t < nt; t++) {
+        const int buf = t & 1;
+        if (t + 1 < nt) load(t + 1);
+        f32x16 sc[SUB];
+#pragma unroll
+        for (int u = 0; u < SUB; u++) {
+            const int r = u * 32 + (lane & 31);
+#pragma unroll
+            for (int e = 0; e < 16; e++) sc[u][e] = 0.f;
+#pragma unroll
+            for (int i = 0; i < S::NF; i++) {
+                const u32x4 kf = *(const u32x4*)(lds_k[buf] + r * ROWB + ((S::chunk(i, h) ^ S::swz_k(r)) << 4));
+                sc[u] = mfma_chunk<T>(kf, qf[i], sc[u]);
+            }
+        }
+        const unsigned long long gone = __ballot(lane < BN && lds_dead[buf][lane & (BN - 1)]);
+        if (gone) {
+#pragma unroll
+            for (int u = 0; u < SUB; u++) mask_scores(sc[u], (unsigned)(gone >> (32 * u)), h);
+        }
+        run.template weights<SUB>(sc, c, slack);
+#pragma unroll
+        for (int u = 0; u < SUB; u++) run.add_values(sc[u], lds_v[buf], u * 32, lane);
+        if (t + 1 < nt) store(buf ^ 1);   // last read one tile ago, before the barrier below
+        __syncthreads();
+    }
+    if (row >= rows) return;
+    const float l = other_half(run.l, false);
+    store_out<T, D>(a.out, place, run.o, inverse_sum(l), h);
+    if (a.lse && h == 0) a.lse[place.q * a.q.heads + place.head] = log_sum(run.m, l, c);
+}
+
+// A wave's own stretch of keys: operands straight from memory, values through an LDS image of its own.
+template <class T, int D, int BN> struct OwnKeys {
+    using S = Shape<T, D>;
+    static constexpr int SUB = BN / 32, VC = BN * S::CPR / 64, ROWB = D * (int)sizeof(T);
+    u32x4 rk[SUB][S::NF], rv[VC];
+    unsigned long long gone;
+    // keys j0 .. j0 + BN - 1 of the set at kp / vp, of which n exist (n >= 1: row n - 1 stands in for those behind it)
+    __device__ __forceinline__ void load(const T* kp, const T* vp, long long k_row, long long v_row, const uint8_t* skip, int j0, int n, int lane) {
+        const int h = lane >> 5;
+#pragma unroll
+        for (int u = 0; u < SUB; u++) {
+            const T* x = kp + (long long)min(j0 + u * 32 + (lane & 31), n - 1) * k_row;
+#pragma unroll
+            for (int i = 0; i < S::NF; i++) rk[u][i] = *(const u32x4*)(x + S::chunk(i, h) * S::N);
+        }
+        const int j = j0 + (lane & (BN - 1));
+        gone = __ballot(lane < BN && (j >= n || (skip && skip[min(j, n - 1)])));
+#pragma unroll
+        for (int i = 0; i < VC; i++) {
+            const int x = lane + 64 * i, r = x / S::CPR;
+            rv[i] = *(const u32x4*)(vp + (long long)min(j0 + r, n - 1) * v_row + (x % S::CPR) * S::N);
+        }
+    }
+    __device__ __forceinline__ void values_to_lds(char* v, int lane) const {
+#pragma unroll
+        for (int i = 0; i < VC; i++) {
+            const int x = lane + 64 * i, r = x / S::CPR, ch = x % S::CPR;
+            *(u32x4*)(v + r * ROWB + ((ch ^ S::swz_v(r)) << 4)) = (gone >> r) & 1 ? u32x4{0, 0, 0, 0} : rv[i];
+        }
+    }
+    __device__ __forceinline__ void scores(f32x16 (&sc)[SUB], const u32x4 (&qf)[S::NF], int lane) const {
+#pragma unroll
+        for (int u = 0; u < SUB; u++) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) sc[u][e] = 0.f;
+#pragma unroll
+            for (int i = 0; i < S::NF; i++) sc[u] = mfma_chunk<T>(rk[u][i], qf[i], sc[u]);
+            if (gone) mask_scores(sc[u], (unsigned)(gone >> (32 * u)), lane >> 5);
+        }
+    }
+};
+
+// The sums of the four waves of a work-group meet in LDS: [row][D] components and (m, l) per row, from wave 0 upwards.
+template <class T, int D> struct Meeting {
+    float o[32][D + 4];   // + 4: the 32 rows that a 16-byte access takes start in different banks
+    float m[32], l[32];
+};
+template <class T, int D> __device__ __forceinline__ void meet(Meeting<T, D>& x, Running<T, D>& run, float c, int wave, int waves, int lane) {
+    const int h = lane >> 5, col = lane & 31;
+    run.l = other_half(run.l, false);
+    for (int w = 0; w < waves; w++) {
+        if (w == wave) {
+            float keep = 0.f, add = 1.f, l = run.l, m = run.m;
+            if (w) {
+                const float m0 = x.m[col];
+                m = fmaxf(m0, run.m);
+                keep = m0 == m ? 1.f : __builtin_amdgcn_exp2f((m0 - m) * c);
+                add = run.m == m ? 1.f : __builtin_amdgcn_exp2f((run.m - m) * c);
+                l = x.l[col] * keep + run.l * add;
+            }
+#pragma unroll
+            for (int t = 0; t < D / 32; t++)
+#pragma unroll
+                for (int b = 0; b < 4; b++) {
+                    f32x4* at = (f32x4*)&x.o[col][t * 32 + 8 * b + 4 * h];
+                    f32x4 y = {run.o[t][4 * b], run.o[t][4 * b + 1], run.o[t][4 * b + 2], run.o[t][4 * b + 3]};
+                    y *= add;
+                    if (w) y += *at * keep;
+                    *at = y;
+                }
+            // both halves of the wave have read m and l of the column before either writes them (one wave, in order)
+            __builtin_amdgcn_wave_barrier();
+            if (h == 0) {
+                x.m[col] = m;
+                x.l[col] = l;
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Sums of one (row, part): D components, then m and l.  A part without keys has m = -inf, l = 0.
+template <int D> struct Part {
+    float o[D];
+    float m, l;
+    float pad[2];
+};
+
+template <class T, int D, int BN>
+__global__ __launch_bounds__(256, 2) void attention_split_kernel(AttentionLaunch a, AttnSets sets, int parts) {
+    using S = Shape<T, D>;
+    constexpr int SUB = BN / 32, IMG = BN * D * (int)sizeof(T);
+    __shared__ alignas(16) union {
+        char v[4][IMG];
+        Meeting<T, D> sums;
+    } lds;
+    const int units = sets.tile[sets.n] * parts, unit = xcd_unit(blockIdx.x, units);
+    if (unit >= units) return;
+    const int part = unit % parts, tile = unit / parts;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int s = find_set(sets.tile, sets.n, tile);
+    const int q0 = sets.q_off[s], k0 = sets.k_off[s], nk = sets.k_off[s + 1] - k0, kvh = a.k.heads, group = a.q.heads / kvh;
+    const int rows = (sets.q_off[s + 1] - q0) * group, tiles = (rows + 31) / 32;
+    const int g = (tile - sets.tile[s]) / tiles, row0 = ((tile - sets.tile[s]) % tiles) * 32;
+    u32x4 qf[S::NF];
+    load_query<T, D>(qf, a.q, row_place(row0 + (lane & 31), rows, group, g, q0), h);
+    const float c = a.scale * kLog2e, slack = 8.f / c;
+    Running<T, D> run;
+    run.clear();
+    const T* kp = (const T*)a.k.p + g * a.k.head + (long long)k0 * a.k.row;
+    const T* vp = (const T*)a.v.p + g * a.v.head + (long long)k0 * a.v.row;
+    const uint8_t* skip = a.skip ? a.skip + k0 : nullptr;
+    const long long nt = (nk + BN - 1) / BN;
+    const int from = (int)(nt * part / parts), to = (int)(nt * (part + 1) / parts);
+    OwnKeys<T, D, BN> keys;
+    if (from + wave < to) keys.load(kp, vp, a.k.row, a.v.row, skip, (from + wave) * BN, nk, lane);
+    for (int t = from + wave; t < to; t += 4) {
+        f32x16 sc[SUB];
+        keys.scores(sc, qf, lane);
+        keys.values_to_lds(lds.v[wave], lane);
+        if (t + 4 < to) keys.load(kp, vp, a.k.row, a.v.row, skip, (t + 4) * BN, nk, lane);
+        run.template weights<SUB>(sc, c, slack);
+        __builtin_amdgcn_wave_barrier();   // the image is this wave's own and LDS serves a wave in order
+#pragma unroll
+        for (int u = 0; u < SUB; u++) run.add_values(sc[u], lds.v[wave], u * 32, lane);
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    meet(lds.sums, run, c, wave, 4, lane);
+    // 32 rows x D components out, 4 per thread and round
+    for (int i = threadIdx.x; i < 32 * (D / 4); i += 256) {
+        const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+        if (row0 + r >= rows) continue;
+        const f32x4 y = *(const f32x4*)&lds.sums.o[r][d];
+        const RowPlace p = row_place(row0 + r, rows, group, g, q0);
+        const float m = lds.sums.m[r], l = lds.sums.l[r];
+        if (parts > 1) {
+            Part<D>& w = ((Part<D>*)a.work)[((p.q - sets.q_off[0]) * a.q.heads + p.head) * parts + part];
+            *(f32x4*)&w.o[d] = y;
+            if (d == 0) {
+                w.m = m;
+                w.l = l;
+            }
+            continue;
+        }
+        const float inv = inverse_sum(l);
+        T out[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) out[e] = (T)(inv == 0.f ? 0.f : y[e] * inv);
+        T* to_ = (T*)a.out.p + p.q * a.out.row + p.head * a.out.head + d;
+        if constexpr (IsF32<T>::v) *(f32x4*)to_ = __builtin_bit_cast(f32x4, out);
+        else *(s16x4*)to_ = __builtin_bit_cast(s16x4, out);
+        if (a.lse && d == 0) a.lse[p.q * a.q.heads + p.head] = log_sum(m, l, c);
+    }
+}
+
+// One thread per four components of a (row, head): the parts' sums in their order.
+template <class T, int D>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, AttnSets sets, int parts) {
+    constexpr int PER = D / 4;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, rh = i / PER;
+    const int d = (int)(i % PER) * 4;
+    if (rh >= ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads) return;
+    const float c = a.scale * kLog2e;
+    const Part<D>* w = (const Part<D>*)a.work + rh * parts;
+    float m = -INFINITY, l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int p = 0; p < parts; p++) m = fmaxf(m, w[p].m);
+    for (int p = 0; p < parts; p++) {
+        const float f = w[p].m == m ? 1.f : __builtin_amdgcn_exp2f((w[p].m - m) * c);
+        l += w[p].l * f;
+        o += *(const f32x4*)&w[p].o[d] * f;
+    }
+    const long long q = sets.q_off[0] + rh / a.q.heads;
+    const int head = (int)(rh % a.q.heads);
+    const float inv = inverse_sum(l);
+    T out[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) out[e] = (T)(inv == 0.f ? 0.f : o[e] * inv);
+    T* to = (T*)a.out.p + q * a.out.row + head * a.out.head + d;
+    if constexpr (IsF32<T>::v) *(f32x4*)to = __builtin_bit_cast(f32x4, out);
+    else *(s16x4*)to = __builtin_bit_cast(s16x4, out);
+    if (a.lse && d == 0) a.lse[q * a.q.heads + head] = log_sum(m, l, c);
+}
+
+// ---- which kernel ----
+namespace {
+
+struct DensePlan {
+    bool wide;
+    int parts;
+};
+constexpr int kFill = 512;   // work-groups that fill the chip (two per CU)
+
+// units of `rows` rows of the call into sets.tile
+int count_tiles(const AttentionLaunch& a, AttnSets& sets, int rows) {
+    const long long kvh = a.k.heads, group = a.q.heads / kvh;
+    sets.tile[0] = 0;
+    for (int s = 0; s < sets.n; s++)
+        sets.tile[s + 1] = sets.tile[s] + (int)(((sets.q_off[s + 1] - (long long)sets.q_off[s]) * group + rows - 1) / rows * kvh);
+    return sets.tile[sets.n];
+}
+DensePlan dense_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets) {
+    if (count_tiles(a, sets, 128) >= kFill) return {true, 1};
+    const int units = count_tiles(a, sets, 32);
+    long long longest = 0;
+    for (int s = 0; s < sets.n; s++) longest = std::max(longest, (long long)sets.k_off[s + 1] - sets.k_off[s]);
+    const int bn = dtype == PPG_F32 || head_dim == 128 ? 32 : 64;
+    // a part has a tile for each of its waves at least
+    const long long most = std::max(1LL, longest / (4 * bn));
+    return {false, (int)std::min<long long>(most, units ? (kFill + units - 1) / units : 1)};
+}
+
+template <class T, int D> hipError_t run_dense(const AttentionLaunch& a, AttnSets& sets, DensePlan p, hipStream_t s) {
+    constexpr int WIDE_BN = IsF32<T>::v ? 32 : 64, SPLIT_BN = IsF32<T>::v || D == 128 ? 32 : 64;
+    if (p.wide) {
+        attention_wide_kernel<T, D, WIDE_BN><<<xcd_grid(sets.tile[sets.n]), 256, 0, s>>>(a, sets);
+        return hipGetLastError();
+    }
+    attention_split_kernel<T, D, SPLIT_BN><<<xcd_grid(sets.tile[sets.n] * p.parts), 256, 0, s>>>(a, sets, p.parts);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.parts == 1) return e;
+    const long long n = ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads * (D / 4);
+    attention_join_kernel<T, D><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a, sets, p.parts);
+    return hipGetLastError();
+}
+template <class T> hipError_t run_dense_dim(int head_dim, const AttentionLaunch& a, AttnSets& sets, DensePlan p, hipStream_t s) {
+    return head_dim == 32 ? run_dense<T, 32>(a, sets, p, s) : head_dim == 64 ? run_dense<T, 64>(a, sets, p, s) : run_dense<T, 128>(a, sets, p, s);
+}
+
+}  // namespace
+
+size_t dense_work(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets) {
+    const DensePlan p = dense_plan(dtype, head_dim, a, sets);
+    return p.parts == 1 ? 0 : ((size_t)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads * p.parts * (head_dim + 4) * sizeof(float);
+}
+hipError_t launch_dense(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets, hipStream_t s) {
+    const DensePlan p = dense_plan(dtype, head_dim, a, sets);
+    if (!sets.tile[sets.n]) return hipSuccess;
+    return dtype == PPG_F32    ? run_dense_dim<float>(head_dim, a, sets, p, s)
+           : dtype == PPG_BF16 ? run_dense_dim<__bf16>(head_dim, a, sets, p, s)
+                               : run_dense_dim<_Float16>(head_dim, a, sets, p, s);
+}
+
+}  // namespace ppg

@@ -1,0 +1,173 @@
+// What the matrix-core attention kernels share: operand layouts, the running softmax, the two products of a tile.
+//
+// Scores are computed transposed, S^T = K Q^T, on v_mfma_f32_32x32x16 (16-bit types) or v_mfma_f32_32x32x2_f32: rows are 32
+// keys, columns 32 queries.  A lane then holds 16 scores of ONE query (column lane & 31; the other 16 are in lane ^ 32), so
+// maximum and sum need one exchange per tile, and the weights are already where the second product, O^T = V^T P^T, wants
+// its B operand: sum over keys in the order that the lanes hold them.  For that V's operand is read in the same order, with
+// the LDS read that transposes 16-bit numbers (four keys of one component per lane).
+#pragma once
+#include "attn_kernels.h"
+
+namespace ppg {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
+// the set whose [off[i], off[i+1]) holds x; off ascends, off[0] <= x < off[n]
+__device__ __forceinline__ int find_set(const int* off, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (off[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+template <class T> struct IsF32 { static constexpr bool v = false; };
+template <> struct IsF32<float> { static constexpr bool v = true; };
+
+// 16-byte chunks: N components each, CPR per row of D; a lane's operand for 32 rows is NF of them
+template <class T, int D> struct Shape {
+    static constexpr int N = 16 / (int)sizeof(T), CPR = D / N, NF = CPR / 2;
+    // chunk i of the operand of the lane half h: 16-bit: the 8 components that one MFMA wants from it; 32-bit: the two
+    // halves of a row belong to the two lane halves (any pairing of components serves, the same for both operands)
+    static __device__ __forceinline__ int chunk(int i, int h) { return IsF32<T>::v ? h * NF + i : 2 * i + h; }
+    // LDS images keep a row's chunks permuted so that what one access touches lies in different banks: the eight rows that
+    // the lanes of a 16-byte read take the same chunk of, and the four rows by two chunks of a transposing read
+    static __device__ __forceinline__ int swz_k(int row) { return CPR >= 8 ? row & 7 : (row >> 1) & 3; }
+    static __device__ __forceinline__ int swz_v(int row) {
+        if (IsF32<T>::v) return swz_k(row);
+        return CPR >= 8 ? ((row & 3) << 1) | ((row >> 2) & 1) : row & 2;
+    }
+};
+
+template <class T> __device__ __forceinline__ f32x16 mfma_chunk(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (IsF32<T>::v) {
+        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], c, 0, 0, 0);
+        return c;
+    } else if constexpr (__is_same(T, _Float16)) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+}
+
+// key of register r of a 32-key tile in the lane half h
+__device__ __forceinline__ int key_of(int r, int h) { return (r & 3) + 8 * (r >> 2) + 4 * h; }
+
+__device__ __forceinline__ float other_half(float x, bool take_max) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    const float lo = __uint_as_float(r[0]), hi = __uint_as_float(r[1]);
+    return take_max ? fmaxf(lo, hi) : lo + hi;
+}
+
+// Running softmax of the 32 queries of a wave, and their sums; m is the largest product seen (or up to 2^8 less in the
+// exponent: the sums are rescaled only when a product passes it by that much, which any type holds), c = scale * log2 e.
+template <class T, int D> struct Running {
+    using S = Shape<T, D>;
+    f32x16 o[D / 32];
+    float m, l;
+    __device__ __forceinline__ void clear() {
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int t = 0; t < D / 32; t++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[t][r] = 0.f;
+    }
+    // scores of 32 * SUB keys against the wave's queries: weights instead of them
+    template <int SUB> __device__ __forceinline__ void weights(f32x16 (&s)[SUB], float c, float slack) {
+        float mt = s[0][0];
+#pragma unroll
+        for (int u = 0; u < SUB; u++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) mt = fmaxf(mt, s[u][r]);
+        mt = other_half(mt, true);
+        const bool up = mt > m + slack;
+        if (__any(up)) {
+            const float mn = up ? mt : m;
+            const float alpha = mn == m ? 1.f : __builtin_amdgcn_exp2f((m - mn) * c);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int t = 0; t < D / 32; t++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) o[t][r] *= alpha;
+        }
+        const float mc = m == -INFINITY ? 0.f : m * c;   // nothing so far: every weight below is exp2(-inf)
+        float sum = 0.f;
+#pragma unroll
+        for (int u = 0; u < SUB; u++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], c, -mc));
+                sum += s[u][r];
+            }
+        l += sum;   // of this lane's half of the keys; the halves meet at the end
+    }
+    // o += P V for 32 keys; v: LDS image of the values, key0 their first row in it
+    __device__ __forceinline__ void add_values(const f32x16& p, const char* v, int key0, int lane) {
+        const int h = lane >> 5;
+        if constexpr (IsF32<T>::v) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int row = key0 + key_of(r, h);
+#pragma unroll
+                for (int t = 0; t < D / 32; t++) {
+                    const int d = t * 32 + (lane & 31);
+                    const float a = *(const float*)(v + row * (D * 4) + ((((d >> 2) ^ S::swz_v(row)) << 4) | ((d & 3) << 2)));
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], o[t], 0, 0, 0);
+                }
+            }
+        } else {
+            const int i = lane & 15, part = (lane >> 4) & 1;
+#pragma unroll
+            for (int st = 0; st < 2; st++) {
+                T pb[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) pb[e] = (T)p[8 * st + e];   // the weights' one rounding
+                const u32x4 b = __builtin_bit_cast(u32x4, pb);
+                const int r0 = key0 + 16 * st + 4 * h + (i >> 2), r1 = r0 + 8;
+#pragma unroll
+                for (int t = 0; t < D / 32; t++) {
+                    const int ch = t * 4 + part * 2 + ((i & 3) >> 1), in = (i & 1) * 8;
+                    const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(v + r0 * (D * 2) + ((ch ^ S::swz_v(r0)) << 4) + in));
+                    const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(v + r1 * (D * 2) + ((ch ^ S::swz_v(r1)) << 4) + in));
+                    const s16x8 a = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+                    o[t] = mfma_chunk<T>(__builtin_bit_cast(u32x4, a), b, o[t]);
+                }
+            }
+        }
+    }
+};
+
+// scores of masked keys (bit set in `dead`, bit 0 = the tile's first key) become -inf, whatever the product gave
+__device__ __forceinline__ void mask_scores(f32x16& s, unsigned dead, int h) {
+    const int d = (int)(dead >> (4 * h));
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+        const unsigned x = (unsigned)((d << (31 - key_of(r, 0))) >> 31);   // all ones where masked
+        s[r] = __uint_as_float((__float_as_uint(s[r]) & ~x) | (0xff800000u & x));
+    }
+}
+
+// work-group L of a launch of n units: XCD L % 8 (launch order) serves a contiguous range of the units, so that the units that
+// read the same keys meet in one L2; n or more: nothing to do
+__device__ __forceinline__ int xcd_unit(int L, int n) {
+    const int per = (n + 7) >> 3;
+    const int u = (L & 7) * per + (L >> 3);
+    return (L >> 3) < per ? u : n;
+}
+__host__ __device__ inline unsigned xcd_grid(int n) { return 8u * (unsigned)((n + 7) >> 3); }
+
+}  // namespace ppg

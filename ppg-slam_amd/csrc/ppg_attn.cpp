@@ -81,6 +81,8 @@ int attention_checked(ppg_ctx* c, const ppg_attention_args* a, bool sizes_only, 
     if ((rc = set_offsets(c, who, a->n_sets, a->q_off, "q_off", sets.q_off))) return rc;
     if ((rc = set_offsets(c, who, a->n_sets, a->k_off, "k_off", sets.k_off))) return rc;
     const long long nq = (long long)sets.q_off[sets.n] - sets.q_off[0], nk = (long long)sets.k_off[sets.n] - sets.k_off[0];
+    if (nq * a->q.heads >= (1LL << 31) || nk * a->k.heads >= (1LL << 31))
+        return fail(c, PPG_ECAP, "%s: rows times heads must stay below 2^31", who);
     const ppg_rows* r[4] = {&a->q, &a->k, &a->v, &a->out};
     static const char* name[4] = {"q", "k", "v", "out"};
     for (int i = 0; i < 4; i++) {

@@ -52,10 +52,6 @@ struct AttentionLaunch {
     const int32_t* sel;
     void* work;
 };
-// over whole sets (attn_mfma.hip)
-size_t dense_work(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets);
-hipError_t launch_dense(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets, hipStream_t s);
-// either
 size_t attention_work(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets);
 hipError_t launch_attention(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets, hipStream_t s);
 

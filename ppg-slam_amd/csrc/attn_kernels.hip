@@ -1,10 +1,7 @@
-// Attention between descriptor sets on gfx950: rotary positions, block means, block selection, attention over whole sets
-// or over selected blocks.  Sums, softmax statistics and means are held in 32 bits or more; what is stored in fewer bits is
-// rounded once, to nearest even.
+// What stands around the attention between descriptor sets (attn_mfma.hip): rotary positions, block means, block selection.
+// Sums are held in 32 bits or more; what is stored in fewer bits is rounded once, to nearest even.
 #include "attn_tile.h"
 #include "wave_util.h"
-
-#include <algorithm>
 
 namespace ppg {
 
@@ -154,78 +151,6 @@ __global__ __launch_bounds__(256) void block_select_kernel(BlockSelectLaunch a, 
     if (lane < a.n_sel) a.sel[((long long)r * a.kv_heads + g) * a.n_sel + lane] = out.idx == 0x7fffffff ? -1 : out.idx;
 }
 
-// ---- attention, one wave per (query row, head) ----
-// 64 keys at a time: a lane's product with its key, the running maximum and sum of the softmax, then the weighted values
-// with a lane per component.
-template <class T, int D>
-__global__ __launch_bounds__(256) void attention_row_kernel(AttentionLaunch a, AttnSets sets) {
-    constexpr int N = 16 / sizeof(T), DL = (D + 63) / 64;
-    __shared__ float qs[4][D];
-    __shared__ float ps[4][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const long long unit = (long long)blockIdx.x * 4 + w, rows = sets.q_off[sets.n] - sets.q_off[0];
-    const bool live = unit < rows * a.q.heads;
-    const int r = sets.q_off[0] + (int)((live ? unit : 0) / a.q.heads), h = (int)((live ? unit : 0) % a.q.heads);
-    const int g = h / (a.q.heads / a.k.heads);
-    for (int d = lane; d < D; d += 64) qs[w][d] = to_float(((const T*)a.q.p)[(long long)r * a.q.row + h * a.q.head + d]);
-    __syncthreads();
-    if (!live) return;
-    const int s = find_set(sets.q_off, sets.n, r), k0 = sets.k_off[s], nk = sets.k_off[s + 1] - k0;
-    const T* kp = (const T*)a.k.p + g * a.k.head;
-    const T* vp = (const T*)a.v.p + g * a.v.head;
-    const float scale = a.scale * 1.44269504088896340736f;
-    float m = -INFINITY, l = 0.f, o[DL] = {};
-    const int* sel = a.sel ? a.sel + ((long long)r * a.k.heads + g) * a.n_sel : nullptr;
-    const int ranges = sel ? a.n_sel : 1;
-    for (int i = 0; i < ranges; i++) {
-        int from = 0, to = nk;
-        if (sel) {
-            const int b = sel[i];
-            if (b < 0 || b >= (nk + a.block - 1) / a.block) continue;
-            from = b * a.block;
-            to = min(from + a.block, nk);
-        }
-        for (int c = from; c < to; c += 64) {
-            const int j = c + lane;
-            const bool on = j < to && !(a.skip && a.skip[k0 + j]);
-            float x = -INFINITY;
-            if (on) {
-                float dot = 0.f;
-                const Vec16<T>* row = (const Vec16<T>*)(kp + (long long)(k0 + j) * a.k.row);
-#pragma unroll
-                for (int v = 0; v < D / N; v++) {
-                    const Vec16<T> t = row[v];
-#pragma unroll
-                    for (int e = 0; e < N; e++) dot = fmaf(qs[w][v * N + e], to_float(t.v[e]), dot);
-                }
-                x = dot * scale;
-            }
-            const float mn = fmaxf(m, wave_max(x)), safe = mn == -INFINITY ? 0.f : mn;
-            const float alpha = exp2f(m - safe), p = x != x ? x : exp2f(x - safe);
-            l = l * alpha + wave_sum(p);
-            m = mn;
-            ps[w][lane] = p;
-#pragma unroll
-            for (int e = 0; e < DL; e++) o[e] *= alpha;
-            __builtin_amdgcn_wave_barrier();
-            for (unsigned long long left = __ballot(on); left; left &= left - 1) {
-                const int q = __builtin_ctzll(left);
-                const T* row = vp + (long long)(k0 + c + q) * a.v.row;
-                const float pw = ps[w][q];
-#pragma unroll
-                for (int e = 0; e < DL; e++)
-                    if (D >= 64 || lane < D) o[e] = fmaf(pw, to_float(row[e * 64 + lane]), o[e]);
-            }
-            __builtin_amdgcn_wave_barrier();
-        }
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int e = 0; e < DL; e++)
-        if (D >= 64 || lane < D) ((T*)a.out.p)[(long long)r * a.out.row + h * a.out.head + e * 64 + lane] = (T)(l == 0.f ? 0.f : o[e] * inv);
-    if (a.lse && lane == 0) a.lse[(long long)r * a.q.heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
-}
-
 // ---- launches ----
 #define BY_TYPE(dtype, CALL)                   \
     do {                                       \
@@ -233,13 +158,6 @@ __global__ __launch_bounds__(256) void attention_row_kernel(AttentionLaunch a, A
         else if (dtype == PPG_BF16) { using T = __bf16; CALL; } \
         else { using T = _Float16; CALL; }     \
     } while (0)
-#define BY_DIM(dim, CALL)                                     \
-    do {                                                      \
-        if (dim == 32) { constexpr int D = 32; CALL; }        \
-        else if (dim == 64) { constexpr int D = 64; CALL; }   \
-        else { constexpr int D = 128; CALL; }                 \
-    } while (0)
-
 hipError_t launch_rotary(int dtype, const RotaryLaunch& a, hipStream_t s) {
     const long long per_head = a.rot_dim / 2 + (a.head_dim - a.rot_dim);
     const long long u0 = a.n_rows[0] ? a.n_rows[0] * (long long)a.src[0].heads * per_head : 0;
@@ -261,16 +179,6 @@ hipError_t launch_block_select(int dtype, int head_dim, const BlockSelectLaunch&
     const long long units = ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.kv_heads;
     if (!units) return hipSuccess;
     BY_TYPE(dtype, (block_select_kernel<T><<<(unsigned)((units + 3) / 4), 256, 0, s>>>(a, sets, head_dim)));
-    return hipGetLastError();
-}
-
-size_t attention_work(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets) { return a.n_sel ? 0 : dense_work(dtype, head_dim, a, sets); }
-
-hipError_t launch_attention(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets, hipStream_t s) {
-    if (!a.sel) return launch_dense(dtype, head_dim, a, sets, s);
-    const long long units = ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads;
-    if (!units) return hipSuccess;
-    BY_TYPE(dtype, BY_DIM(head_dim, (attention_row_kernel<T, D><<<(unsigned)((units + 3) / 4), 256, 0, s>>>(a, sets))));
     return hipGetLastError();
 }
 

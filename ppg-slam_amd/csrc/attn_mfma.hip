@@ -1,10 +1,14 @@
-// Attention over whole sets on the matrix cores (layouts and softmax in attn_tile.h).
+// Attention on the matrix cores, over whole sets or over selected blocks (layouts and softmax in attn_tile.h).
 //
 // Rows: the queries of the `group` heads that share a key head are one long list, row r = query r / group, head r % group.
 //   attention_wide_kernel  four waves of 32 rows each share the key and value tiles in LDS (two stages: the next tile's
 //                          loads are in flight in registers while this one is multiplied);
 //   attention_split_kernel 32 rows per work-group, its four waves (and, where rows are few, several work-groups) share out the
 //                          keys; sums meet in LDS, and those of several work-groups in attention_join_kernel.
+// Selected blocks, few queries: attention_split_kernel too, the listed blocks of ONE query as its keys.
+// Selected blocks, many queries: the lists are turned round (bin_kernel: for every block the queries that name it), so that a
+// block's keys and values are read once for all of them (attention_blocks_kernel, a wave per block and 32 rows), and every
+// (query, place in its list) leaves its sums for attention_join_kernel.
 #include "attn_tile.h"
 
 #include <algorithm>
@@ -216,7 +220,8 @@ template <int D> struct Part {
     float pad[2];
 };
 
-template <class T, int D, int BN>
+// SEL: a unit's rows are the group of one query, its keys the blocks of that query's list.
+template <class T, int D, int BN, bool SEL>
 __global__ __launch_bounds__(256, 2) void attention_split_kernel(AttentionLaunch a, AttnSets sets, int parts) {
     using S = Shape<T, D>;
     constexpr int SUB = BN / 32, IMG = BN * D * (int)sizeof(T);
@@ -230,8 +235,11 @@ __global__ __launch_bounds__(256, 2) void attention_split_kernel(AttentionLaunch
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
     const int s = find_set(sets.tile, sets.n, tile);
     const int q0 = sets.q_off[s], k0 = sets.k_off[s], nk = sets.k_off[s + 1] - k0, kvh = a.k.heads, group = a.q.heads / kvh;
-    const int rows = (sets.q_off[s + 1] - q0) * group, tiles = (rows + 31) / 32;
-    const int g = (tile - sets.tile[s]) / tiles, row0 = ((tile - sets.tile[s]) % tiles) * 32;
+    // SEL: tiles of a query's group never hold rows of another query
+    const int nq = sets.q_off[s + 1] - q0, all = nq * group, per_q = (group + 31) / 32, tiles = SEL ? nq * per_q : (all + 31) / 32;
+    const int g = (tile - sets.tile[s]) / tiles, at = (tile - sets.tile[s]) % tiles;
+    const int row0 = SEL ? at / per_q * group + at % per_q * 32 : at * 32;
+    const int rows = SEL ? (at / per_q + 1) * group : all;
     u32x4 qf[S::NF];
     load_query<T, D>(qf, a.q, row_place(row0 + (lane & 31), rows, group, g, q0), h);
     const float c = a.scale * kLog2e, slack = 8.f / c;
@@ -240,15 +248,28 @@ __global__ __launch_bounds__(256, 2) void attention_split_kernel(AttentionLaunch
     const T* kp = (const T*)a.k.p + g * a.k.head + (long long)k0 * a.k.row;
     const T* vp = (const T*)a.v.p + g * a.v.head + (long long)k0 * a.v.row;
     const uint8_t* skip = a.skip ? a.skip + k0 : nullptr;
-    const long long nt = (nk + BN - 1) / BN;
+    const int* sel = SEL ? a.sel + ((long long)(q0 + at / per_q) * kvh + g) * a.n_sel : nullptr;
+    const int per_block = SEL ? (a.block + BN - 1) / BN : 1, blocks = SEL ? (nk + a.block - 1) / a.block : 0;
+    const long long nt = SEL ? (nk ? (long long)a.n_sel * per_block : 0) : (nk + BN - 1) / BN;
     const int from = (int)(nt * part / parts), to = (int)(nt * (part + 1) / parts);
     OwnKeys<T, D, BN> keys;
-    if (from + wave < to) keys.load(kp, vp, a.k.row, a.v.row, skip, (from + wave) * BN, nk, lane);
+    auto load = [&](int t) {
+        if constexpr (SEL) {
+            const int b = sel[t / per_block], j = t % per_block * BN;
+            const bool ok = b >= 0 && b < blocks;
+            const int first = ok ? b * a.block : 0, n = min(a.block, nk - first);
+            keys.load(kp + first * a.k.row, vp + first * a.v.row, a.k.row, a.v.row, skip ? skip + first : nullptr, j, n, lane);
+            if (!ok) keys.gone = ~0ull;
+        } else {
+            keys.load(kp, vp, a.k.row, a.v.row, skip, t * BN, nk, lane);
+        }
+    };
+    if (from + wave < to) load(from + wave);
     for (int t = from + wave; t < to; t += 4) {
         f32x16 sc[SUB];
         keys.scores(sc, qf, lane);
         keys.values_to_lds(lds.v[wave], lane);
-        if (t + 4 < to) keys.load(kp, vp, a.k.row, a.v.row, skip, (t + 4) * BN, nk, lane);
+        if (t + 4 < to) load(t + 4);
         run.template weights<SUB>(sc, c, slack);
         __builtin_amdgcn_wave_barrier();   // the image is this wave's own and LDS serves a wave in order
 #pragma unroll
@@ -284,8 +305,9 @@ __global__ __launch_bounds__(256, 2) void attention_split_kernel(AttentionLaunch
     }
 }
 
-// One thread per four components of a (row, head): the parts' sums in their order.
-template <class T, int D>
+// One thread per four components of a (row, head): the parts' sums in their order.  SEL: part i belongs to place i of the
+// query's list and exists only if that names a block.
+template <class T, int D, bool SEL>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, AttnSets sets, int parts) {
     constexpr int PER = D / 4;
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x, rh = i / PER;
@@ -293,16 +315,25 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, 
     if (rh >= ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads) return;
     const float c = a.scale * kLog2e;
     const Part<D>* w = (const Part<D>*)a.work + rh * parts;
+    const long long q = sets.q_off[0] + rh / a.q.heads;
+    const int head = (int)(rh % a.q.heads);
+    unsigned long long use = ~0ull;
+    if constexpr (SEL) {
+        const int s = find_set(sets.q_off, sets.n, (int)q), blocks = sets.blk[s + 1] - sets.blk[s];
+        const int* sel = a.sel + (q * a.k.heads + head / (a.q.heads / a.k.heads)) * a.n_sel;
+        use = 0;
+        for (int p = 0; p < parts; p++) use |= (unsigned long long)(sel[p] >= 0 && sel[p] < blocks) << p;
+    }
     float m = -INFINITY, l = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int p = 0; p < parts; p++) m = fmaxf(m, w[p].m);
+    for (int p = 0; p < parts; p++)
+        if (!SEL || (use >> p) & 1) m = fmaxf(m, w[p].m);
     for (int p = 0; p < parts; p++) {
+        if (SEL && !((use >> p) & 1)) continue;
         const float f = w[p].m == m ? 1.f : __builtin_amdgcn_exp2f((w[p].m - m) * c);
         l += w[p].l * f;
         o += *(const f32x4*)&w[p].o[d] * f;
     }
-    const long long q = sets.q_off[0] + rh / a.q.heads;
-    const int head = (int)(rh % a.q.heads);
     const float inv = inverse_sum(l);
     T out[4];
 #pragma unroll
@@ -311,6 +342,139 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, 
     if constexpr (IsF32<T>::v) *(f32x4*)to = __builtin_bit_cast(f32x4, out);
     else *(s16x4*)to = __builtin_bit_cast(s16x4, out);
     if (a.lse && d == 0) a.lse[q * a.q.heads + head] = log_sum(m, l, c);
+}
+
+// ---- selected blocks, many queries ----
+// A region is one (set, key head); entry e of it is place e % n_sel in the list of its query e / n_sel.  Where things lie:
+struct BinWork {
+    int* list;     // entries by block, [regions][queries of the set * n_sel]
+    int4* tile;    // (block, first entry in the region's list, rows of the block = entries * group, first row of the tile)
+    int* tiles;    // tiles of a region
+};
+// tiles that a region may need: its rows in 32s, and one more for every block's last
+__host__ __device__ inline int region_tiles(long long nq, int n_sel, int group, int blocks) {
+    const long long e = nq * n_sel;
+    return (int)(e * group / 32 + (e < blocks ? e : blocks));
+}
+
+// One work-group per region: counts per block, their running sum, and the entries put in their places.  Which entry of a block
+// comes first is left to the atomics: entries of a block never meet in a sum.
+constexpr int kBins = 8192;   // blocks counted at a time (32 KB of LDS)
+__global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets sets, BinWork w) {
+    __shared__ int cnt[kBins];
+    __shared__ int sum_e[16], sum_t[16];
+    const int kvh = a.k.heads, group = a.q.heads / kvh, s = blockIdx.x / kvh, g = blockIdx.x % kvh;
+    const int q0 = sets.q_off[s], nq = sets.q_off[s + 1] - q0, blocks = sets.blk[s + 1] - sets.blk[s], n = nq * a.n_sel;
+    const int* sel = a.sel + ((long long)q0 * kvh + g) * a.n_sel;
+    int* list = w.list + ((long long)(q0 - sets.q_off[0]) * kvh + (long long)g * nq) * a.n_sel;
+    int4* tile = w.tile + sets.tile[s] + (long long)g * region_tiles(nq, a.n_sel, group, blocks);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int e0 = 0, t0 = 0;   // entries and tiles of the bins before this round's
+    for (int b0 = 0; b0 < blocks; b0 += kBins) {
+        const int nb = min(kBins, blocks - b0), per = (nb + 1023) / 1024;
+        for (int i = tid; i < nb; i += 1024) cnt[i] = 0;
+        __syncthreads();
+        for (int e = tid; e < n; e += 1024) {
+            const int b = sel[(long long)(e / a.n_sel) * kvh * a.n_sel + e % a.n_sel] - b0;
+            if (b >= 0 && b < nb) atomicAdd(&cnt[b], 1);
+        }
+        __syncthreads();
+        int es = 0, ts = 0;
+        for (int i = tid * per; i < min(nb, (tid + 1) * per); i++) {
+            es += cnt[i];
+            ts += (cnt[i] * group + 31) / 32;
+        }
+        int ei = es, ti = ts;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int x = __shfl_up(ei, d), y = __shfl_up(ti, d);
+            if (lane >= d) {
+                ei += x;
+                ti += y;
+            }
+        }
+        if (lane == 63) {
+            sum_e[wave] = ei;
+            sum_t[wave] = ti;
+        }
+        __syncthreads();
+        int eb = e0 + ei - es, tb = t0 + ti - ts;
+        for (int i = 0; i < 16; i++) {
+            if (i < wave) {
+                eb += sum_e[i];
+                tb += sum_t[i];
+            }
+            e0 += sum_e[i];
+            t0 += sum_t[i];
+        }
+        for (int i = tid * per; i < min(nb, (tid + 1) * per); i++) {
+            const int c = cnt[i], rows = c * group;
+            for (int r = 0; r < rows; r += 32) tile[tb++] = make_int4(b0 + i, eb, rows, r);
+            cnt[i] = eb;   // where the block's next entry goes
+            eb += c;
+        }
+        __syncthreads();
+        for (int e = tid; e < n; e += 1024) {
+            const int b = sel[(long long)(e / a.n_sel) * kvh * a.n_sel + e % a.n_sel] - b0;
+            if (b >= 0 && b < nb) list[atomicAdd(&cnt[b], 1)] = e;
+        }
+        __syncthreads();
+    }
+    if (tid == 0) w.tiles[blockIdx.x] = t0;
+}
+
+// A wave per tile: one block's keys against 32 rows out of the queries that name it.
+template <class T, int D, int BN>
+__global__ __launch_bounds__(256, 2) void attention_blocks_kernel(AttentionLaunch a, AttnSets sets, BinWork w) {
+    using S = Shape<T, D>;
+    constexpr int SUB = BN / 32, IMG = BN * D * (int)sizeof(T);
+    __shared__ alignas(16) char lds_v[4][IMG];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int at = __builtin_amdgcn_readfirstlane(xcd_unit(blockIdx.x, (sets.tile[sets.n] + 3) / 4) * 4 + wave);
+    if (at >= sets.tile[sets.n]) return;   // waves share nothing here: each may leave by itself
+    const int s = find_set(sets.tile, sets.n, at), kvh = a.k.heads, group = a.q.heads / kvh;
+    const int q0 = sets.q_off[s], nq = sets.q_off[s + 1] - q0, k0 = sets.k_off[s], nk = sets.k_off[s + 1] - k0;
+    const int cap = region_tiles(nq, a.n_sel, group, sets.blk[s + 1] - sets.blk[s]);
+    const int g = (at - sets.tile[s]) / cap, i = (at - sets.tile[s]) % cap;
+    if (i >= w.tiles[s * kvh + g]) return;
+    const int4 t = w.tile[at];
+    const int first = t.x * a.block, n = min(a.block, nk - first);
+    const T* kp = (const T*)a.k.p + g * a.k.head + (long long)(k0 + first) * a.k.row;
+    const T* vp = (const T*)a.v.p + g * a.v.head + (long long)(k0 + first) * a.v.row;
+    const uint8_t* skip = a.skip ? a.skip + k0 + first : nullptr;
+    OwnKeys<T, D, BN> keys;
+    keys.load(kp, vp, a.k.row, a.v.row, skip, 0, n, lane);
+    const int row = t.w + (lane & 31), rr = min(row, t.z - 1);
+    const int entry = w.list[((long long)(q0 - sets.q_off[0]) * kvh + (long long)g * nq) * a.n_sel + t.y + (group == 1 ? rr : rr / group)];
+    const long long q = q0 + entry / a.n_sel;
+    const int slot = entry % a.n_sel, head = g * group + (group == 1 ? 0 : rr % group);
+    u32x4 qf[S::NF];
+    load_query<T, D>(qf, a.q, RowPlace{q, head}, h);
+    const float c = a.scale * kLog2e, slack = 8.f / c;
+    Running<T, D> run;
+    run.clear();
+    for (int j = 0; j < n; j += BN) {
+        f32x16 sc[SUB];
+        keys.scores(sc, qf, lane);
+        keys.values_to_lds(lds_v[wave], lane);
+        if (j + BN < n) keys.load(kp, vp, a.k.row, a.v.row, skip, j + BN, n, lane);
+        run.template weights<SUB>(sc, c, slack);
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int u = 0; u < SUB; u++) run.add_values(sc[u], lds_v[wave], u * 32, lane);
+        __builtin_amdgcn_wave_barrier();
+    }
+    if (row >= t.z) return;
+    const float l = other_half(run.l, false);
+    Part<D>& to = ((Part<D>*)a.work)[((q - sets.q_off[0]) * a.q.heads + head) * a.n_sel + slot];
+#pragma unroll
+    for (int u = 0; u < D / 32; u++)
+#pragma unroll
+        for (int b = 0; b < 4; b++) *(f32x4*)&to.o[u * 32 + 8 * b + 4 * h] = f32x4{run.o[u][4 * b], run.o[u][4 * b + 1], run.o[u][4 * b + 2], run.o[u][4 * b + 3]};
+    if (h == 0) {
+        to.m = run.m;
+        to.l = l;
+    }
 }
 
 // ---- which kernel ----
@@ -341,35 +505,98 @@ DensePlan dense_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSets
     return {false, (int)std::min<long long>(most, units ? (kFill + units - 1) / units : 1)};
 }
 
-template <class T, int D> hipError_t run_dense(const AttentionLaunch& a, AttnSets& sets, DensePlan p, hipStream_t s) {
-    constexpr int WIDE_BN = IsF32<T>::v ? 32 : 64, SPLIT_BN = IsF32<T>::v || D == 128 ? 32 : 64;
+
+// selected blocks
+struct BlocksPlan {
+    bool binned;
+    int parts;
+    size_t part_bytes, list_bytes, tile_bytes, tiles_bytes;   // of the binned form, in this order
+};
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+// Below this many list entries a query's blocks are read for itself: one launch instead of three
+constexpr long long kBinnedFrom = 512;
+BlocksPlan blocks_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets) {
+    const long long nq = (long long)sets.q_off[sets.n] - sets.q_off[0], kvh = a.k.heads, group = a.q.heads / kvh;
+    const size_t part = (size_t)(head_dim + 4) * sizeof(float);
+    BlocksPlan p{};
+    sets.tile[0] = 0;
+    if (nq * kvh * a.n_sel >= kBinnedFrom) {
+        p.binned = true;
+        p.parts = a.n_sel;
+        for (int s = 0; s < sets.n; s++)
+            sets.tile[s + 1] = sets.tile[s] + (int)kvh * region_tiles(sets.q_off[s + 1] - sets.q_off[s], a.n_sel, (int)group, sets.blk[s + 1] - sets.blk[s]);
+        p.part_bytes = up256((size_t)nq * a.q.heads * a.n_sel * part);
+        p.list_bytes = up256((size_t)nq * kvh * a.n_sel * sizeof(int));
+        p.tile_bytes = up256((size_t)sets.tile[sets.n] * sizeof(int4));
+        p.tiles_bytes = up256((size_t)sets.n * kvh * sizeof(int));
+        return p;
+    }
+    const long long per_q = (group + 31) / 32;
+    for (int s = 0; s < sets.n; s++) sets.tile[s + 1] = sets.tile[s] + (int)((sets.q_off[s + 1] - sets.q_off[s]) * per_q * kvh);
+    const int units = sets.tile[sets.n], bn = dtype == PPG_F32 || head_dim == 128 ? 32 : 64;
+    const long long most = std::max(1LL, (long long)a.n_sel * ((a.block + bn - 1) / bn) / 4);
+    p.parts = (int)std::min<long long>(most, units ? (kFill + units - 1) / units : 1);
+    if (p.parts > 1) p.part_bytes = (size_t)nq * a.q.heads * p.parts * part;
+    return p;
+}
+
+template <class T, int D> hipError_t join(const AttentionLaunch& a, AttnSets& sets, int parts, bool by_list, hipStream_t s) {
+    const long long n = ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads * (D / 4);
+    if (by_list) attention_join_kernel<T, D, true><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a, sets, parts);
+    else attention_join_kernel<T, D, false><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a, sets, parts);
+    return hipGetLastError();
+}
+template <class T, int D> hipError_t run(const AttentionLaunch& a, AttnSets& sets, int dtype, hipStream_t s) {
+    constexpr int WIDE_BN = IsF32<T>::v ? 32 : 64, OWN_BN = IsF32<T>::v || D == 128 ? 32 : 64;
+    hipError_t e;
+    if (a.sel) {
+        const BlocksPlan p = blocks_plan(dtype, D, a, sets);
+        if (!sets.tile[sets.n] && !p.binned) return hipSuccess;
+        if (!p.binned) {
+            attention_split_kernel<T, D, OWN_BN, true><<<xcd_grid(sets.tile[sets.n] * p.parts), 256, 0, s>>>(a, sets, p.parts);
+            e = hipGetLastError();
+            return e != hipSuccess || p.parts == 1 ? e : join<T, D>(a, sets, p.parts, false, s);
+        }
+        BinWork w;
+        w.list = (int*)((char*)a.work + p.part_bytes);
+        w.tile = (int4*)((char*)w.list + p.list_bytes);
+        w.tiles = (int*)((char*)w.tile + p.tile_bytes);
+        if (sets.tile[sets.n]) {
+            bin_kernel<<<sets.n * a.k.heads, 1024, 0, s>>>(a, sets, w);
+            if ((e = hipGetLastError()) != hipSuccess) return e;
+            attention_blocks_kernel<T, D, OWN_BN><<<xcd_grid((sets.tile[sets.n] + 3) / 4), 256, 0, s>>>(a, sets, w);
+            if ((e = hipGetLastError()) != hipSuccess) return e;
+        }
+        return join<T, D>(a, sets, p.parts, true, s);
+    }
+    const DensePlan p = dense_plan(dtype, D, a, sets);
+    if (!sets.tile[sets.n]) return hipSuccess;
     if (p.wide) {
         attention_wide_kernel<T, D, WIDE_BN><<<xcd_grid(sets.tile[sets.n]), 256, 0, s>>>(a, sets);
         return hipGetLastError();
     }
-    attention_split_kernel<T, D, SPLIT_BN><<<xcd_grid(sets.tile[sets.n] * p.parts), 256, 0, s>>>(a, sets, p.parts);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.parts == 1) return e;
-    const long long n = ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads * (D / 4);
-    attention_join_kernel<T, D><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a, sets, p.parts);
-    return hipGetLastError();
+    attention_split_kernel<T, D, OWN_BN, false><<<xcd_grid(sets.tile[sets.n] * p.parts), 256, 0, s>>>(a, sets, p.parts);
+    e = hipGetLastError();
+    return e != hipSuccess || p.parts == 1 ? e : join<T, D>(a, sets, p.parts, false, s);
 }
-template <class T> hipError_t run_dense_dim(int head_dim, const AttentionLaunch& a, AttnSets& sets, DensePlan p, hipStream_t s) {
-    return head_dim == 32 ? run_dense<T, 32>(a, sets, p, s) : head_dim == 64 ? run_dense<T, 64>(a, sets, p, s) : run_dense<T, 128>(a, sets, p, s);
+template <class T> hipError_t run_dim(const AttentionLaunch& a, AttnSets& sets, int dtype, int head_dim, hipStream_t s) {
+    return head_dim == 32 ? run<T, 32>(a, sets, dtype, s) : head_dim == 64 ? run<T, 64>(a, sets, dtype, s) : run<T, 128>(a, sets, dtype, s);
 }
 
 }  // namespace
 
-size_t dense_work(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets) {
+size_t attention_work(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets) {
+    if (a.n_sel) {
+        const BlocksPlan p = blocks_plan(dtype, head_dim, a, sets);
+        return p.part_bytes + p.list_bytes + p.tile_bytes + p.tiles_bytes;
+    }
     const DensePlan p = dense_plan(dtype, head_dim, a, sets);
     return p.parts == 1 ? 0 : ((size_t)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads * p.parts * (head_dim + 4) * sizeof(float);
 }
-hipError_t launch_dense(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets, hipStream_t s) {
-    const DensePlan p = dense_plan(dtype, head_dim, a, sets);
-    if (!sets.tile[sets.n]) return hipSuccess;
-    return dtype == PPG_F32    ? run_dense_dim<float>(head_dim, a, sets, p, s)
-           : dtype == PPG_BF16 ? run_dense_dim<__bf16>(head_dim, a, sets, p, s)
-                               : run_dense_dim<_Float16>(head_dim, a, sets, p, s);
+hipError_t launch_attention(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets, hipStream_t s) {
+    return dtype == PPG_F32    ? run_dim<float>(a, sets, dtype, head_dim, s)
+           : dtype == PPG_BF16 ? run_dim<__bf16>(a, sets, dtype, head_dim, s)
+                               : run_dim<_Float16>(a, sets, dtype, head_dim, s);
 }
 
 }  // namespace ppg

@@ -98,6 +98,7 @@ int attention_checked(ppg_ctx* c, const ppg_attention_args* a, bool sizes_only, 
         if (!known_block(a->block)) return fail(c, PPG_EINVAL, "%s: block %d (32, 64 and 128 are built)", who, a->block);
         if (a->n_sel < 1) return fail(c, PPG_EINVAL, "%s: n_sel must be at least 1", who);
         if (a->n_sel > PPG_ATTN_MAX_SEL) return fail(c, PPG_ECAP, "%s: n_sel %d, at most %d", who, a->n_sel, PPG_ATTN_MAX_SEL);
+        if (nq * a->q.heads * a->n_sel >= (1LL << 30)) return fail(c, PPG_ECAP, "%s: rows times heads times n_sel must stay below 2^30", who);
         if (!a->sel && !sizes_only && nq) return fail(c, PPG_EINVAL, "%s: block or n_sel is set and sel is NULL", who);
         block_offsets(sets, a->block);
     }

@@ -24,53 +24,156 @@ __device__ __forceinline__ void cos_sin_turns(double turns, float& c, float& s) 
 }
 
 // ---- rotary positions ----
-// One thread per pair, and per component that is only copied.
-template <class T>
-__global__ __launch_bounds__(256) void rotary_kernel(RotaryLaunch a, long long units0, long long units1) {
-    const int half = a.rot_dim / 2, rest = a.head_dim - a.rot_dim, per_head = half + rest;
-    long long u = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int t = u >= units0;
-    if (t) u -= units0;
-    if (u >= (t ? units1 : units0)) return;
-    const int j = (int)(u % per_head);
-    const long long rh = u / per_head;
-    const int h = (int)(rh % a.src[t].heads);
-    const long long r = rh / a.src[t].heads;
-    const T* x = (const T*)a.src[t].p + r * a.src[t].row + h * a.src[t].head;
-    T* y = (T*)a.dst[t].p + r * a.dst[t].row + h * a.dst[t].head;
-    if (j >= half) {
-        const int i = a.rot_dim + (j - half);
-        y[i] = x[i];
-        return;
+// A work-group turns RB rows of one tensor: the cosines and sines of its (row, pair)s go to LDS once and serve every head,
+// then a thread takes 16 bytes at a time.
+//   kInterleaved  a chunk holds whole pairs
+//   kHalves       half of the turned part is whole chunks: a thread takes a chunk and the one its partners are in
+//   kStaged       it is not (rot_dim = head_dim - 4, say): the rows pass through LDS, from where a chunk's partners are picked
+enum RotaryForm { kInterleaved, kHalves, kStaged };
+template <class T, int D, int RB, int FORM>
+__global__ __launch_bounds__(256) void rotary_kernel(RotaryLaunch a, int tiles0) {
+    constexpr int N = 16 / (int)sizeof(T), CPR = D / N, PITCH = D + 2;
+    extern __shared__ char lds[];
+    float2* turn = (float2*)lds;                      // [RB][rot_dim / 2]
+    const int half = a.rot_dim / 2, t = (int)blockIdx.x >= tiles0, row0 = ((int)blockIdx.x - (t ? tiles0 : 0)) * RB;
+    T* stage = (T*)(lds + RB * (size_t)half * sizeof(float2));   // kStaged: [RB * heads of a round][PITCH]
+    const int rows = min(RB, a.n_rows[t] - row0), heads = a.src[t].heads;
+    const T* src = (const T*)a.src[t].p + (long long)row0 * a.src[t].row;
+    T* dst = (T*)a.dst[t].p + (long long)row0 * a.dst[t].row;
+    for (int i = threadIdx.x; i < rows * half; i += 256) {
+        const int r = i / half, j = i % half;
+        const float pos = a.pos[t][(long long)(row0 + r) * a.n_axes + (a.n_axes == 2 && j >= half / 2)];
+        float2 cs;
+        cos_sin_turns((double)pos * a.freq[j] * 0.15915494309189533577, cs.x, cs.y);
+        if (a.inverse) cs.y = -cs.y;
+        turn[i] = cs;
     }
-    const int axis = a.n_axes == 2 && j >= half / 2;
-    float c, s;
-    cos_sin_turns((double)a.pos[t][r * a.n_axes + axis] * a.freq[j] * 0.15915494309189533577, c, s);
-    if (a.inverse) s = -s;
-    const int i0 = a.layout == PPG_ROTARY_HALF ? j : 2 * j, i1 = a.layout == PPG_ROTARY_HALF ? j + half : 2 * j + 1;
-    const float u0 = to_float(x[i0]), u1 = to_float(x[i1]);
-    y[i0] = (T)(u0 * c - u1 * s);
-    y[i1] = (T)(u0 * s + u1 * c);
+    __syncthreads();
+    if constexpr (FORM == kStaged) {
+        // rounds of as many (row, head) vectors as the stage holds; a chunk is written only after all of its round was read
+        constexpr int VR = 256 / CPR;
+        for (int v0 = 0; v0 < rows * heads; v0 += VR) {
+            const int v = v0 + threadIdx.x / CPR, ch = threadIdx.x % CPR;
+            const bool on = v < rows * heads;
+            const int r = on ? v / heads : 0, h = on ? v % heads : 0;
+            Vec16<T> x;
+            T* mine = stage + (threadIdx.x / CPR) * PITCH;
+            if (on) {
+                x = *(const Vec16<T>*)(src + r * a.src[t].row + h * a.src[t].head + ch * N);
+#pragma unroll
+                for (int e = 0; e < N; e++) mine[ch * N + e] = x.v[e];
+            }
+            __syncthreads();
+            if (on) {
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    const int d = ch * N + e;
+                    if (d < a.rot_dim) {
+                        const bool low = d < half;
+                        const float2 cs = turn[r * half + (low ? d : d - half)];
+                        const float u = to_float(x.v[e]), w = to_float(mine[low ? d + half : d - half]);
+                        x.v[e] = (T)(low ? u * cs.x - w * cs.y : w * cs.y + u * cs.x);
+                    }
+                }
+                *(Vec16<T>*)(dst + r * a.dst[t].row + h * a.dst[t].head + ch * N) = x;
+            }
+            __syncthreads();
+        }
+    } else {
+        const int cut = a.rot_dim / N;   // kHalves: whole chunks turned; those behind are copied
+        const int units = FORM == kHalves ? cut / 2 + (CPR - cut) : CPR;
+        for (int i = threadIdx.x; i < rows * heads * units; i += 256) {
+            const int u = i % units, v = i / units, h = v % heads, r = v / heads;
+            const T* x = src + r * a.src[t].row + h * a.src[t].head;
+            T* y = dst + r * a.dst[t].row + h * a.dst[t].head;
+            if constexpr (FORM == kHalves) {
+                if (u >= cut / 2) {
+                    const int ch = u + cut / 2;
+                    *(Vec16<T>*)(y + ch * N) = *(const Vec16<T>*)(x + ch * N);
+                    continue;
+                }
+                Vec16<T> p = *(const Vec16<T>*)(x + u * N), q = *(const Vec16<T>*)(x + half + u * N);
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    const float2 cs = turn[r * half + u * N + e];
+                    const float f = to_float(p.v[e]), g = to_float(q.v[e]);
+                    p.v[e] = (T)(f * cs.x - g * cs.y);
+                    q.v[e] = (T)(f * cs.y + g * cs.x);
+                }
+                *(Vec16<T>*)(y + u * N) = p;
+                *(Vec16<T>*)(y + half + u * N) = q;
+            } else {
+                Vec16<T> p = *(const Vec16<T>*)(x + u * N);
+#pragma unroll
+                for (int e = 0; e < N; e += 2) {
+                    const int j = (u * N + e) / 2;
+                    if (j < half) {
+                        const float2 cs = turn[r * half + j];
+                        const float f = to_float(p.v[e]), g = to_float(p.v[e + 1]);
+                        p.v[e] = (T)(f * cs.x - g * cs.y);
+                        p.v[e + 1] = (T)(f * cs.y + g * cs.x);
+                    }
+                }
+                *(Vec16<T>*)(y + u * N) = p;
+            }
+        }
+    }
 }
 
 // ---- block means ----
-// One thread per (block, head, component).
-template <class T>
-__global__ __launch_bounds__(256) void block_means_kernel(BlockMeansLaunch a, AttnSets sets, int D) {
-    const int b = blockIdx.x, s = find_set(sets.blk, sets.n, b);
-    const int first = sets.k_off[s] + (b - sets.blk[s]) * a.block, last = min(first + a.block, sets.k_off[s + 1]);
-    int n = last - first;
-    if (a.skip) {
-        n = 0;
-        for (int r = first; r < last; r++) n += a.skip[r] == 0;
+// One work-group per block.  The block's rows are taken 16 bytes at a time: a thread owns one chunk position and every
+// `lanes`-th row, sums in 64 bits (two terms of 16-bit types per exponent step fit many times over: the sum is exact), and the
+// partial sums of a position meet in LDS.
+template <class T, int D>
+__global__ __launch_bounds__(256) void block_means_kernel(BlockMeansLaunch a, AttnSets sets) {
+    constexpr int N = 16 / (int)sizeof(T), CPR = D / N;
+    __shared__ double part[256][N];
+    __shared__ unsigned char keep[128];
+    __shared__ int kept[2];
+    const int b = blockIdx.x, s = find_set(sets.blk, sets.n, b), tid = threadIdx.x;
+    const int first = sets.k_off[s] + (b - sets.blk[s]) * a.block, n = min(a.block, sets.k_off[s + 1] - first);
+    if (tid < 128) {
+        const bool on = tid < n && !(a.skip && a.skip[first + tid]);
+        keep[tid] = on;
+        const unsigned long long m = __ballot(on);
+        if ((tid & 63) == 0) kept[tid >> 6] = __popcll(m);
     }
-    if (threadIdx.x == 0) a.count[b] = n;
-    for (int i = threadIdx.x; i < a.k.heads * D; i += 256) {
-        const T* x = (const T*)a.k.p + (i / D) * a.k.head + i % D;
-        double sum = 0;
-        for (int r = first; r < last; r++)
-            if (!a.skip || a.skip[r] == 0) sum += (double)to_float(x[(long long)r * a.k.row]);
-        a.mean[(long long)b * a.k.heads * D + i] = n ? (float)(sum / n) : 0.f;
+    __syncthreads();
+    const int count = kept[0] + kept[1];
+    if (tid == 0) a.count[b] = count;
+    const int chunks = a.k.heads * CPR;
+    for (int c0 = 0; c0 < chunks; c0 += 256) {
+        const int width = min(256, chunks - c0), lanes = 256 / width;   // positions of this round, rows at a time
+        const int c = tid % width, r0 = tid / width, h = (c0 + c) / CPR;
+        double sum[N] = {};
+        if (r0 < lanes) {
+            const T* x = (const T*)a.k.p + (long long)first * a.k.row + h * a.k.head + (c0 + c) % CPR * N;
+            // four rows in flight; what a skipped row holds, NaN included, counts as zero
+            for (int r = r0; r < n; r += 4 * lanes) {
+                Vec16<T> v[4];
+                bool on[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int rr = r + i * lanes;
+                    v[i] = *(const Vec16<T>*)(x + (long long)min(rr, n - 1) * a.k.row);
+                    on[i] = rr < n && keep[rr];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int e = 0; e < N; e++) sum[e] += on[i] ? (double)to_float(v[i].v[e]) : 0.0;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < N; e++) part[tid][e] = sum[e];
+        __syncthreads();
+        for (int i = tid; i < width * N; i += 256) {
+            const int p = i / N, e = i % N;
+            double total = 0;
+            for (int l = 0; l < lanes; l++) total += part[l * width + p][e];
+            a.mean[(long long)b * a.k.heads * D + (long long)c0 * N + i] = count ? (float)(total / count) : 0.f;
+        }
+        __syncthreads();
     }
 }
 
@@ -87,6 +190,16 @@ struct Scored {
     int idx;
 };
 __device__ __forceinline__ bool scored_before(const Scored& a, const Scored& b) { return a.key > b.key || (a.key == b.key && a.idx < b.idx); }
+// what lane l (the same for all) holds, without a trip through LDS
+__device__ __forceinline__ double lane_value(double x, int l) {
+    const long long b = __double_as_longlong(x);
+    const unsigned lo = __builtin_amdgcn_readlane((int)b, l), hi = __builtin_amdgcn_readlane((int)(b >> 32), l);
+    return __longlong_as_double((long long)(((unsigned long long)hi << 32) | lo));
+}
+__device__ __forceinline__ Scored scored_lane(const Scored& a, int l) {
+    const unsigned lo = __builtin_amdgcn_readlane((int)a.key, l), hi = __builtin_amdgcn_readlane((int)(a.key >> 32), l);
+    return Scored{((unsigned long long)hi << 32) | lo, __builtin_amdgcn_readlane(a.idx, l)};
+}
 __device__ __forceinline__ Scored scored_shfl(const Scored& a, int lane) {
     Scored r;
     r.key = __shfl(a.key, lane);
@@ -106,79 +219,295 @@ __device__ __forceinline__ void scored_sort(Scored& a, int lane) {
         for (int j = k >> 1; j > 0; j >>= 1) scored_step(a, lane, j, !(lane & k));
 }
 
-// One wave per (query row, key head).  A lane scores one block; the best n_sel so far are kept one per lane, in order, and
-// 64 new ones are merged in only when one of them beats the last of those.
-template <class T>
-__global__ __launch_bounds__(256) void block_select_kernel(BlockSelectLaunch a, AttnSets sets, int D) {
-    __shared__ double qs[4][128];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const long long unit = (long long)blockIdx.x * 4 + w;
-    const long long rows = sets.q_off[sets.n] - sets.q_off[0];
-    const bool live = unit < rows * a.kv_heads;
-    const int r = sets.q_off[0] + (int)((live ? unit : 0) / a.kv_heads), g = (int)((live ? unit : 0) % a.kv_heads);
-    const int group = a.q.heads / a.kv_heads;
-    for (int d = lane; d < D; d += 64) {
-        double sum = 0;
-        for (int h = 0; h < group; h++) sum += (double)to_float(((const T*)a.q.p)[(long long)r * a.q.row + (g * group + h) * a.q.head + d]);
-        qs[w][d] = sum;
-    }
-    __syncthreads();
-    if (!live) return;
-    const int s = find_set(sets.q_off, sets.n, r), nb = sets.blk[s + 1] - sets.blk[s];
+// The plain way, a wave per (query row, key head): a lane scores one block in 64 bits; the best n_sel so far are kept one per
+// lane, in order, and 64 new ones are merged in only when one of them beats the last of those.  q: the summed query, component
+// d in lane d % 64, place d / 64.
+template <int D>
+__device__ Scored select_all(const double (&q)[(D + 63) / 64], const float* mean, const int* count, int nb, int kv_heads, int n_sel, int lane) {
     Scored best{0, 0x7fffffff};
     for (int b0 = 0; b0 < nb; b0 += 64) {
         const int b = b0 + lane;
-        Scored c{0, 0x7fffffff};
-        if (b < nb && a.count[sets.blk[s] + b] > 0) {
-            const float* m = a.mean + ((long long)(sets.blk[s] + b) * a.kv_heads + g) * D;
-            double dot = 0;
-            for (int d = 0; d < D; d++) dot = fma(qs[w][d], (double)m[d], dot);
-            c.key = score_key(dot);
-            c.idx = b;
-        }
-        const Scored worst = scored_shfl(best, a.n_sel - 1);
+        const bool on = b < nb && count[b] > 0;
+        const float* m = mean + (long long)(on ? b : 0) * kv_heads * D;
+        double dot = 0;
+        for (int d = 0; d < D; d++) dot = fma(lane_value(q[d >> 6], d & 63), (double)m[d], dot);
+        const Scored c = on ? Scored{score_key(dot), b} : Scored{0, 0x7fffffff};
+        const Scored worst = scored_lane(best, n_sel - 1);
         if (!__any(scored_before(c, worst))) continue;
-        scored_sort(c, lane);
+        Scored x = c;
+        scored_sort(x, lane);
         // the 64 best of two ordered lists: the better of every mirrored pair, which leaves a bitonic row
-        const Scored o = scored_shfl(c, 63 - lane);
+        const Scored o = scored_shfl(x, 63 - lane);
         if (scored_before(o, best)) best = o;
 #pragma unroll
         for (int j = 32; j > 0; j >>= 1) scored_step(best, lane, j, true);
     }
-    // ascending by block
-    Scored out{0, lane < a.n_sel ? best.idx : 0x7fffffff};
-    scored_sort(out, lane);
-    if (lane < a.n_sel) a.sel[((long long)r * a.kv_heads + g) * a.n_sel + lane] = out.idx == 0x7fffffff ? -1 : out.idx;
+    return best;
+}
+
+// float as a whole number in its order; 0 stays below every number
+__device__ __forceinline__ unsigned float_key(float f) {
+    const unsigned b = __float_as_uint(f);
+    return b >> 31 ? ~b : b | 0x80000000u;
+}
+
+// A work-group selects for 16 query rows of one (set, key head).  The products of all 16 with a stretch of blocks come from the
+// bf16 matrix unit (inputs rounded: off by at most E = 2^-7 |q| |mean|, Cauchy-Schwarz over the two roundings, with room for the
+// 32-bit sum) and stay in LDS.  Then a wave takes a row: the n_sel-th largest of (product - E) is a bound t that the n_sel
+// best blocks pass for sure, so only blocks with product + E >= t can be among them; those, about n_sel and a few, are scored
+// in 64 bits and ranked exactly.  Rows for which that does not hold together (a product that is not finite, or more than 128
+// left, as with many equal means) go the plain way.
+constexpr int kSelRows = 16, kSelChunk = 1088, kSelWaves = 8, kSelPitch = kSelChunk + 4;
+struct SelectLds {
+    float score[kSelRows][kSelPitch];
+    float norm[kSelChunk];            // |mean|, -1 for a block that cannot be selected
+    unsigned short cand[kSelWaves][128];
+};
+template <class T, int D>
+__global__ __launch_bounds__(512, 4) void block_select_kernel(BlockSelectLaunch a, AttnSets sets) {
+    constexpr int PER = kSelChunk / 64, QW = (D + 63) / 64, RPW = kSelRows / kSelWaves;
+    __shared__ alignas(16) SelectLds lds;
+    const int unit = xcd_unit(blockIdx.x, sets.tile[sets.n]);
+    if (unit >= sets.tile[sets.n]) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, s = find_set(sets.tile, sets.n, unit);
+    const int q0 = sets.q_off[s], nq = sets.q_off[s + 1] - q0, tiles = (nq + kSelRows - 1) / kSelRows;
+    const int g = (unit - sets.tile[s]) / tiles, row0 = ((unit - sets.tile[s]) % tiles) * kSelRows;
+    const int group = a.q.heads / a.kv_heads, nb = sets.blk[s + 1] - sets.blk[s];
+    const float* mean = a.mean + ((long long)sets.blk[s] * a.kv_heads + g) * D;
+    const long long stride = (long long)a.kv_heads * D;
+    const int* count = a.count + sets.blk[s];
+
+    auto query = [&](int row, int d) {   // of the summed group
+        const T* x = (const T*)a.q.p + (long long)(q0 + min(row, nq - 1)) * a.q.row + (long long)g * group * a.q.head + d;
+        double sum = 0;
+        for (int h = 0; h < group; h++) sum += (double)to_float(x[h * a.q.head]);
+        return sum;
+    };
+    // operand of the matrix unit: row lane & 15, components 8 (lane >> 4) ... of every 32
+    bf16x8 qf[D / 32];
+#pragma unroll
+    for (int k = 0; k < D / 32; k++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) qf[k][e] = (__bf16)(float)query(row0 + (lane & 15), k * 32 + (lane >> 4) * 8 + e);
+    double q[RPW][QW];
+    float eq[RPW];
+    bool slow[RPW];
+    Scored best[RPW];
+#pragma unroll
+    for (int i = 0; i < RPW; i++) {
+        double sq = 0;
+#pragma unroll
+        for (int k = 0; k < QW; k++) {
+            const int d = k * 64 + lane;
+            q[i][k] = d < D ? query(row0 + wave * RPW + i, d) : 0.0;
+            sq += q[i][k] * q[i][k];
+        }
+        sq = wave_sum_d(sq);
+        // a query so short that its components leave bf16's range has no such bound, unless it is zero
+        slow[i] = !(sq < 1e36) || (sq < 1e-24 && sq > 0);
+        eq[i] = (float)sqrt(sq) * 0.0079f;   // 2^-7 and 1 %
+        best[i] = Scored{0, 0x7fffffff};
+    }
+
+    for (int b0 = 0; b0 < nb; b0 += kSelChunk) {
+        const int n = min(kSelChunk, nb - b0);
+        if (b0) __syncthreads();   // the last stretch has been read
+        for (int t = wave; t * 16 < n; t += kSelWaves) {
+            const int b = t * 16 + (lane & 15), bb = min(b, n - 1);
+            const float* m = mean + (b0 + bb) * stride + (lane >> 4) * 8;
+            typedef float f32x4s __attribute__((ext_vector_type(4)));
+            f32x4s acc = {0.f, 0.f, 0.f, 0.f};
+            float sq = 0.f;
+#pragma unroll
+            for (int k = 0; k < D / 32; k++) {
+                const f32x4s x = *(const f32x4s*)(m + k * 32), y = *(const f32x4s*)(m + k * 32 + 4);
+                bf16x8 mf;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    mf[e] = (__bf16)x[e];
+                    mf[4 + e] = (__bf16)y[e];
+                    sq = fmaf(x[e], x[e], fmaf(y[e], y[e], sq));
+                }
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mf, qf[k], acc, 0, 0, 0);
+            }
+            *(f32x4s*)&lds.score[lane & 15][t * 16 + (lane >> 4) * 4] = acc;
+            sq += __shfl_xor(sq, 16);
+            sq += __shfl_xor(sq, 32);
+            // (a mean as short as a short query: NaN, which sends the rows the plain way)
+            if (lane < 16) lds.norm[b] = b < n && count[b0 + b] > 0 ? (sq < 1e-24f && sq > 0.f ? NAN : sqrtf(sq) * 1.001f) : -1.f;
+        }
+        for (int b = (n + 15) / 16 * 16 + threadIdx.x; b < kSelChunk; b += 512) lds.norm[b] = -1.f;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < RPW; i++) {
+            const int row = wave * RPW + i;
+            if (slow[i] || row0 + row >= nq) continue;   // the same for all lanes
+            unsigned low[PER], high[PER], top = 0;
+            bool odd = false;
+#pragma unroll
+            for (int p = 0; p < PER; p++) {
+                const float x = lds.score[row][p * 64 + lane], nm = lds.norm[p * 64 + lane], e = nm * eq[i];
+                const bool on = !(nm < 0.f);
+                odd |= on && !(fabsf(x) + e < 3e38f);
+                low[p] = on ? float_key(x - e) : 0;
+                high[p] = on ? float_key(x + e) : 0;
+                top = max(top, low[p]);
+            }
+            if (__any(odd)) {
+                slow[i] = true;
+                continue;
+            }
+            // a bound that n_sel blocks reach: the n_sel-th largest of the lanes' largest, to 18 of its 32 bits
+            unsigned t = 0;
+            for (int bit = 31; bit >= 14; bit--) {
+                const unsigned c = t | (1u << bit);
+                if (__popcll(__ballot(top >= c)) >= a.n_sel) t = c;
+            }
+            auto passing = [&](const unsigned (&key)[PER], unsigned from) {
+                int c = 0;
+#pragma unroll
+                for (int p = 0; p < PER; p++) c += __popcll(__ballot(key[p] >= from));
+                return c;
+            };
+            t = max(t, 1u);
+            int left = passing(high, t);
+            if (left > 128) {   // long lists: the n_sel-th largest of all
+                t = 0;
+                for (int bit = 31; bit >= 8; bit--) {
+                    const unsigned c = t | (1u << bit);
+                    if (passing(low, c) >= a.n_sel) t = c;
+                }
+                t = max(t, 1u);
+                left = passing(high, t);
+            }
+            if (left > 128) {
+                slow[i] = true;
+                continue;
+            }
+            int at = 0;
+            unsigned short* cand = lds.cand[wave];
+#pragma unroll
+            for (int p = 0; p < PER; p++) {
+                const bool on = high[p] >= t;
+                const unsigned long long m = __ballot(on);
+                if (on) cand[at + __popcll(m & ((1ull << lane) - 1))] = (unsigned short)(p * 64 + lane);
+                at += __popcll(m);
+            }
+            __builtin_amdgcn_wave_barrier();   // the list is this wave's own
+            Scored c[2];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                c[k] = Scored{0, 0x7fffffff};
+                if (k * 64 >= left) continue;
+                const bool on = k * 64 + lane < left;
+                const int b = b0 + (on ? cand[k * 64 + lane] : cand[0]);
+                const float* m = mean + b * stride;
+                double dot = 0;
+#pragma unroll 4
+                for (int d = 0; d < D; d += 4) {
+                    const float4 x = *(const float4*)(m + d);
+                    const double* w = q[i];
+                    dot = fma(lane_value(w[d >> 6], d & 63), (double)x.x, dot);
+                    dot = fma(lane_value(w[d >> 6], (d + 1) & 63), (double)x.y, dot);
+                    dot = fma(lane_value(w[d >> 6], (d + 2) & 63), (double)x.z, dot);
+                    dot = fma(lane_value(w[d >> 6], (d + 3) & 63), (double)x.w, dot);
+                }
+                if (on) c[k] = Scored{score_key(dot), b};
+            }
+            __builtin_amdgcn_wave_barrier();
+            // ranks among these and the best of the stretches before; every lane's are in ascending block order already
+            int rank[3] = {0, 0, 0};
+            const Scored all[3] = {best[i], c[0], c[1]};
+            const int sizes[3] = {b0 ? a.n_sel : 0, min(left, 64), max(left - 64, 0)};
+#pragma unroll
+            for (int k = 0; k < 3; k++)
+                for (int l = 0; l < sizes[k]; l++) {
+                    const Scored o = scored_lane(all[k], l);
+#pragma unroll
+                    for (int x = 0; x < 3; x++) rank[x] += scored_before(o, all[x]);
+                }
+            // the n_sel first, by block: the earlier stretches', then these
+            Scored next{0, 0x7fffffff};
+            int to = 0;
+#pragma unroll
+            for (int k = 0; k < 3; k++) {
+                unsigned long long in = __ballot(all[k].idx != 0x7fffffff && rank[k] < a.n_sel);
+                while (in) {
+                    const int l = __builtin_ctzll(in);
+                    in &= in - 1;
+                    const Scored o = scored_lane(all[k], l);
+                    if (lane == to) next = o;
+                    to++;
+                }
+            }
+            best[i] = next;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RPW; i++) {
+        const int row = row0 + wave * RPW + i;
+        if (row >= nq) continue;
+        if (slow[i]) {
+            Scored x{0, 0x7fffffff};
+            const Scored b = select_all<D>(q[i], mean, count, nb, a.kv_heads, a.n_sel, lane);
+            if (lane < a.n_sel) x.idx = b.idx;
+            scored_sort(x, lane);
+            best[i] = x;
+        }
+        if (lane < a.n_sel) a.sel[((long long)(q0 + row) * a.kv_heads + g) * a.n_sel + lane] = best[i].idx == 0x7fffffff ? -1 : best[i].idx;
+    }
 }
 
 // ---- launches ----
-#define BY_TYPE(dtype, CALL)                   \
-    do {                                       \
+#define BY_TYPE(dtype, CALL)                                    \
+    do {                                                        \
         if (dtype == PPG_F32) { using T = float; CALL; }        \
         else if (dtype == PPG_BF16) { using T = __bf16; CALL; } \
-        else { using T = _Float16; CALL; }     \
+        else { using T = _Float16; CALL; }                      \
     } while (0)
+#define BY_DIM(dim, CALL)                                     \
+    do {                                                      \
+        if (dim == 32) { constexpr int D = 32; CALL; }        \
+        else if (dim == 64) { constexpr int D = 64; CALL; }   \
+        else { constexpr int D = 128; CALL; }                 \
+    } while (0)
+
 hipError_t launch_rotary(int dtype, const RotaryLaunch& a, hipStream_t s) {
-    const long long per_head = a.rot_dim / 2 + (a.head_dim - a.rot_dim);
-    const long long u0 = a.n_rows[0] ? a.n_rows[0] * (long long)a.src[0].heads * per_head : 0;
-    const long long u1 = a.n_rows[1] ? a.n_rows[1] * (long long)a.src[1].heads * per_head : 0;
-    if (u0 + u1 == 0) return hipSuccess;
-    const unsigned grid = (unsigned)((u0 + u1 + 255) / 256);
-    BY_TYPE(dtype, (rotary_kernel<T><<<grid, 256, 0, s>>>(a, u0, u1)));
-    return hipGetLastError();
+    const long long rows = (long long)a.n_rows[0] + a.n_rows[1];
+    if (!rows) return hipSuccess;
+    const int n = dtype == PPG_F32 ? 4 : 8, half = a.rot_dim / 2;
+    const int form = a.layout == PPG_ROTARY_INTERLEAVED ? kInterleaved : half % n == 0 ? kHalves : kStaged;
+    auto go = [&](auto kernel, int rb, size_t stage) {
+        const int t0 = (int)(((long long)a.n_rows[0] + rb - 1) / rb), t1 = (int)(((long long)a.n_rows[1] + rb - 1) / rb);
+        kernel<<<(unsigned)t0 + (unsigned)t1, 256, rb * (size_t)half * sizeof(float2) + stage, s>>>(a, t0);
+        return hipGetLastError();
+    };
+    hipError_t e = hipSuccess;
+    // few rows: four to a work-group, so that more of them run; many: sixteen, so that a work-group has enough to load
+#define FORMS(RB)                                                                                                              \
+    BY_TYPE(dtype, BY_DIM(a.head_dim, (e = form == kInterleaved ? go(rotary_kernel<T, D, RB, kInterleaved>, RB, 0)             \
+                                           : form == kHalves    ? go(rotary_kernel<T, D, RB, kHalves>, RB, 0)                  \
+                                                                : go(rotary_kernel<T, D, RB, kStaged>, RB,                     \
+                                                                     (size_t)256 / (D * sizeof(T) / 16) * (D + 2) * sizeof(T)))))
+    if (rows < 16384) FORMS(4);
+    else FORMS(16);
+#undef FORMS
+    return e;
 }
 
 hipError_t launch_block_means(int dtype, int head_dim, const BlockMeansLaunch& a, AttnSets& sets, hipStream_t s) {
     const int nb = sets.blk[sets.n];
     if (!nb) return hipSuccess;
-    BY_TYPE(dtype, (block_means_kernel<T><<<nb, 256, 0, s>>>(a, sets, head_dim)));
+    BY_TYPE(dtype, BY_DIM(head_dim, (block_means_kernel<T, D><<<nb, 256, 0, s>>>(a, sets))));
     return hipGetLastError();
 }
 
 hipError_t launch_block_select(int dtype, int head_dim, const BlockSelectLaunch& a, AttnSets& sets, hipStream_t s) {
-    const long long units = ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.kv_heads;
-    if (!units) return hipSuccess;
-    BY_TYPE(dtype, (block_select_kernel<T><<<(unsigned)((units + 3) / 4), 256, 0, s>>>(a, sets, head_dim)));
+    sets.tile[0] = 0;
+    for (int i = 0; i < sets.n; i++)
+        sets.tile[i + 1] = sets.tile[i] + (int)(((long long)sets.q_off[i + 1] - sets.q_off[i] + kSelRows - 1) / kSelRows * a.kv_heads);
+    if (!sets.tile[sets.n]) return hipSuccess;
+    BY_TYPE(dtype, BY_DIM(head_dim, (block_select_kernel<T, D><<<xcd_grid(sets.tile[sets.n]), 512, 0, s>>>(a, sets))));
     return hipGetLastError();
 }
 

@@ -293,7 +293,8 @@ def _select_ref(q, mean, count, q_off, k_off, block, kv_heads, n_sel):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim, heads, kv_heads, n_sel, nk", ((64, 4, 4, 16, 5000), (32, 4, 1, 1, 3000), (128, 8, 2, 64, 9000), (64, 2, 2, 7, 130),
-                                                             (32, 3, 1, 33, 33)))
+                                                             (32, 3, 1, 33, 33), (64, 2, 2, 16, 80000), (32, 2, 1, 64, 120000),
+                                                             (128, 2, 1, 5, 34815)))
 def test_block_select(gpu, dtype, dim, heads, kv_heads, n_sel, nk):
     """Ragged sets (one without keys, one without queries), dead blocks, exact ties (repeated and all-zero means), NaN means, a
     zero query, infinite queries; rows outside the sets stay."""

@@ -223,14 +223,14 @@ __device__ __forceinline__ void scored_sort(Scored& a, int lane) {
 // lane, in order, and 64 new ones are merged in only when one of them beats the last of those.  q: the summed query, component
 // d in lane d % 64, place d / 64.
 template <int D>
-__device__ Scored select_all(const double (&q)[(D + 63) / 64], const float* mean, const int* count, int nb, int kv_heads, int n_sel, int lane) {
+__device__ Scored select_all(const double (&q)[(D + 63) / 64][1], const float* mean, const int* count, int nb, int kv_heads, int n_sel, int lane) {
     Scored best{0, 0x7fffffff};
     for (int b0 = 0; b0 < nb; b0 += 64) {
         const int b = b0 + lane;
         const bool on = b < nb && count[b] > 0;
         const float* m = mean + (long long)(on ? b : 0) * kv_heads * D;
         double dot = 0;
-        for (int d = 0; d < D; d++) dot = fma(lane_value(q[d >> 6], d & 63), (double)m[d], dot);
+        for (int d = 0; d < D; d++) dot = fma(lane_value(q[d >> 6][0], d & 63), (double)m[d], dot);
         const Scored c = on ? Scored{score_key(dot), b} : Scored{0, 0x7fffffff};
         const Scored worst = scored_lane(best, n_sel - 1);
         if (!__any(scored_before(c, worst))) continue;
@@ -258,14 +258,24 @@ __device__ __forceinline__ unsigned float_key(float f) {
 // in 64 bits and ranked exactly.  Rows for which that does not hold together (a product that is not finite, or more than 128
 // left, as with many equal means) go the plain way.
 constexpr int kSelRows = 16, kSelChunk = 1088, kSelWaves = 8, kSelPitch = kSelChunk + 4;
+// A row's scores, and once its wave has them in registers, that wave's notes: the blocks left, their exact keys.
+union SelectRow {
+    float score[kSelPitch];
+    struct {
+        unsigned short cand[128];
+        unsigned long long key[128];
+        unsigned long long best_key[64];
+        int best_idx[64];
+    } note;
+};
 struct SelectLds {
-    float score[kSelRows][kSelPitch];
+    SelectRow row[kSelRows];
     float norm[kSelChunk];            // |mean|, -1 for a block that cannot be selected
-    unsigned short cand[kSelWaves][128];
 };
 template <class T, int D>
 __global__ __launch_bounds__(512, 4) void block_select_kernel(BlockSelectLaunch a, AttnSets sets) {
-    constexpr int PER = kSelChunk / 64, QW = (D + 63) / 64, RPW = kSelRows / kSelWaves;
+    constexpr int PER = kSelChunk / 64, RPW = kSelRows / kSelWaves, N = 16 / (int)sizeof(T);
+    constexpr int LPC = D / 16, CPP = 64 / LPC;   // lanes that share a candidate's product, candidates of a pass
     __shared__ alignas(16) SelectLds lds;
     const int unit = xcd_unit(blockIdx.x, sets.tile[sets.n]);
     if (unit >= sets.tile[sets.n]) return;
@@ -277,64 +287,76 @@ __global__ __launch_bounds__(512, 4) void block_select_kernel(BlockSelectLaunch 
     const long long stride = (long long)a.kv_heads * D;
     const int* count = a.count + sets.blk[s];
 
-    auto query = [&](int row, int d) {   // of the summed group
+    // components d .. d + C - 1 of the summed group of a row
+    auto query = [&](int row, int d, auto& out) {
+        constexpr int C = sizeof(out) / sizeof(out[0]);
         const T* x = (const T*)a.q.p + (long long)(q0 + min(row, nq - 1)) * a.q.row + (long long)g * group * a.q.head + d;
-        double sum = 0;
-        for (int h = 0; h < group; h++) sum += (double)to_float(x[h * a.q.head]);
-        return sum;
+#pragma unroll
+        for (int e = 0; e < C; e++) out[e] = 0;
+        for (int h = 0; h < group; h++)
+#pragma unroll
+            for (int v = 0; v < C / N; v++) {
+                const Vec16<T> y = *(const Vec16<T>*)(x + h * a.q.head + v * N);
+#pragma unroll
+                for (int e = 0; e < N; e++) out[v * N + e] += (double)to_float(y.v[e]);
+            }
     };
     // operand of the matrix unit: row lane & 15, components 8 (lane >> 4) ... of every 32
     bf16x8 qf[D / 32];
 #pragma unroll
-    for (int k = 0; k < D / 32; k++)
+    for (int k = 0; k < D / 32; k++) {
+        double x[8];
+        query(row0 + (lane & 15), k * 32 + (lane >> 4) * 8, x);
 #pragma unroll
-        for (int e = 0; e < 8; e++) qf[k][e] = (__bf16)(float)query(row0 + (lane & 15), k * 32 + (lane >> 4) * 8 + e);
-    double q[RPW][QW];
-    float eq[RPW];
-    bool slow[RPW];
+        for (int e = 0; e < 8; e++) qf[k][e] = (__bf16)(float)x[e];
+    }
     Scored best[RPW];
+    bool slow[RPW];
 #pragma unroll
     for (int i = 0; i < RPW; i++) {
-        double sq = 0;
-#pragma unroll
-        for (int k = 0; k < QW; k++) {
-            const int d = k * 64 + lane;
-            q[i][k] = d < D ? query(row0 + wave * RPW + i, d) : 0.0;
-            sq += q[i][k] * q[i][k];
-        }
-        sq = wave_sum_d(sq);
-        // a query so short that its components leave bf16's range has no such bound, unless it is zero
-        slow[i] = !(sq < 1e36) || (sq < 1e-24 && sq > 0);
-        eq[i] = (float)sqrt(sq) * 0.0079f;   // 2^-7 and 1 %
+        slow[i] = false;
         best[i] = Scored{0, 0x7fffffff};
     }
 
     for (int b0 = 0; b0 < nb; b0 += kSelChunk) {
         const int n = min(kSelChunk, nb - b0);
         if (b0) __syncthreads();   // the last stretch has been read
-        for (int t = wave; t * 16 < n; t += kSelWaves) {
-            const int b = t * 16 + (lane & 15), bb = min(b, n - 1);
-            const float* m = mean + (b0 + bb) * stride + (lane >> 4) * 8;
-            typedef float f32x4s __attribute__((ext_vector_type(4)));
-            f32x4s acc = {0.f, 0.f, 0.f, 0.f};
-            float sq = 0.f;
+        f32x4 mx[D / 32][2];
+        bool alive = false;
+        auto load = [&](int t) {
+            const int b = t * 16 + (lane & 15), bb = b0 + min(b, n - 1);
+            const float* m = mean + bb * stride + (lane >> 4) * 8;
 #pragma unroll
             for (int k = 0; k < D / 32; k++) {
-                const f32x4s x = *(const f32x4s*)(m + k * 32), y = *(const f32x4s*)(m + k * 32 + 4);
-                bf16x8 mf;
+                mx[k][0] = *(const f32x4*)(m + k * 32);
+                mx[k][1] = *(const f32x4*)(m + k * 32 + 4);
+            }
+            alive = b < n && count[bb] > 0;
+        };
+        if (wave * 16 < n) load(wave);
+        for (int t = wave; t * 16 < n; t += kSelWaves) {
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+            float sq = 0.f;
+            bf16x8 mf[D / 32];
+#pragma unroll
+            for (int k = 0; k < D / 32; k++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    mf[e] = (__bf16)x[e];
-                    mf[4 + e] = (__bf16)y[e];
-                    sq = fmaf(x[e], x[e], fmaf(y[e], y[e], sq));
+                    const float x = mx[k][0][e], y = mx[k][1][e];
+                    mf[k][e] = (__bf16)x;
+                    mf[k][4 + e] = (__bf16)y;
+                    sq = fmaf(x, x, fmaf(y, y, sq));
                 }
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mf, qf[k], acc, 0, 0, 0);
-            }
-            *(f32x4s*)&lds.score[lane & 15][t * 16 + (lane >> 4) * 4] = acc;
+            const bool on = alive;
+            if ((t + kSelWaves) * 16 < n) load(t + kSelWaves);
+#pragma unroll
+            for (int k = 0; k < D / 32; k++) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mf[k], qf[k], acc, 0, 0, 0);
+            *(f32x4*)&lds.row[lane & 15].score[t * 16 + (lane >> 4) * 4] = acc;
             sq += __shfl_xor(sq, 16);
             sq += __shfl_xor(sq, 32);
-            // (a mean as short as a short query: NaN, which sends the rows the plain way)
-            if (lane < 16) lds.norm[b] = b < n && count[b0 + b] > 0 ? (sq < 1e-24f && sq > 0.f ? NAN : sqrtf(sq) * 1.001f) : -1.f;
+            // (a mean so short that its components leave bf16's range has no such bound, unless it is zero: NaN, which sends
+            // the rows the plain way)
+            if (lane < 16) lds.norm[t * 16 + lane] = on ? (sq < 1e-24f && sq > 0.f ? NAN : sqrtf(sq) * 1.001f) : -1.f;
         }
         for (int b = (n + 15) / 16 * 16 + threadIdx.x; b < kSelChunk; b += 512) lds.norm[b] = -1.f;
         __syncthreads();
@@ -342,11 +364,18 @@ __global__ __launch_bounds__(512, 4) void block_select_kernel(BlockSelectLaunch 
         for (int i = 0; i < RPW; i++) {
             const int row = wave * RPW + i;
             if (slow[i] || row0 + row >= nq) continue;   // the same for all lanes
+            double q[16], sq = 0;
+            query(row0 + row, (lane % LPC) * 16, q);
+#pragma unroll
+            for (int e = 0; e < 16; e++) sq += q[e] * q[e];
+#pragma unroll
+            for (int x = 1; x < LPC; x <<= 1) sq += __shfl_xor(sq, x);
+            const float eq = (float)sqrt(sq) * 0.0079f;   // 2^-7 and 1 %
+            bool odd = !(sq < 1e36) || (sq < 1e-24 && sq > 0);   // as with the means
             unsigned low[PER], high[PER], top = 0;
-            bool odd = false;
 #pragma unroll
             for (int p = 0; p < PER; p++) {
-                const float x = lds.score[row][p * 64 + lane], nm = lds.norm[p * 64 + lane], e = nm * eq[i];
+                const float x = lds.row[row].score[p * 64 + lane], nm = lds.norm[p * 64 + lane], e = nm * eq;
                 const bool on = !(nm < 0.f);
                 odd |= on && !(fabsf(x) + e < 3e38f);
                 low[p] = on ? float_key(x - e) : 0;
@@ -384,63 +413,75 @@ __global__ __launch_bounds__(512, 4) void block_select_kernel(BlockSelectLaunch 
                 slow[i] = true;
                 continue;
             }
+            // (LDS serves a wave in order, and nobody else touches this row any more)
+            auto& note = lds.row[row].note;
+            __builtin_amdgcn_wave_barrier();
             int at = 0;
-            unsigned short* cand = lds.cand[wave];
 #pragma unroll
             for (int p = 0; p < PER; p++) {
                 const bool on = high[p] >= t;
                 const unsigned long long m = __ballot(on);
-                if (on) cand[at + __popcll(m & ((1ull << lane) - 1))] = (unsigned short)(p * 64 + lane);
+                if (on) note.cand[at + __popcll(m & ((1ull << lane) - 1))] = (unsigned short)(p * 64 + lane);
                 at += __popcll(m);
             }
-            __builtin_amdgcn_wave_barrier();   // the list is this wave's own
+            __builtin_amdgcn_wave_barrier();
+            const bool choose = b0 || left > a.n_sel;   // else all of them are selected and no key is needed
+            if (choose) {
+                for (int c0 = 0; c0 < left; c0 += CPP) {
+                    const int c = c0 + lane / LPC, b = b0 + note.cand[min(c, left - 1)];
+                    const float* m = mean + b * stride + (lane % LPC) * 16;
+                    f32x4 x[4];
+#pragma unroll
+                    for (int v = 0; v < 4; v++) x[v] = *(const f32x4*)(m + 4 * v);
+                    double dot = 0;
+#pragma unroll
+                    for (int e = 0; e < 16; e++) dot = fma(q[e], (double)x[e / 4][e % 4], dot);
+#pragma unroll
+                    for (int w = 1; w < LPC; w <<= 1) dot += __shfl_xor(dot, w);
+                    if (lane % LPC == 0 && c < left) note.key[c] = score_key(dot);
+                }
+                __builtin_amdgcn_wave_barrier();
+            }
             Scored c[2];
 #pragma unroll
             for (int k = 0; k < 2; k++) {
-                c[k] = Scored{0, 0x7fffffff};
-                if (k * 64 >= left) continue;
-                const bool on = k * 64 + lane < left;
-                const int b = b0 + (on ? cand[k * 64 + lane] : cand[0]);
-                const float* m = mean + b * stride;
-                double dot = 0;
-#pragma unroll 4
-                for (int d = 0; d < D; d += 4) {
-                    const float4 x = *(const float4*)(m + d);
-                    const double* w = q[i];
-                    dot = fma(lane_value(w[d >> 6], d & 63), (double)x.x, dot);
-                    dot = fma(lane_value(w[d >> 6], (d + 1) & 63), (double)x.y, dot);
-                    dot = fma(lane_value(w[d >> 6], (d + 2) & 63), (double)x.z, dot);
-                    dot = fma(lane_value(w[d >> 6], (d + 3) & 63), (double)x.w, dot);
-                }
-                if (on) c[k] = Scored{score_key(dot), b};
+                const int at_ = k * 64 + lane;
+                c[k] = at_ < left ? Scored{choose ? note.key[at_] : 1, b0 + note.cand[at_]} : Scored{0, 0x7fffffff};
             }
-            __builtin_amdgcn_wave_barrier();
-            // ranks among these and the best of the stretches before; every lane's are in ascending block order already
+            // ranks among these and the best of the stretches before; every list is in ascending block order already
             int rank[3] = {0, 0, 0};
             const Scored all[3] = {best[i], c[0], c[1]};
-            const int sizes[3] = {b0 ? a.n_sel : 0, min(left, 64), max(left - 64, 0)};
+            if (choose) {
+                const int lists = left > 64 ? 3 : 2, from = b0 ? 0 : 1;
+                const int sizes[3] = {a.n_sel, min(left, 64), left - 64};
+                if (from == 1 && lists == 2) {
+                    for (int l = 0; l < left; l++) rank[1] += scored_before(scored_lane(c[0], l), c[0]);
+                } else {
 #pragma unroll
-            for (int k = 0; k < 3; k++)
-                for (int l = 0; l < sizes[k]; l++) {
-                    const Scored o = scored_lane(all[k], l);
+                    for (int k = 0; k < 3; k++)
+                        for (int l = 0; k >= from && k < lists && l < sizes[k]; l++) {
+                            const Scored o = scored_lane(all[k], l);
 #pragma unroll
-                    for (int x = 0; x < 3; x++) rank[x] += scored_before(o, all[x]);
+                            for (int x = 0; x < 3; x++) rank[x] += scored_before(o, all[x]);
+                        }
                 }
+            }
             // the n_sel first, by block: the earlier stretches', then these
-            Scored next{0, 0x7fffffff};
             int to = 0;
 #pragma unroll
             for (int k = 0; k < 3; k++) {
-                unsigned long long in = __ballot(all[k].idx != 0x7fffffff && rank[k] < a.n_sel);
-                while (in) {
-                    const int l = __builtin_ctzll(in);
-                    in &= in - 1;
-                    const Scored o = scored_lane(all[k], l);
-                    if (lane == to) next = o;
-                    to++;
+                const bool in = all[k].idx != 0x7fffffff && rank[k] < a.n_sel;
+                const unsigned long long m = __ballot(in);
+                const int place = to + __popcll(m & ((1ull << lane) - 1));
+                if (in) {
+                    note.best_key[place] = all[k].key;
+                    note.best_idx[place] = all[k].idx;
                 }
+                to += __popcll(m);
             }
-            best[i] = next;
+            __builtin_amdgcn_wave_barrier();
+            best[i] = lane < to ? Scored{note.best_key[lane], note.best_idx[lane]} : Scored{0, 0x7fffffff};
+            __builtin_amdgcn_wave_barrier();
         }
     }
 #pragma unroll
@@ -448,8 +489,15 @@ __global__ __launch_bounds__(512, 4) void block_select_kernel(BlockSelectLaunch 
         const int row = row0 + wave * RPW + i;
         if (row >= nq) continue;
         if (slow[i]) {
+            double q[(D + 63) / 64][1];
+#pragma unroll
+            for (int k = 0; k < (D + 63) / 64; k++) {
+                const T* x = (const T*)a.q.p + (long long)(q0 + row) * a.q.row + (long long)g * group * a.q.head + min(k * 64 + lane, D - 1);
+                q[k][0] = 0;
+                for (int h = 0; h < group; h++) q[k][0] += (double)to_float(x[h * a.q.head]);
+            }
             Scored x{0, 0x7fffffff};
-            const Scored b = select_all<D>(q[i], mean, count, nb, a.kv_heads, a.n_sel, lane);
+            const Scored b = select_all<D>(q, mean, count, nb, a.kv_heads, a.n_sel, lane);
             if (lane < a.n_sel) x.idx = b.idx;
             scored_sort(x, lane);
             best[i] = x;

@@ -305,35 +305,74 @@ __global__ __launch_bounds__(256, 2) void attention_split_kernel(AttentionLaunch
     }
 }
 
-// One thread per four components of a (row, head): the parts' sums in their order.  SEL: part i belongs to place i of the
-// query's list and exists only if that names a block.
-template <class T, int D, bool SEL>
+// Joins the parts of every (row, head): D / 4 threads take four components each, PG such teams the parts of one (row, head) in
+// turn, four loads in flight; the teams' sums meet in LDS in their order.  SEL: part i belongs to place i of the query's list
+// and exists only if that names a block.
+template <class T, int D, bool SEL, int PG>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, AttnSets sets, int parts) {
-    constexpr int PER = D / 4;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, rh = i / PER;
-    const int d = (int)(i % PER) * 4;
-    if (rh >= ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads) return;
+    constexpr int TEAM = D / 4, TEAMS = 256 / TEAM;
+    struct Sum {
+        f32x4 o;
+        float m, l;
+    };
+    __shared__ Sum met[PG > 1 ? 256 : 1];
+    const int team = threadIdx.x / TEAM, sub = team % PG, d = threadIdx.x % TEAM * 4;
+    const long long n = ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads, at = (long long)blockIdx.x * (TEAMS / PG) + team / PG;
+    const long long rh = min(at, n - 1);   // (a team behind the last does its work again and keeps it to itself)
     const float c = a.scale * kLog2e;
     const Part<D>* w = (const Part<D>*)a.work + rh * parts;
     const long long q = sets.q_off[0] + rh / a.q.heads;
     const int head = (int)(rh % a.q.heads);
-    unsigned long long use = ~0ull;
+    int blocks = 0;
+    const int* sel = nullptr;
     if constexpr (SEL) {
-        const int s = find_set(sets.q_off, sets.n, (int)q), blocks = sets.blk[s + 1] - sets.blk[s];
-        const int* sel = a.sel + (q * a.k.heads + head / (a.q.heads / a.k.heads)) * a.n_sel;
-        use = 0;
-        for (int p = 0; p < parts; p++) use |= (unsigned long long)(sel[p] >= 0 && sel[p] < blocks) << p;
+        const int s = find_set(sets.q_off, sets.n, (int)q);
+        blocks = sets.blk[s + 1] - sets.blk[s];
+        sel = a.sel + (q * a.k.heads + head / (a.q.heads / a.k.heads)) * a.n_sel;
     }
     float m = -INFINITY, l = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int p = 0; p < parts; p++)
-        if (!SEL || (use >> p) & 1) m = fmaxf(m, w[p].m);
-    for (int p = 0; p < parts; p++) {
-        if (SEL && !((use >> p) & 1)) continue;
-        const float f = w[p].m == m ? 1.f : __builtin_amdgcn_exp2f((w[p].m - m) * c);
-        l += w[p].l * f;
-        o += *(const f32x4*)&w[p].o[d] * f;
+    for (int p0 = sub; p0 < parts; p0 += 4 * PG) {
+        Sum x[4];
+        bool on[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int p = min(p0 + i * PG, parts - 1);
+            x[i].o = *(const f32x4*)&w[p].o[d];
+            x[i].m = w[p].m;
+            x[i].l = w[p].l;
+            on[i] = p0 + i * PG < parts;
+            if constexpr (SEL) on[i] = on[i] && (unsigned)sel[p] < (unsigned)blocks;
+        }
+        float mn = m;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (on[i]) mn = fmaxf(mn, x[i].m);
+        const float keep = m == mn ? 1.f : __builtin_amdgcn_exp2f((m - mn) * c);
+        m = mn;
+        l *= keep;
+        o *= keep;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (on[i]) {
+                const float f = x[i].m == m ? 1.f : __builtin_amdgcn_exp2f((x[i].m - m) * c);
+                l += x[i].l * f;
+                o += x[i].o * f;
+            }
     }
+    if constexpr (PG > 1) {
+        met[threadIdx.x] = Sum{o, m, l};
+        __syncthreads();
+        if (sub) return;
+        for (int i = 1; i < PG; i++) {
+            const Sum x = met[threadIdx.x + i * TEAM];
+            const float mn = fmaxf(m, x.m), keep = m == mn ? 1.f : __builtin_amdgcn_exp2f((m - mn) * c), add = x.m == mn ? 1.f : __builtin_amdgcn_exp2f((x.m - mn) * c);
+            m = mn;
+            l = l * keep + x.l * add;
+            o = o * keep + x.o * add;
+        }
+    }
+    if (at >= n) return;
     const float inv = inverse_sum(l);
     T out[4];
 #pragma unroll
@@ -359,24 +398,37 @@ __host__ __device__ inline int region_tiles(long long nq, int n_sel, int group, 
 
 // One work-group per region: counts per block, their running sum, and the entries put in their places.  Which entry of a block
 // comes first is left to the atomics: entries of a block never meet in a sum.
-constexpr int kBins = 8192;   // blocks counted at a time (32 KB of LDS)
+constexpr int kBins = 8192;    // blocks counted at a time (32 KB of LDS)
+constexpr int kBinHold = 16;   // entries per thread that stay in registers between the two passes
 __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets sets, BinWork w) {
     __shared__ int cnt[kBins];
     __shared__ int sum_e[16], sum_t[16];
     const int kvh = a.k.heads, group = a.q.heads / kvh, s = blockIdx.x / kvh, g = blockIdx.x % kvh;
     const int q0 = sets.q_off[s], nq = sets.q_off[s + 1] - q0, blocks = sets.blk[s + 1] - sets.blk[s], n = nq * a.n_sel;
     const int* sel = a.sel + ((long long)q0 * kvh + g) * a.n_sel;
+    const long long step = (long long)kvh * a.n_sel;
     int* list = w.list + ((long long)(q0 - sets.q_off[0]) * kvh + (long long)g * nq) * a.n_sel;
     int4* tile = w.tile + sets.tile[s] + (long long)g * region_tiles(nq, a.n_sel, group, blocks);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int e0 = 0, t0 = 0;   // entries and tiles of the bins before this round's
+    int held[kBinHold];
+    auto load = [&](int from) {
+#pragma unroll
+        for (int i = 0; i < kBinHold; i++) {
+            const int e = from + i * 1024 + tid;
+            held[i] = e < n ? sel[(unsigned)e / (unsigned)a.n_sel * step + (unsigned)e % (unsigned)a.n_sel] : -1;
+        }
+    };
     for (int b0 = 0; b0 < blocks; b0 += kBins) {
         const int nb = min(kBins, blocks - b0), per = (nb + 1023) / 1024;
         for (int i = tid; i < nb; i += 1024) cnt[i] = 0;
+        if (b0 == 0) load(0);
         __syncthreads();
-        for (int e = tid; e < n; e += 1024) {
-            const int b = sel[(long long)(e / a.n_sel) * kvh * a.n_sel + e % a.n_sel] - b0;
-            if (b >= 0 && b < nb) atomicAdd(&cnt[b], 1);
+        for (int from = 0; from < n; from += kBinHold * 1024) {
+            if (n > kBinHold * 1024) load(from);
+#pragma unroll
+            for (int i = 0; i < kBinHold; i++)
+                if ((unsigned)(held[i] - b0) < (unsigned)nb && held[i] >= b0) atomicAdd(&cnt[held[i] - b0], 1);
         }
         __syncthreads();
         int es = 0, ts = 0;
@@ -414,9 +466,11 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
             eb += c;
         }
         __syncthreads();
-        for (int e = tid; e < n; e += 1024) {
-            const int b = sel[(long long)(e / a.n_sel) * kvh * a.n_sel + e % a.n_sel] - b0;
-            if (b >= 0 && b < nb) list[atomicAdd(&cnt[b], 1)] = e;
+        for (int from = 0; from < n; from += kBinHold * 1024) {
+            if (n > kBinHold * 1024) load(from);
+#pragma unroll
+            for (int i = 0; i < kBinHold; i++)
+                if ((unsigned)(held[i] - b0) < (unsigned)nb && held[i] >= b0) list[atomicAdd(&cnt[held[i] - b0], 1)] = from + i * 1024 + tid;
         }
         __syncthreads();
     }
@@ -430,7 +484,8 @@ __global__ __launch_bounds__(256, 2) void attention_blocks_kernel(AttentionLaunc
     constexpr int SUB = BN / 32, IMG = BN * D * (int)sizeof(T);
     __shared__ alignas(16) char lds_v[4][IMG];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const int at = __builtin_amdgcn_readfirstlane(xcd_unit(blockIdx.x, (sets.tile[sets.n] + 3) / 4) * 4 + wave);
+    // (in launch order: hardly two tiles read the same block, and a region's unused tiles would leave some XCDs without work)
+    const int at = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + wave);
     if (at >= sets.tile[sets.n]) return;   // waves share nothing here: each may leave by itself
     const int s = find_set(sets.tile, sets.n, at), kvh = a.k.heads, group = a.q.heads / kvh;
     const int q0 = sets.q_off[s], nq = sets.q_off[s + 1] - q0, k0 = sets.k_off[s], nk = sets.k_off[s + 1] - k0;
@@ -541,9 +596,20 @@ BlocksPlan blocks_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSe
 }
 
 template <class T, int D> hipError_t join(const AttentionLaunch& a, AttnSets& sets, int parts, bool by_list, hipStream_t s) {
-    const long long n = ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads * (D / 4);
-    if (by_list) attention_join_kernel<T, D, true><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a, sets, parts);
-    else attention_join_kernel<T, D, false><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a, sets, parts);
+    constexpr int TEAMS = 256 / (D / 4), MANY = std::min(16, TEAMS);
+    const long long n = ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads;
+    // one team per (row, head) where those fill the chip, else several
+    const int pg = n * (D / 4) >= 65536 * 4 || parts < 8 ? 1 : parts < 32 ? 4 : MANY;
+    const unsigned grid = (unsigned)((n + TEAMS / pg - 1) / (TEAMS / pg));
+#define JOIN(SEL)                                                                                    \
+    do {                                                                                             \
+        if (pg == 1) attention_join_kernel<T, D, SEL, 1><<<grid, 256, 0, s>>>(a, sets, parts);       \
+        else if (pg == 4) attention_join_kernel<T, D, SEL, 4><<<grid, 256, 0, s>>>(a, sets, parts);  \
+        else attention_join_kernel<T, D, SEL, MANY><<<grid, 256, 0, s>>>(a, sets, parts);            \
+    } while (0)
+    if (by_list) JOIN(true);
+    else JOIN(false);
+#undef JOIN
     return hipGetLastError();
 }
 template <class T, int D> hipError_t run(const AttentionLaunch& a, AttnSets& sets, int dtype, hipStream_t s) {
@@ -564,7 +630,7 @@ template <class T, int D> hipError_t run(const AttentionLaunch& a, AttnSets& set
         if (sets.tile[sets.n]) {
             bin_kernel<<<sets.n * a.k.heads, 1024, 0, s>>>(a, sets, w);
             if ((e = hipGetLastError()) != hipSuccess) return e;
-            attention_blocks_kernel<T, D, OWN_BN><<<xcd_grid((sets.tile[sets.n] + 3) / 4), 256, 0, s>>>(a, sets, w);
+            attention_blocks_kernel<T, D, OWN_BN><<<(unsigned)((sets.tile[sets.n] + 3) / 4), 256, 0, s>>>(a, sets, w);
             if ((e = hipGetLastError()) != hipSuccess) return e;
         }
         return join<T, D>(a, sets, p.parts, true, s);

@@ -196,6 +196,7 @@ __device__ __forceinline__ double lane_value(double x, int l) {
     const unsigned lo = __builtin_amdgcn_readlane((int)b, l), hi = __builtin_amdgcn_readlane((int)(b >> 32), l);
     return __longlong_as_double((long long)(((unsigned long long)hi << 32) | lo));
 }
+__device__ __forceinline__ float lane_value(float x, int l) { return __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(x), l)); }
 __device__ __forceinline__ Scored scored_lane(const Scored& a, int l) {
     const unsigned lo = __builtin_amdgcn_readlane((int)a.key, l), hi = __builtin_amdgcn_readlane((int)(a.key >> 32), l);
     return Scored{((unsigned long long)hi << 32) | lo, __builtin_amdgcn_readlane(a.idx, l)};
@@ -245,82 +246,83 @@ __device__ Scored select_all(const double (&q)[(D + 63) / 64][1], const float* m
     return best;
 }
 
-// float as a whole number in its order; 0 stays below every number
+// float as a whole number in its order, and back; what no finite number gives becomes the nearest of them
 __device__ __forceinline__ unsigned float_key(float f) {
     const unsigned b = __float_as_uint(f);
     return b >> 31 ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float key_float(unsigned k) {
+    k = max(0x00800000u, min(k, 0xff7fffffu));
+    return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k);
+}
 
-// A work-group selects for 16 query rows of one (set, key head).  The products of all 16 with a stretch of blocks come from the
-// bf16 matrix unit (inputs rounded: off by at most E = 2^-7 |q| |mean|, Cauchy-Schwarz over the two roundings, with room for the
-// 32-bit sum) and stay in LDS.  Then a wave takes a row: the n_sel-th largest of (product - E) is a bound t that the n_sel
-// best blocks pass for sure, so only blocks with product + E >= t can be among them; those, about n_sel and a few, are scored
-// in 64 bits and ranked exactly.  Rows for which that does not hold together (a product that is not finite, or more than 128
-// left, as with many equal means) go the plain way.
-constexpr int kSelRows = 16, kSelChunk = 1088, kSelWaves = 8, kSelPitch = kSelChunk + 4;
-// A row's scores, and once its wave has them in registers, that wave's notes: the blocks left, their exact keys.
+// A work-group selects for 32 query rows of one (set, key head).  The products of all 32 with a stretch of blocks come from the
+// bf16 matrix unit, both inputs split into two halves and three of the four products taken: off by at most
+// E = 2^-13 |q| |mean| (Cauchy-Schwarz; what is left out is below 3 * 2^-16, the 32-bit sums of up to 384 terms below
+// 2^-15).  They stay in LDS.  Then a wave takes a row: the n_sel-th largest of (product - E) is a bound t that the n_sel best
+// blocks reach for sure, so only blocks with product + E >= t can be among them.  Mostly those are n_sel and that is the
+// answer; else they are scored in 64 bits and ranked exactly.  Rows for which that does not hold together (a product that is
+// not finite, or more than 128 left, as with many equal means) go the plain way.
+// 8 streams of 1024 rows against 65537 keys (1025 blocks), 4 heads of 64: LDS_TIME.
+constexpr int kSelRows = 32, kSelChunk = 1088, kSelWaves = 16, kSelPitch = kSelChunk + 4;
+// A row's scores, and once its wave has them in registers, that wave's notes: the blocks left, their bounds, their exact keys.
 union SelectRow {
     float score[kSelPitch];
     struct {
         unsigned short cand[128];
+        float low[128], high[128];
         unsigned long long key[128];
         unsigned long long best_key[64];
         int best_idx[64];
     } note;
 };
-struct SelectLds {
+template <int D> struct SelectLds {
     SelectRow row[kSelRows];
-    float norm[kSelChunk];            // |mean|, -1 for a block that cannot be selected
+    float norm[kSelChunk];                 // |mean|, -1 for a block that cannot be selected
+    char q[2][kSelRows * D * 2];           // the summed queries' upper and lower halves, chunks permuted against bank conflicts
 };
 template <class T, int D>
-__global__ __launch_bounds__(512, 4) void block_select_kernel(BlockSelectLaunch a, AttnSets sets) {
+__global__ __launch_bounds__(1024, 4) void block_select_kernel(BlockSelectLaunch a, AttnSets sets) {
     constexpr int PER = kSelChunk / 64, RPW = kSelRows / kSelWaves, N = 16 / (int)sizeof(T);
     constexpr int LPC = D / 16, CPP = 64 / LPC;   // lanes that share a candidate's product, candidates of a pass
-    __shared__ alignas(16) SelectLds lds;
+    __shared__ alignas(16) SelectLds<D> lds;
     const int unit = xcd_unit(blockIdx.x, sets.tile[sets.n]);
     if (unit >= sets.tile[sets.n]) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, s = find_set(sets.tile, sets.n, unit);
-    const int q0 = sets.q_off[s], nq = sets.q_off[s + 1] - q0, tiles = (nq + kSelRows - 1) / kSelRows;
-    const int g = (unit - sets.tile[s]) / tiles, row0 = ((unit - sets.tile[s]) % tiles) * kSelRows;
+    const int q0 = sets.q_off[s], nq = sets.q_off[s + 1] - q0;
+    // the heads in turn: work-groups that run at the same time then read whole rows of means between them, and with those all
+    // channels of the L2
+    const int g = (unit - sets.tile[s]) % a.kv_heads, row0 = ((unit - sets.tile[s]) / a.kv_heads) * kSelRows;
     const int group = a.q.heads / a.kv_heads, nb = sets.blk[s + 1] - sets.blk[s];
     const float* mean = a.mean + ((long long)sets.blk[s] * a.kv_heads + g) * D;
     const long long stride = (long long)a.kv_heads * D;
     const int* count = a.count + sets.blk[s];
+    auto query = [&](int row, int h) { return (const T*)a.q.p + (long long)(q0 + min(row, nq - 1)) * a.q.row + ((long long)g * group + h) * a.q.head; };
+    auto q_chunk = [&](int half, int r, int ch) { return lds.q[half] + r * (D * 2) + ((ch ^ (r & (D >= 64 ? 7 : 3))) << 4); };
 
-    // components d .. d + C - 1 of the summed group of a row
-    auto query = [&](int row, int d, auto& out) {
-        constexpr int C = sizeof(out) / sizeof(out[0]);
-        const T* x = (const T*)a.q.p + (long long)(q0 + min(row, nq - 1)) * a.q.row + (long long)g * group * a.q.head + d;
-#pragma unroll
-        for (int e = 0; e < C; e++) out[e] = 0;
-        for (int h = 0; h < group; h++)
-#pragma unroll
-            for (int v = 0; v < C / N; v++) {
-                const Vec16<T> y = *(const Vec16<T>*)(x + h * a.q.head + v * N);
-#pragma unroll
-                for (int e = 0; e < N; e++) out[v * N + e] += (double)to_float(y.v[e]);
-            }
-    };
-    // operand of the matrix unit: row lane & 15, components 8 (lane >> 4) ... of every 32
-    bf16x8 qf[D / 32];
-#pragma unroll
-    for (int k = 0; k < D / 32; k++) {
-        double x[8];
-        query(row0 + (lane & 15), k * 32 + (lane >> 4) * 8, x);
-#pragma unroll
-        for (int e = 0; e < 8; e++) qf[k][e] = (__bf16)(float)x[e];
-    }
+    // a wave per RPW rows: the group's sum, its halves to LDS, its length
     Scored best[RPW];
-    bool slow[RPW];
+    float eq[RPW];   // 2^-13 |q|, NaN: the plain way
 #pragma unroll
     for (int i = 0; i < RPW; i++) {
-        slow[i] = false;
+        const int r = wave * RPW + i;
+        double sq = 0;
+        for (int d = lane; d < D; d += 64) {
+            double x = 0;
+            for (int h = 0; h < group; h++) x += (double)to_float(query(row0 + r, h)[d]);
+            const __bf16 hi = (__bf16)(float)x, lo = (__bf16)(float)(x - (double)(float)hi);
+            *(__bf16*)(q_chunk(0, r, d >> 3) + (d & 7) * 2) = hi;
+            *(__bf16*)(q_chunk(1, r, d >> 3) + (d & 7) * 2) = lo;
+            sq += x * x;
+        }
+        sq = wave_sum_d(sq);
+        // (one so short that its components leave bf16's range has no such bound, unless it is zero)
+        eq[i] = sq < 1e36 && !(sq < 1e-24 && sq > 0) ? (float)sqrt(sq) * 1.22071e-4f : NAN;
         best[i] = Scored{0, 0x7fffffff};
     }
 
     for (int b0 = 0; b0 < nb; b0 += kSelChunk) {
         const int n = min(kSelChunk, nb - b0);
-        if (b0) __syncthreads();   // the last stretch has been read
         f32x4 mx[D / 32][2];
         bool alive = false;
         auto load = [&](int t) {
@@ -334,83 +336,87 @@ __global__ __launch_bounds__(512, 4) void block_select_kernel(BlockSelectLaunch 
             alive = b < n && count[bb] > 0;
         };
         if (wave * 16 < n) load(wave);
+        __syncthreads();   // the queries are in LDS; the last stretch has been read
         for (int t = wave; t * 16 < n; t += kSelWaves) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-            float sq = 0.f;
-            bf16x8 mf[D / 32];
+            f32x4 acc[2] = {};
+            float sm = 0.f;
+            bf16x8 mh[D / 32], ml[D / 32];
 #pragma unroll
             for (int k = 0; k < D / 32; k++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float x = mx[k][0][e], y = mx[k][1][e];
-                    mf[k][e] = (__bf16)x;
-                    mf[k][4 + e] = (__bf16)y;
-                    sq = fmaf(x, x, fmaf(y, y, sq));
+                for (int e = 0; e < 8; e++) {
+                    const float x = mx[k][e / 4][e % 4];
+                    mh[k][e] = (__bf16)x;
+                    ml[k][e] = (__bf16)(x - (float)mh[k][e]);
+                    sm = fmaf(x, x, sm);
                 }
             const bool on = alive;
             if ((t + kSelWaves) * 16 < n) load(t + kSelWaves);
 #pragma unroll
-            for (int k = 0; k < D / 32; k++) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mf[k], qf[k], acc, 0, 0, 0);
-            *(f32x4*)&lds.row[lane & 15].score[t * 16 + (lane >> 4) * 4] = acc;
-            sq += __shfl_xor(sq, 16);
-            sq += __shfl_xor(sq, 32);
-            // (a mean so short that its components leave bf16's range has no such bound, unless it is zero: NaN, which sends
-            // the rows the plain way)
-            if (lane < 16) lds.norm[t * 16 + lane] = on ? (sq < 1e-24f && sq > 0.f ? NAN : sqrtf(sq) * 1.001f) : -1.f;
+            for (int rt = 0; rt < 2; rt++) {
+#pragma unroll
+                for (int k = 0; k < D / 32; k++) {
+                    const int r = rt * 16 + (lane & 15), ch = k * 4 + (lane >> 4);
+                    const bf16x8 qh = *(const bf16x8*)q_chunk(0, r, ch), ql = *(const bf16x8*)q_chunk(1, r, ch);
+                    acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mh[k], qh, acc[rt], 0, 0, 0);
+                    acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mh[k], ql, acc[rt], 0, 0, 0);
+                    acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ml[k], qh, acc[rt], 0, 0, 0);
+                }
+                *(f32x4*)&lds.row[rt * 16 + (lane & 15)].score[t * 16 + (lane >> 4) * 4] = acc[rt];
+            }
+            sm += __shfl_xor(sm, 16);
+            sm += __shfl_xor(sm, 32);
+            // (as short a mean as the query above: NaN, which sends the rows the plain way)
+            if (lane < 16) lds.norm[t * 16 + lane] = on ? (sm < 1e-24f && sm > 0.f ? NAN : sqrtf(sm) * 1.0001f) : -1.f;
         }
-        for (int b = (n + 15) / 16 * 16 + threadIdx.x; b < kSelChunk; b += 512) lds.norm[b] = -1.f;
+        for (int b = (n + 15) / 16 * 16 + threadIdx.x; b < kSelChunk; b += 1024) lds.norm[b] = -1.f;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < RPW; i++) {
             const int row = wave * RPW + i;
-            if (slow[i] || row0 + row >= nq) continue;   // the same for all lanes
-            double q[16], sq = 0;
-            query(row0 + row, (lane % LPC) * 16, q);
-#pragma unroll
-            for (int e = 0; e < 16; e++) sq += q[e] * q[e];
-#pragma unroll
-            for (int x = 1; x < LPC; x <<= 1) sq += __shfl_xor(sq, x);
-            const float eq = (float)sqrt(sq) * 0.0079f;   // 2^-7 and 1 %
-            bool odd = !(sq < 1e36) || (sq < 1e-24 && sq > 0);   // as with the means
-            unsigned low[PER], high[PER], top = 0;
+            if (eq[i] != eq[i] || row0 + row >= nq) continue;   // the same for all lanes
+            float low[PER], high[PER], top = -INFINITY;
+            bool odd = false;
 #pragma unroll
             for (int p = 0; p < PER; p++) {
-                const float x = lds.row[row].score[p * 64 + lane], nm = lds.norm[p * 64 + lane], e = nm * eq;
+                const float x = lds.row[row].score[p * 64 + lane], nm = lds.norm[p * 64 + lane], e = nm * eq[i];
                 const bool on = !(nm < 0.f);
                 odd |= on && !(fabsf(x) + e < 3e38f);
-                low[p] = on ? float_key(x - e) : 0;
-                high[p] = on ? float_key(x + e) : 0;
-                top = max(top, low[p]);
+                low[p] = on ? x - e : -INFINITY;
+                high[p] = on ? x + e : -INFINITY;
+                top = fmaxf(top, low[p]);
             }
             if (__any(odd)) {
-                slow[i] = true;
+                eq[i] = NAN;
                 continue;
             }
-            // a bound that n_sel blocks reach: the n_sel-th largest of the lanes' largest, to 18 of its 32 bits
-            unsigned t = 0;
+            // a bound that n_sel blocks reach: the n_sel-th largest of the lanes' largest, to 18 of its 32 bits (or, with fewer
+            // blocks, the lowest number)
+            const unsigned top_key = top == -INFINITY ? 0 : float_key(top);
+            unsigned tk = 0;
             for (int bit = 31; bit >= 14; bit--) {
-                const unsigned c = t | (1u << bit);
-                if (__popcll(__ballot(top >= c)) >= a.n_sel) t = c;
+                const unsigned c = tk | (1u << bit);
+                if (__popcll(__ballot(top_key >= c)) >= a.n_sel) tk = c;
             }
-            auto passing = [&](const unsigned (&key)[PER], unsigned from) {
+            float t = key_float(tk);
+            auto passing = [&](const float (&x)[PER], float from) {
                 int c = 0;
 #pragma unroll
-                for (int p = 0; p < PER; p++) c += __popcll(__ballot(key[p] >= from));
+                for (int p = 0; p < PER; p++) c += __popcll(__ballot(x[p] >= from));
                 return c;
             };
-            t = max(t, 1u);
             int left = passing(high, t);
             if (left > 128) {   // long lists: the n_sel-th largest of all
-                t = 0;
-                for (int bit = 31; bit >= 8; bit--) {
-                    const unsigned c = t | (1u << bit);
-                    if (passing(low, c) >= a.n_sel) t = c;
+                tk = 0;
+                for (int bit = 31; bit >= 0; bit--) {
+                    const unsigned c = tk | (1u << bit);
+                    if (passing(low, key_float(c)) >= a.n_sel) tk = c;
                 }
-                t = max(t, 1u);
+                t = key_float(tk);
                 left = passing(high, t);
             }
             if (left > 128) {
-                slow[i] = true;
+                eq[i] = NAN;
                 continue;
             }
             // (LDS serves a wave in order, and nobody else touches this row any more)
@@ -421,12 +427,77 @@ __global__ __launch_bounds__(512, 4) void block_select_kernel(BlockSelectLaunch 
             for (int p = 0; p < PER; p++) {
                 const bool on = high[p] >= t;
                 const unsigned long long m = __ballot(on);
-                if (on) note.cand[at + __popcll(m & ((1ull << lane) - 1))] = (unsigned short)(p * 64 + lane);
+                if (on) {
+                    const int to = at + __popcll(m & ((1ull << lane) - 1));
+                    note.cand[to] = (unsigned short)(p * 64 + lane);
+                    note.low[to] = low[p];
+                    note.high[to] = high[p];
+                }
                 at += __popcll(m);
             }
             __builtin_amdgcn_wave_barrier();
-            const bool choose = b0 || left > a.n_sel;   // else all of them are selected and no key is needed
-            if (choose) {
+            int cand[2];
+            unsigned long long key[2];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                cand[k] = k * 64 + lane < left ? note.cand[k * 64 + lane] : -1;
+                key[k] = 1;
+            }
+            bool in[2] = {cand[0] >= 0, cand[1] >= 0};
+            if (left > a.n_sel) {
+                // the bound once more, exactly: the largest that n_sel of what is left reach
+                float lo[2], hi[2];
+                int reach[2] = {0, 0};
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    lo[k] = in[k] ? note.low[k * 64 + lane] : -INFINITY;
+                    hi[k] = in[k] ? note.high[k * 64 + lane] : -INFINITY;
+                }
+                if (left <= 64) {
+                    for (int l = 0; l < left; l++) reach[0] += lane_value(lo[0], l) >= lo[0];
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 2; k++)
+                        for (int l = 0; l < min(left - 64 * k, 64); l++) {
+                            const float o = lane_value(lo[k], l);
+                            reach[0] += o >= lo[0];
+                            reach[1] += o >= lo[1];
+                        }
+                }
+                t = wave_max(fmaxf(in[0] && reach[0] >= a.n_sel ? lo[0] : -INFINITY, in[1] && reach[1] >= a.n_sel ? lo[1] : -INFINITY));
+                int kept = 0;
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    in[k] = in[k] && hi[k] >= t;
+                    const unsigned long long m = __ballot(in[k]);
+                    if (in[k]) note.cand[kept + __popcll(m & ((1ull << lane) - 1))] = (unsigned short)cand[k];
+                    kept += __popcll(m);
+                }
+                __builtin_amdgcn_wave_barrier();
+                left = kept;
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    in[k] = k * 64 + lane < left;
+                    cand[k] = in[k] ? note.cand[k * 64 + lane] : -1;
+                }
+            }
+            const bool choose = b0 || nb > kSelChunk || left > a.n_sel;   // (keys for the stretches to come, too)
+            if (!choose) {
+                best[i] = in[0] ? Scored{1, cand[0]} : Scored{0, 0x7fffffff};   // (at most n_sel of them, in order)
+                continue;
+            }
+            int order[3] = {0, 0, 0};
+            {
+                double q[16];
+#pragma unroll
+                for (int e = 0; e < 16; e++) q[e] = 0;
+                for (int h = 0; h < group; h++)
+#pragma unroll
+                    for (int v = 0; v < 16 / N; v++) {
+                        const Vec16<T> y = *(const Vec16<T>*)(query(row0 + row, h) + (lane % LPC) * 16 + v * N);
+#pragma unroll
+                        for (int e = 0; e < N; e++) q[v * N + e] += (double)to_float(y.v[e]);
+                    }
                 for (int c0 = 0; c0 < left; c0 += CPP) {
                     const int c = c0 + lane / LPC, b = b0 + note.cand[min(c, left - 1)];
                     const float* m = mean + b * stride + (lane % LPC) * 16;
@@ -441,39 +512,31 @@ __global__ __launch_bounds__(512, 4) void block_select_kernel(BlockSelectLaunch 
                     if (lane % LPC == 0 && c < left) note.key[c] = score_key(dot);
                 }
                 __builtin_amdgcn_wave_barrier();
-            }
-            Scored c[2];
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const int at_ = k * 64 + lane;
-                c[k] = at_ < left ? Scored{choose ? note.key[at_] : 1, b0 + note.cand[at_]} : Scored{0, 0x7fffffff};
+                for (int k = 0; k < 2; k++)
+                    if (in[k]) key[k] = note.key[k * 64 + lane];
             }
             // ranks among these and the best of the stretches before; every list is in ascending block order already
-            int rank[3] = {0, 0, 0};
-            const Scored all[3] = {best[i], c[0], c[1]};
-            if (choose) {
-                const int lists = left > 64 ? 3 : 2, from = b0 ? 0 : 1;
-                const int sizes[3] = {a.n_sel, min(left, 64), left - 64};
-                if (from == 1 && lists == 2) {
-                    for (int l = 0; l < left; l++) rank[1] += scored_before(scored_lane(c[0], l), c[0]);
-                } else {
+            const Scored all[3] = {best[i], in[0] ? Scored{key[0], b0 + cand[0]} : Scored{0, 0x7fffffff},
+                                   in[1] ? Scored{key[1], b0 + cand[1]} : Scored{0, 0x7fffffff}};
+            {
+                const int sizes[3] = {b0 ? a.n_sel : 0, min(left, 64), left - 64};
 #pragma unroll
-                    for (int k = 0; k < 3; k++)
-                        for (int l = 0; k >= from && k < lists && l < sizes[k]; l++) {
-                            const Scored o = scored_lane(all[k], l);
+                for (int k = 0; k < 3; k++)
+                    for (int l = 0; l < sizes[k]; l++) {
+                        const Scored o = scored_lane(all[k], l);
 #pragma unroll
-                            for (int x = 0; x < 3; x++) rank[x] += scored_before(o, all[x]);
-                        }
-                }
+                        for (int x = 0; x < 3; x++) order[x] += scored_before(o, all[x]);
+                    }
             }
             // the n_sel first, by block: the earlier stretches', then these
             int to = 0;
 #pragma unroll
             for (int k = 0; k < 3; k++) {
-                const bool in = all[k].idx != 0x7fffffff && rank[k] < a.n_sel;
-                const unsigned long long m = __ballot(in);
+                const bool take = all[k].idx != 0x7fffffff && order[k] < a.n_sel;
+                const unsigned long long m = __ballot(take);
                 const int place = to + __popcll(m & ((1ull << lane) - 1));
-                if (in) {
+                if (take) {
                     note.best_key[place] = all[k].key;
                     note.best_idx[place] = all[k].idx;
                 }
@@ -488,13 +551,12 @@ __global__ __launch_bounds__(512, 4) void block_select_kernel(BlockSelectLaunch 
     for (int i = 0; i < RPW; i++) {
         const int row = row0 + wave * RPW + i;
         if (row >= nq) continue;
-        if (slow[i]) {
+        if (eq[i] != eq[i]) {
             double q[(D + 63) / 64][1];
 #pragma unroll
             for (int k = 0; k < (D + 63) / 64; k++) {
-                const T* x = (const T*)a.q.p + (long long)(q0 + row) * a.q.row + (long long)g * group * a.q.head + min(k * 64 + lane, D - 1);
                 q[k][0] = 0;
-                for (int h = 0; h < group; h++) q[k][0] += (double)to_float(x[h * a.q.head]);
+                for (int h = 0; h < group; h++) q[k][0] += (double)to_float(query(row, h)[min(k * 64 + lane, D - 1)]);
             }
             Scored x{0, 0x7fffffff};
             const Scored b = select_all<D>(q, mean, count, nb, a.kv_heads, a.n_sel, lane);
@@ -555,7 +617,7 @@ hipError_t launch_block_select(int dtype, int head_dim, const BlockSelectLaunch&
     for (int i = 0; i < sets.n; i++)
         sets.tile[i + 1] = sets.tile[i] + (int)(((long long)sets.q_off[i + 1] - sets.q_off[i] + kSelRows - 1) / kSelRows * a.kv_heads);
     if (!sets.tile[sets.n]) return hipSuccess;
-    BY_TYPE(dtype, BY_DIM(head_dim, (block_select_kernel<T, D><<<xcd_grid(sets.tile[sets.n]), 512, 0, s>>>(a, sets))));
+    BY_TYPE(dtype, BY_DIM(head_dim, (block_select_kernel<T, D><<<xcd_grid(sets.tile[sets.n]), 1024, 0, s>>>(a, sets))));
     return hipGetLastError();
 }
 

@@ -412,11 +412,18 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int e0 = 0, t0 = 0;   // entries and tiles of the bins before this round's
     int held[kBinHold];
+    const int dq = 1024 / a.n_sel, dr = 1024 % a.n_sel;   // 1024 entries on, in queries and places
     auto load = [&](int from) {
+        int q = (from + tid) / a.n_sel, r = (from + tid) % a.n_sel;
 #pragma unroll
         for (int i = 0; i < kBinHold; i++) {
-            const int e = from + i * 1024 + tid;
-            held[i] = e < n ? sel[(unsigned)e / (unsigned)a.n_sel * step + (unsigned)e % (unsigned)a.n_sel] : -1;
+            held[i] = from + i * 1024 + tid < n ? sel[q * step + r] : -1;
+            q += dq;
+            r += dr;
+            if (r >= a.n_sel) {
+                r -= a.n_sel;
+                q++;
+            }
         }
     };
     for (int b0 = 0; b0 < blocks; b0 += kBins) {

@@ -50,86 +50,160 @@ template <class T, int D> __device__ __forceinline__ void store_out(const ppg_ro
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }
 __device__ __forceinline__ float log_sum(float m, float l, float c) { return l == 0.f ? -INFINITY : fmaf(m, c, __log2f(l)) * kLn2; }
 
-template <class T, int D, int BN>
-__global__ __launch_bounds__(256, 2) void attention_wide_kernel(AttentionLaunch a, AttnSets sets) {
+// Which keys are masked is read once, a bit each, kWindow words ahead, so that the loads of a tile do not wait for it.
+// UNIT (16-bit types): the matrix unit adds up the weights (a product with ones); the vector unit, which has the exponentials, is
+// the busier one (4 % of the time at 64 and at 128 components).  Those are the rounded weights, the same that meet the
+// values, but their sum is not good enough for a log: with lse the vector unit adds up the unrounded ones.
+constexpr int kWindow = 64;   // 64-key words of the mask in LDS at a time
+template <class T, int D, int BN, int QT, bool UNIT>
+__global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) void attention_wide_kernel(AttentionLaunch a, AttnSets sets) {
     using S = Shape<T, D>;
-    constexpr int SUB = BN / 32, CH = BN * S::CPR / 256, ROWB = D * (int)sizeof(T), TILE = BN * ROWB;
+    constexpr int SUB = BN / 32, CH = BN * S::CPR / 256, ROWB = D * (int)sizeof(T), TILE = BN * ROWB, WG = 128 * QT, STEP = 256 / S::CPR;
+    constexpr unsigned long long FULL = BN == 64 ? ~0ull : 0xffffffffull;
     static_assert(BN * S::CPR % 256 == 0, "tile loads are whole rounds of the work-group");
     __shared__ alignas(16) char lds_k[2][TILE], lds_v[2][TILE];
-    __shared__ unsigned char lds_dead[2][BN];
+    __shared__ unsigned long long lds_dead[kWindow];
     const int unit = xcd_unit(blockIdx.x, sets.tile[sets.n]);
     if (unit >= sets.tile[sets.n]) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    const int s = find_set(sets.tile, sets.n, unit);
+    const int s = find_set_wave(sets.tile, sets.n, unit, lane);
     const int q0 = sets.q_off[s], k0 = sets.k_off[s], nk = sets.k_off[s + 1] - k0, kvh = a.k.heads, group = a.q.heads / kvh;
-    const int rows = (sets.q_off[s + 1] - q0) * group, tiles = (rows + 127) / 128;
-    const int g = (unit - sets.tile[s]) / tiles, row = ((unit - sets.tile[s]) % tiles) * 128 + wave * 32 + (lane & 31);
-    const RowPlace place = row_place(row, rows, group, g, q0);
-    u32x4 qf[S::NF];
-    load_query<T, D>(qf, a.q, place, h);
+    const int rows = (sets.q_off[s + 1] - q0) * group, tiles = (rows + WG - 1) / WG;
+    const int g = (unit - sets.tile[s]) / tiles, row = ((unit - sets.tile[s]) % tiles) * WG + wave * (32 * QT) + (lane & 31);
     const float c = a.scale * kLog2e, slack = 8.f / c;
-    Running<T, D> run;
-    run.clear();
-
-    // tile loads: thread -> (row, chunk); rows behind the set are its last one with zero values
-    const T* kp = (const T*)a.k.p + g * a.k.head + (long long)k0 * a.k.row;
-    const T* vp = (const T*)a.v.p + g * a.v.head + (long long)k0 * a.v.row;
-    u32x4 rk[CH], rv[CH];
-    bool dead[CH];
-    auto load = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < CH; i++) {
-            const int x = tid + 256 * i, j = t * BN + x / S::CPR, ch = x % S::CPR, jj = min(j, nk - 1);
-            rk[i] = *(const u32x4*)(kp + (long long)jj * a.k.row + ch * S::N);
-            rv[i] = *(const u32x4*)(vp + (long long)jj * a.v.row + ch * S::N);
-            dead[i] = j >= nk || (a.skip && a.skip[k0 + jj]);
-        }
-    };
-    auto store = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < CH; i++) {
-            const int x = tid + 256 * i, r = x / S::CPR, ch = x % S::CPR;
-            *(u32x4*)(lds_k[buf] + r * ROWB + ((ch ^ S::swz_k(r)) << 4)) = rk[i];
-            *(u32x4*)(lds_v[buf] + r * ROWB + ((ch ^ S::swz_v(r)) << 4)) = dead[i] ? u32x4{0, 0, 0, 0} : rv[i];
-            if (ch == 0) lds_dead[buf][r] = dead[i];
-        }
-    };
     const int nt = (nk + BN - 1) / BN;
+
+    // tile loads: thread -> (row, chunk) and STEP rows on
+    const int r0 = tid / S::CPR, ch0 = tid % S::CPR;
+    const T* kp = (const T*)a.k.p + g * a.k.head + (long long)k0 * a.k.row + ch0 * S::N;
+    const T* vp = (const T*)a.v.p + g * a.v.head + (long long)k0 * a.v.row + ch0 * S::N;
+    const T *kr = kp + r0 * a.k.row, *vr = vp + r0 * a.v.row;
+    u32x4 rk[CH], rv[CH];
+    auto fetch = [&](int t) {
+        const long long j = (long long)t * BN;
+        if (j + BN <= nk) {   // the same for all
+            const T *x = kr + j * a.k.row, *y = vr + j * a.v.row;
+#pragma unroll
+            for (int i = 0; i < CH; i++) {
+                rk[i] = *(const u32x4*)(x + (long long)STEP * i * a.k.row);
+                rv[i] = *(const u32x4*)(y + (long long)STEP * i * a.v.row);
+            }
+        } else {   // rows behind the set are its last one
+#pragma unroll
+            for (int i = 0; i < CH; i++) {
+                const long long r = min((int)j + r0 + STEP * i, nk - 1);
+                rk[i] = *(const u32x4*)(kp + r * a.k.row);
+                rv[i] = *(const u32x4*)(vp + r * a.v.row);
+            }
+        }
+    };
+    auto store = [&](int t, unsigned long long dead) {   // masked values are zero
+#pragma unroll
+        for (int i = 0; i < CH; i++) {
+            const int r = r0 + STEP * i;
+            const unsigned live = (dead >> r) & 1 ? 0u : ~0u;
+            *(u32x4*)(lds_k[t & 1] + r * ROWB + ((ch0 ^ S::swz_k(r)) << 4)) = rk[i];
+            *(u32x4*)(lds_v[t & 1] + r * ROWB + ((ch0 ^ S::swz_v(r)) << 4)) = rv[i] & u32x4{live, live, live, live};
+        }
+    };
+    // the places of a tile that hold no key to attend to
+    auto window = [&](int t) {   // of the kWindow words from tile t's on
+        for (int w = wave; w < kWindow; w += 4) {
+            const long long j = (long long)t * BN + w * 64 + lane;
+            if (j - lane >= nk) break;
+            const unsigned long long m = __ballot(j >= nk || a.skip[k0 + (int)min(j, (long long)nk - 1)] != 0);
+            if (lane == 0) lds_dead[w] = m;
+        }
+    };
+    auto dead_of = [&](int t) -> unsigned long long {
+        unsigned long long m;
+        if (a.skip) {
+            const unsigned long long x = lds_dead[(t * (BN / 32) / 2) % kWindow] >> (BN == 32 ? (t & 1) * 32 : 0);
+            m = ((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)x);
+        } else {
+            const long long left = nk - (long long)t * BN;
+            m = left >= BN ? 0 : ~0ull << left;
+        }
+        return m & FULL;
+    };
+    constexpr int PER_WINDOW = kWindow * 64 / BN;   // tiles
+
+    unsigned long long dead = 0;   // of the tile being multiplied
     if (nt) {
-        load(0);
-        store(0);
+        if (a.skip) {
+            window(0);
+            __syncthreads();
+        }
+        dead = dead_of(0);
+        fetch(0);
     }
-    __syncthreads();
-    for (int t = 0; t < nt; t++) {
-        const int buf = t & 1;
-        if (t + 1 < nt) load(t + 1);
-        f32x16 sc[SUB];
+    u32x4 qf[QT][S::NF];
+#pragma unroll
+    for (int q = 0; q < QT; q++) load_query<T, D>(qf[q], a.q, row_place(row + 32 * q, rows, group, g, q0), h);
+    Running<T, D, UNIT> run[QT];
+#pragma unroll
+    for (int q = 0; q < QT; q++) run[q].clear();
+    if (nt) store(0, dead);
+    auto multiply = [&](int buf) {
+        f32x16 sc[SUB][QT];
+        __builtin_amdgcn_s_setprio(1);   // the matrix unit's share first: 4 % at 128 components, nothing at 64
 #pragma unroll
         for (int u = 0; u < SUB; u++) {
             const int r = u * 32 + (lane & 31);
 #pragma unroll
-            for (int e = 0; e < 16; e++) sc[u][e] = 0.f;
+            for (int q = 0; q < QT; q++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) sc[u][q][e] = 0.f;
 #pragma unroll
             for (int i = 0; i < S::NF; i++) {
                 const u32x4 kf = *(const u32x4*)(lds_k[buf] + r * ROWB + ((S::chunk(i, h) ^ S::swz_k(r)) << 4));
-                sc[u] = mfma_chunk<T>(kf, qf[i], sc[u]);
+#pragma unroll
+                for (int q = 0; q < QT; q++) sc[u][q] = mfma_chunk<T>(kf, qf[q][i], sc[u][q]);
             }
-        }
-        const unsigned long long gone = __ballot(lane < BN && lds_dead[buf][lane & (BN - 1)]);
-        if (gone) {
+            if (dead)
 #pragma unroll
-            for (int u = 0; u < SUB; u++) mask_scores(sc[u], (unsigned)(gone >> (32 * u)), h);
+                for (int q = 0; q < QT; q++) mask_scores(sc[u][q], (unsigned)(dead >> (32 * u)), h);
         }
-        run.template weights<SUB>(sc, c, slack);
+        __builtin_amdgcn_s_setprio(0);
 #pragma unroll
-        for (int u = 0; u < SUB; u++) run.add_values(sc[u], lds_v[buf], u * 32, lane);
-        if (t + 1 < nt) store(buf ^ 1);   // last read one tile ago, before the barrier below
+        for (int q = 0; q < QT; q++) {
+            f32x16 one[SUB];
+#pragma unroll
+            for (int u = 0; u < SUB; u++) one[u] = sc[u][q];
+            run[q].template weights<SUB>(one, c, slack);
+#pragma unroll
+            for (int u = 0; u < SUB; u++) sc[u][q] = one[u];
+        }
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int u = 0; u < SUB; u++) add_values<T, D, QT, UNIT>(run, sc[u], lds_v[buf], u * 32, lane);
+        __builtin_amdgcn_s_setprio(0);
+    };
+    __syncthreads();
+    for (int t = 0; t < nt; t++) {
+        const int buf = t & 1;
+        unsigned long long next = 0;
+        if (t + 1 < nt) {
+            if (a.skip && (t + 1) % PER_WINDOW == 0) {   // (all words so far have been read, before the last barrier)
+                window(t + 1);
+                __syncthreads();
+            }
+            next = dead_of(t + 1);
+            fetch(t + 1);
+        }
+        multiply(buf);
+        if (t + 1 < nt) store(t + 1, next);   // last read one tile ago, before the barrier below
+        dead = next;
         __syncthreads();
     }
-    if (row >= rows) return;
-    const float l = other_half(run.l, false);
-    store_out<T, D>(a.out, place, run.o, inverse_sum(l), h);
-    if (a.lse && h == 0) a.lse[place.q * a.q.heads + place.head] = log_sum(run.m, l, c);
+#pragma unroll
+    for (int q = 0; q < QT; q++) {
+        if (row + 32 * q >= rows) return;
+        const RowPlace place = row_place(row + 32 * q, rows, group, g, q0);
+        const float l = run[q].sum();
+        store_out<T, D>(a.out, place, run[q].o, inverse_sum(l), h);
+        if (a.lse && h == 0) a.lse[place.q * a.q.heads + place.head] = log_sum(run[q].m, l, c);
+    }
 }
 
 // A wave's own stretch of keys: operands straight from memory, values through an LDS image of its own.
@@ -181,7 +255,7 @@ template <class T, int D> struct Meeting {
 };
 template <class T, int D> __device__ __forceinline__ void meet(Meeting<T, D>& x, Running<T, D>& run, float c, int wave, int waves, int lane) {
     const int h = lane >> 5, col = lane & 31;
-    run.l = other_half(run.l, false);
+    run.l = run.sum();
     for (int w = 0; w < waves; w++) {
         if (w == wave) {
             float keep = 0.f, add = 1.f, l = run.l, m = run.m;
@@ -233,7 +307,7 @@ __global__ __launch_bounds__(256, 2) void attention_split_kernel(AttentionLaunch
     if (unit >= units) return;
     const int part = unit % parts, tile = unit / parts;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const int s = find_set(sets.tile, sets.n, tile);
+    const int s = find_set_wave(sets.tile, sets.n, tile, lane);
     const int q0 = sets.q_off[s], k0 = sets.k_off[s], nk = sets.k_off[s + 1] - k0, kvh = a.k.heads, group = a.q.heads / kvh;
     // SEL: tiles of a query's group never hold rows of another query
     const int nq = sets.q_off[s + 1] - q0, all = nq * group, per_q = (group + 31) / 32, tiles = SEL ? nq * per_q : (all + 31) / 32;
@@ -243,8 +317,8 @@ __global__ __launch_bounds__(256, 2) void attention_split_kernel(AttentionLaunch
     u32x4 qf[S::NF];
     load_query<T, D>(qf, a.q, row_place(row0 + (lane & 31), rows, group, g, q0), h);
     const float c = a.scale * kLog2e, slack = 8.f / c;
-    Running<T, D> run;
-    run.clear();
+    Running<T, D> run[1];
+    run[0].clear();
     const T* kp = (const T*)a.k.p + g * a.k.head + (long long)k0 * a.k.row;
     const T* vp = (const T*)a.v.p + g * a.v.head + (long long)k0 * a.v.row;
     const uint8_t* skip = a.skip ? a.skip + k0 : nullptr;
@@ -270,14 +344,14 @@ __global__ __launch_bounds__(256, 2) void attention_split_kernel(AttentionLaunch
         keys.scores(sc, qf, lane);
         keys.values_to_lds(lds.v[wave], lane);
         if (t + 4 < to) load(t + 4);
-        run.template weights<SUB>(sc, c, slack);
+        run[0].template weights<SUB>(sc, c, slack);
         __builtin_amdgcn_wave_barrier();   // the image is this wave's own and LDS serves a wave in order
 #pragma unroll
-        for (int u = 0; u < SUB; u++) run.add_values(sc[u], lds.v[wave], u * 32, lane);
+        for (int u = 0; u < SUB; u++) add_values<T, D, 1, false>(run, *(f32x16(*)[1])&sc[u], lds.v[wave], u * 32, lane);
         __builtin_amdgcn_wave_barrier();
     }
     __syncthreads();
-    meet(lds.sums, run, c, wave, 4, lane);
+    meet(lds.sums, run[0], c, wave, 4, lane);
     // 32 rows x D components out, 4 per thread and round
     for (int i = threadIdx.x; i < 32 * (D / 4); i += 256) {
         const int r = i / (D / 4), d = (i % (D / 4)) * 4;
@@ -494,7 +568,7 @@ __global__ __launch_bounds__(256, 2) void attention_blocks_kernel(AttentionLaunc
     // (in launch order: hardly two tiles read the same block, and a region's unused tiles would leave some XCDs without work)
     const int at = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + wave);
     if (at >= sets.tile[sets.n]) return;   // waves share nothing here: each may leave by itself
-    const int s = find_set(sets.tile, sets.n, at), kvh = a.k.heads, group = a.q.heads / kvh;
+    const int s = find_set_wave(sets.tile, sets.n, at, lane), kvh = a.k.heads, group = a.q.heads / kvh;
     const int q0 = sets.q_off[s], nq = sets.q_off[s + 1] - q0, k0 = sets.k_off[s], nk = sets.k_off[s + 1] - k0;
     const int cap = region_tiles(nq, a.n_sel, group, sets.blk[s + 1] - sets.blk[s]);
     const int g = (at - sets.tile[s]) / cap, i = (at - sets.tile[s]) % cap;
@@ -513,28 +587,28 @@ __global__ __launch_bounds__(256, 2) void attention_blocks_kernel(AttentionLaunc
     u32x4 qf[S::NF];
     load_query<T, D>(qf, a.q, RowPlace{q, head}, h);
     const float c = a.scale * kLog2e, slack = 8.f / c;
-    Running<T, D> run;
-    run.clear();
+    Running<T, D> run[1];
+    run[0].clear();
     for (int j = 0; j < n; j += BN) {
         f32x16 sc[SUB];
         keys.scores(sc, qf, lane);
         keys.values_to_lds(lds_v[wave], lane);
         if (j + BN < n) keys.load(kp, vp, a.k.row, a.v.row, skip, j + BN, n, lane);
-        run.template weights<SUB>(sc, c, slack);
+        run[0].template weights<SUB>(sc, c, slack);
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int u = 0; u < SUB; u++) run.add_values(sc[u], lds_v[wave], u * 32, lane);
+        for (int u = 0; u < SUB; u++) add_values<T, D, 1, false>(run, *(f32x16(*)[1])&sc[u], lds_v[wave], u * 32, lane);
         __builtin_amdgcn_wave_barrier();
     }
     if (row >= t.z) return;
-    const float l = other_half(run.l, false);
+    const float l = run[0].sum();
     Part<D>& to = ((Part<D>*)a.work)[((q - sets.q_off[0]) * a.q.heads + head) * a.n_sel + slot];
 #pragma unroll
     for (int u = 0; u < D / 32; u++)
 #pragma unroll
-        for (int b = 0; b < 4; b++) *(f32x4*)&to.o[u * 32 + 8 * b + 4 * h] = f32x4{run.o[u][4 * b], run.o[u][4 * b + 1], run.o[u][4 * b + 2], run.o[u][4 * b + 3]};
+        for (int b = 0; b < 4; b++) *(f32x4*)&to.o[u * 32 + 8 * b + 4 * h] = f32x4{run[0].o[u][4 * b], run[0].o[u][4 * b + 1], run[0].o[u][4 * b + 2], run[0].o[u][4 * b + 3]};
     if (h == 0) {
-        to.m = run.m;
+        to.m = run[0].m;
         to.l = l;
     }
 }
@@ -645,7 +719,8 @@ template <class T, int D> hipError_t run(const AttentionLaunch& a, AttnSets& set
     const DensePlan p = dense_plan(dtype, D, a, sets);
     if (!sets.tile[sets.n]) return hipSuccess;
     if (p.wide) {
-        attention_wide_kernel<T, D, WIDE_BN><<<xcd_grid(sets.tile[sets.n]), 256, 0, s>>>(a, sets);
+        if (a.lse || IsF32<T>::v) attention_wide_kernel<T, D, WIDE_BN, 1, false><<<xcd_grid(sets.tile[sets.n]), 256, 0, s>>>(a, sets);
+        else attention_wide_kernel<T, D, WIDE_BN, 1, !IsF32<T>::v><<<xcd_grid(sets.tile[sets.n]), 256, 0, s>>>(a, sets);
         return hipGetLastError();
     }
     attention_split_kernel<T, D, OWN_BN, false><<<xcd_grid(sets.tile[sets.n] * p.parts), 256, 0, s>>>(a, sets, p.parts);

@@ -30,6 +30,12 @@ __device__ __forceinline__ int find_set(const int* off, int n, int x) {
     }
     return lo;
 }
+// the same for an x that all 64 lanes share, in one load instead of a chain of them
+__device__ __forceinline__ int find_set_wave(const int* off, int n, int x, int lane) {
+    static_assert(PPG_ATTN_MAX_SETS == 128, "two sets per lane");
+    const int a = off[min(lane + 1, n)], b = off[min(lane + 65, n)];
+    return __popcll(__ballot(lane + 1 < n && a <= x)) + __popcll(__ballot(lane + 65 < n && b <= x));
+}
 
 template <class T> struct IsF32 { static constexpr bool v = false; };
 template <> struct IsF32<float> { static constexpr bool v = true; };
@@ -73,91 +79,135 @@ __device__ __forceinline__ float other_half(float x, bool take_max) {
 
 // Running softmax of the 32 queries of a wave, and their sums; m is the largest product seen (or up to 2^8 less in the
 // exponent: the sums are rescaled only when a product passes it by that much, which any type holds), c = scale * log2 e.
-template <class T, int D> struct Running {
+//
+// The sum of the weights: in l, added up by the vector unit, of this lane's half of the keys (the halves meet at the end); or
+// (UNIT) in every component of u, by the matrix unit, as a product with ones.
+template <class T, int D, bool UNIT = false> struct Running {
     using S = Shape<T, D>;
-    f32x16 o[D / 32];
+    f32x16 o[D / 32], u;
     float m, l;
+    __device__ __forceinline__ float sum() const { return UNIT ? u[0] : other_half(l, false); }
     __device__ __forceinline__ void clear() {
         m = -INFINITY;
         l = 0.f;
+        if constexpr (UNIT)
+#pragma unroll
+            for (int r = 0; r < 16; r++) u[r] = 0.f;
 #pragma unroll
         for (int t = 0; t < D / 32; t++)
 #pragma unroll
             for (int r = 0; r < 16; r++) o[t][r] = 0.f;
     }
-    // scores of 32 * SUB keys against the wave's queries: weights instead of them
-    template <int SUB> __device__ __forceinline__ void weights(f32x16 (&s)[SUB], float c, float slack) {
+    // largest score of this lane's query (both lane halves)
+    template <int SUB> static __device__ __forceinline__ float largest(const f32x16 (&s)[SUB]) {
         float mt = s[0][0];
 #pragma unroll
         for (int u = 0; u < SUB; u++)
 #pragma unroll
             for (int r = 0; r < 16; r++) mt = fmaxf(mt, s[u][r]);
-        mt = other_half(mt, true);
+        return other_half(mt, true);
+    }
+    // makes room for scores up to mt
+    __device__ __forceinline__ void rise(float mt, float c, float slack) {
         const bool up = mt > m + slack;
         if (__any(up)) {
             const float mn = up ? mt : m;
             const float alpha = mn == m ? 1.f : __builtin_amdgcn_exp2f((m - mn) * c);
             m = mn;
-            l *= alpha;
+            if constexpr (UNIT) {
+#pragma unroll
+                for (int r = 0; r < 16; r++) u[r] *= alpha;
+            } else {
+                l *= alpha;
+            }
 #pragma unroll
             for (int t = 0; t < D / 32; t++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) o[t][r] *= alpha;
         }
+    }
+    // weights in the place of the scores
+    template <int SUB> __device__ __forceinline__ void weigh(f32x16 (&s)[SUB], float c) {
         const float mc = m == -INFINITY ? 0.f : m * c;   // nothing so far: every weight below is exp2(-inf)
-        float sum = 0.f;
+        float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int u = 0; u < SUB; u++)
 #pragma unroll
             for (int r = 0; r < 16; r++) {
                 s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], c, -mc));
-                sum += s[u][r];
+                if constexpr (!UNIT) sum[r & 1] += s[u][r];
             }
-        l += sum;   // of this lane's half of the keys; the halves meet at the end
+        if constexpr (!UNIT) l += sum[0] + sum[1];
     }
-    // o += P V for 32 keys; v: LDS image of the values, key0 their first row in it
-    __device__ __forceinline__ void add_values(const f32x16& p, const char* v, int key0, int lane) {
-        const int h = lane >> 5;
-        if constexpr (IsF32<T>::v) {
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int row = key0 + key_of(r, h);
-#pragma unroll
-                for (int t = 0; t < D / 32; t++) {
-                    const int d = t * 32 + (lane & 31);
-                    const float a = *(const float*)(v + row * (D * 4) + ((((d >> 2) ^ S::swz_v(row)) << 4) | ((d & 3) << 2)));
-                    o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], o[t], 0, 0, 0);
-                }
-            }
-        } else {
-            const int i = lane & 15, part = (lane >> 4) & 1;
-#pragma unroll
-            for (int st = 0; st < 2; st++) {
-                T pb[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) pb[e] = (T)p[8 * st + e];   // the weights' one rounding
-                const u32x4 b = __builtin_bit_cast(u32x4, pb);
-                const int r0 = key0 + 16 * st + 4 * h + (i >> 2), r1 = r0 + 8;
-#pragma unroll
-                for (int t = 0; t < D / 32; t++) {
-                    const int ch = t * 4 + part * 2 + ((i & 3) >> 1), in = (i & 1) * 8;
-                    const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(v + r0 * (D * 2) + ((ch ^ S::swz_v(r0)) << 4) + in));
-                    const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(v + r1 * (D * 2) + ((ch ^ S::swz_v(r1)) << 4) + in));
-                    const s16x8 a = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
-                    o[t] = mfma_chunk<T>(__builtin_bit_cast(u32x4, a), b, o[t]);
-                }
-            }
-        }
+    template <int SUB> __device__ __forceinline__ void weights(f32x16 (&s)[SUB], float c, float slack) {
+        rise(largest(s), c, slack);
+        weigh(s, c);
     }
 };
 
-// scores of masked keys (bit set in `dead`, bit 0 = the tile's first key) become -inf, whatever the product gave
-__device__ __forceinline__ void mask_scores(f32x16& s, unsigned dead, int h) {
-    const int d = (int)(dead >> (4 * h));
+// o += P V of 32 keys for QT groups of 32 queries; v: LDS image of the values, key0 the keys' first row in it.  The weights are
+// rounded to the values' type here, once.
+template <class T, int D, int QT, bool UNIT>
+__device__ __forceinline__ void add_values(Running<T, D, UNIT> (&run)[QT], const f32x16 (&p)[QT], const char* v, int key0, int lane) {
+    using S = Shape<T, D>;
+    const int h = lane >> 5;
+    if constexpr (IsF32<T>::v) {
+        static_assert(!UNIT, "the 32-bit matrix unit is the bottleneck: sums are the vector unit's");
 #pragma unroll
-    for (int r = 0; r < 16; r++) {
-        const unsigned x = (unsigned)((d << (31 - key_of(r, 0))) >> 31);   // all ones where masked
-        s[r] = __uint_as_float((__float_as_uint(s[r]) & ~x) | (0xff800000u & x));
+        for (int r = 0; r < 16; r++) {
+            const int row = key0 + key_of(r, h);
+#pragma unroll
+            for (int t = 0; t < D / 32; t++) {
+                const int d = t * 32 + (lane & 31);
+                const float a = *(const float*)(v + row * (D * 4) + ((((d >> 2) ^ S::swz_v(row)) << 4) | ((d & 3) << 2)));
+#pragma unroll
+                for (int q = 0; q < QT; q++) run[q].o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[q][r], run[q].o[t], 0, 0, 0);
+            }
+        }
+    } else {
+        const int i = lane & 15, part = (lane >> 4) & 1;
+#pragma unroll
+        for (int st = 0; st < 2; st++) {
+            u32x4 b[QT];
+#pragma unroll
+            for (int q = 0; q < QT; q++) {
+                T pb[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) pb[e] = (T)p[q][8 * st + e];
+                b[q] = __builtin_bit_cast(u32x4, pb);
+            }
+            if constexpr (UNIT) {
+                const short one = __builtin_bit_cast(short, (T)1.f);
+                const s16x8 ones = {one, one, one, one, one, one, one, one};
+#pragma unroll
+                for (int q = 0; q < QT; q++) run[q].u = mfma_chunk<T>(__builtin_bit_cast(u32x4, ones), b[q], run[q].u);
+            }
+            const int r0 = key0 + 16 * st + 4 * h + (i >> 2), r1 = r0 + 8;
+#pragma unroll
+            for (int t = 0; t < D / 32; t++) {
+                const int ch = t * 4 + part * 2 + ((i & 3) >> 1), in = (i & 1) * 8;
+                const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(v + r0 * (D * 2) + ((ch ^ S::swz_v(r0)) << 4) + in));
+                const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(v + r1 * (D * 2) + ((ch ^ S::swz_v(r1)) << 4) + in));
+                const s16x8 a = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                for (int q = 0; q < QT; q++) run[q].o[t] = mfma_chunk<T>(__builtin_bit_cast(u32x4, a), b[q], run[q].o[t]);
+            }
+        }
+    }
+}
+
+// Scores of masked keys (bit set in `dead`, the same for the wave; bit 0 = the tile's first key) become -inf, whatever the product
+// gave.  Eight keys at a time, four of each lane half: with few keys masked most groups cost a scalar test.
+__device__ __forceinline__ void mask_scores(f32x16& s, unsigned dead, int h) {
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+        if (!((dead >> (8 * b)) & 0xff)) continue;
+        const int d = (int)((dead >> (8 * b)) >> (4 * h));
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const unsigned x = (unsigned)((d << (31 - e)) >> 31);   // all ones where masked
+            s[4 * b + e] = __uint_as_float(__builtin_amdgcn_bitop3_b32(x, 0xff800000u, __float_as_uint(s[4 * b + e]), 0xca));   // x ? -inf : s
+        }
     }
 }
 

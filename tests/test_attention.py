@@ -406,6 +406,10 @@ SHAPES = [
     (64, 6, 2, [37], [500], 0.0), (64, 16, 1, [1], [3001], 0.05), (128, 8, 8, [1, 1], [2500, 1300], 0.0), (64, 4, 4, [500], [487], 0.0),
     (32, 1, 1, [700], [1025], 0.2), (64, 2, 2, [3] * 40, list(range(0, 160, 4)), 0.1), (64, 4, 1, [2], [20000], 0.9), (128, 5, 5, [64], [777], 1.0),
     (64, 1, 1, [1030], [2050], 0.03), (64, 4, 4, [257] * 9, [255] * 9, 0.03),
+    # enough rows for the kernel that shares tiles between 128 of them: more keys than its mask window, every tail, shared key heads
+    (64, 2, 2, [130] + [129] * 127, [4500] + [40] * 127, 0.05), (128, 2, 2, [130] + [129] * 127, [4500] + list(range(127)), 0.3),
+    (32, 4, 4, [100, 129, 1, 0] * 32, [65, 0, 127, 3] * 31 + [64, 63, 8200, 1], 0.0), (64, 12, 4, [90, 129] * 20, [33, 64] * 20, 0.5),
+    (128, 8, 2, [300] * 22, [130, 1] * 11, 0.0),
 ]
 
 
@@ -431,6 +435,9 @@ def test_attention_whole_sets(gpu, dtype, shape):
     a, b = q_off[0], q_off[-1]
     assert (out[:a] == 3).all() and (out[b:] == 3).all() and (lse[:a] == 3).all() and (lse[b:] == 3).all()
     _check_attend(torch, dtype, out[a:b], lse[a:b], [x[a:b] for x in ref])
+    out, _ = _run_attention(gpu, dtype, q.cuda(), k.cuda(), v.cuda(), scale, q_off, k_off, None if skip is None else skip.cuda(), lse=False)
+    assert (out[:a] == 3).all() and (out[b:] == 3).all()
+    _check_attend(torch, dtype, out[a:b], None, [x[a:b] for x in ref])
 
 
 @pytest.mark.gpu

@@ -3,6 +3,8 @@
 #include "attn_tile.h"
 #include "wave_util.h"
 
+#include <algorithm>
+
 namespace ppg {
 
 // ---- element types ----
@@ -256,7 +258,7 @@ __device__ __forceinline__ float key_float(unsigned k) {
     return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k);
 }
 
-// A work-group selects for 32 query rows of one (set, key head).  The products of all 32 with a stretch of blocks come from the
+// A work-group selects for ROWS query rows of one (set, key head).  The products of all of them with a stretch of blocks come from the
 // bf16 matrix unit, both inputs split into two halves and three of the four products taken: off by at most
 // E = 2^-13 |q| |mean| (Cauchy-Schwarz; what is left out is below 3 * 2^-16, the 32-bit sums of up to 384 terms below
 // 2^-15).  They stay in LDS.  Then a wave takes a row: the n_sel-th largest of (product - E) is a bound t that the n_sel best
@@ -264,10 +266,10 @@ __device__ __forceinline__ float key_float(unsigned k) {
 // answer; else they are scored in 64 bits and ranked exactly.  Rows for which that does not hold together (a product that is
 // not finite, or more than 128 left, as with many equal means) go the plain way.
 // 8 streams of 1024 rows against 65537 keys (1025 blocks), 4 heads of 64: LDS_TIME.
-constexpr int kSelRows = 32, kSelChunk = 1088, kSelWaves = 16, kSelPitch = kSelChunk + 4;
+constexpr int kSelWaves = 16;
 // A row's scores, and once its wave has them in registers, that wave's notes: the blocks left, their bounds, their exact keys.
-union SelectRow {
-    float score[kSelPitch];
+template <int PER> union SelectRow {
+    float score[PER * 64 + 4];
     struct {
         unsigned short cand[128];
         float low[128], high[128];
@@ -276,23 +278,23 @@ union SelectRow {
         int best_idx[64];
     } note;
 };
-template <int D> struct SelectLds {
-    SelectRow row[kSelRows];
-    float norm[kSelChunk];                 // |mean|, -1 for a block that cannot be selected
-    char q[2][kSelRows * D * 2];           // the summed queries' upper and lower halves, chunks permuted against bank conflicts
+template <int D, int ROWS, int PER> struct SelectLds {
+    SelectRow<PER> row[ROWS];
+    float norm[PER * 64];                 // |mean|, -1 for a block that cannot be selected
+    char q[2][ROWS * D * 2];           // the summed queries' upper and lower halves, chunks permuted against bank conflicts
 };
-template <class T, int D>
+template <class T, int D, int ROWS, int PER>
 __global__ __launch_bounds__(1024, 4) void block_select_kernel(BlockSelectLaunch a, AttnSets sets) {
-    constexpr int PER = kSelChunk / 64, RPW = kSelRows / kSelWaves, N = 16 / (int)sizeof(T);
+    constexpr int CHUNK = PER * 64, RPW = ROWS / kSelWaves, N = 16 / (int)sizeof(T);
     constexpr int LPC = D / 16, CPP = 64 / LPC;   // lanes that share a candidate's product, candidates of a pass
-    __shared__ alignas(16) SelectLds<D> lds;
+    __shared__ alignas(16) SelectLds<D, ROWS, PER> lds;
     const int unit = xcd_unit(blockIdx.x, sets.tile[sets.n]);
     if (unit >= sets.tile[sets.n]) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, s = find_set(sets.tile, sets.n, unit);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, s = find_set_wave(sets.tile, sets.n, unit, lane);
     const int q0 = sets.q_off[s], nq = sets.q_off[s + 1] - q0;
     // the heads in turn: work-groups that run at the same time then read whole rows of means between them, and with those all
     // channels of the L2
-    const int g = (unit - sets.tile[s]) % a.kv_heads, row0 = ((unit - sets.tile[s]) / a.kv_heads) * kSelRows;
+    const int g = (unit - sets.tile[s]) % a.kv_heads, row0 = ((unit - sets.tile[s]) / a.kv_heads) * ROWS;
     const int group = a.q.heads / a.kv_heads, nb = sets.blk[s + 1] - sets.blk[s];
     const float* mean = a.mean + ((long long)sets.blk[s] * a.kv_heads + g) * D;
     const long long stride = (long long)a.kv_heads * D;
@@ -321,8 +323,8 @@ __global__ __launch_bounds__(1024, 4) void block_select_kernel(BlockSelectLaunch
         best[i] = Scored{0, 0x7fffffff};
     }
 
-    for (int b0 = 0; b0 < nb; b0 += kSelChunk) {
-        const int n = min(kSelChunk, nb - b0);
+    for (int b0 = 0; b0 < nb; b0 += CHUNK) {
+        const int n = min(CHUNK, nb - b0);
         f32x4 mx[D / 32][2];
         bool alive = false;
         auto load = [&](int t) {
@@ -338,7 +340,7 @@ __global__ __launch_bounds__(1024, 4) void block_select_kernel(BlockSelectLaunch
         if (wave * 16 < n) load(wave);
         __syncthreads();   // the queries are in LDS; the last stretch has been read
         for (int t = wave; t * 16 < n; t += kSelWaves) {
-            f32x4 acc[2] = {};
+            f32x4 acc[RPW] = {};
             float sm = 0.f;
             bf16x8 mh[D / 32], ml[D / 32];
 #pragma unroll
@@ -353,7 +355,7 @@ __global__ __launch_bounds__(1024, 4) void block_select_kernel(BlockSelectLaunch
             const bool on = alive;
             if ((t + kSelWaves) * 16 < n) load(t + kSelWaves);
 #pragma unroll
-            for (int rt = 0; rt < 2; rt++) {
+            for (int rt = 0; rt < RPW; rt++) {
 #pragma unroll
                 for (int k = 0; k < D / 32; k++) {
                     const int r = rt * 16 + (lane & 15), ch = k * 4 + (lane >> 4);
@@ -369,7 +371,7 @@ __global__ __launch_bounds__(1024, 4) void block_select_kernel(BlockSelectLaunch
             // (as short a mean as the query above: NaN, which sends the rows the plain way)
             if (lane < 16) lds.norm[t * 16 + lane] = on ? (sm < 1e-24f && sm > 0.f ? NAN : sqrtf(sm) * 1.0001f) : -1.f;
         }
-        for (int b = (n + 15) / 16 * 16 + threadIdx.x; b < kSelChunk; b += 1024) lds.norm[b] = -1.f;
+        for (int b = (n + 15) / 16 * 16 + threadIdx.x; b < CHUNK; b += 1024) lds.norm[b] = -1.f;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < RPW; i++) {
@@ -481,7 +483,7 @@ __global__ __launch_bounds__(1024, 4) void block_select_kernel(BlockSelectLaunch
                     cand[k] = in[k] ? note.cand[k * 64 + lane] : -1;
                 }
             }
-            const bool choose = b0 || nb > kSelChunk || left > a.n_sel;   // (keys for the stretches to come, too)
+            const bool choose = b0 || nb > CHUNK || left > a.n_sel;   // (keys for the stretches to come, too)
             if (!choose) {
                 best[i] = in[0] ? Scored{1, cand[0]} : Scored{0, 0x7fffffff};   // (at most n_sel of them, in order)
                 continue;
@@ -613,11 +615,22 @@ hipError_t launch_block_means(int dtype, int head_dim, const BlockMeansLaunch& a
 }
 
 hipError_t launch_block_select(int dtype, int head_dim, const BlockSelectLaunch& a, AttnSets& sets, hipStream_t s) {
-    sets.tile[0] = 0;
-    for (int i = 0; i < sets.n; i++)
-        sets.tile[i + 1] = sets.tile[i] + (int)(((long long)sets.q_off[i + 1] - sets.q_off[i] + kSelRows - 1) / kSelRows * a.kv_heads);
-    if (!sets.tile[sets.n]) return hipSuccess;
-    BY_TYPE(dtype, BY_DIM(head_dim, (block_select_kernel<T, D><<<xcd_grid(sets.tile[sets.n]), 1024, 0, s>>>(a, sets))));
+    auto tiles = [&](int rows) {
+        sets.tile[0] = 0;
+        for (int i = 0; i < sets.n; i++)
+            sets.tile[i + 1] = sets.tile[i] + (int)(((long long)sets.q_off[i + 1] - sets.q_off[i] + rows - 1) / rows * a.kv_heads);
+        return sets.tile[sets.n];
+    };
+    int most = 0;
+    for (int i = 0; i < sets.n; i++) most = std::max(most, sets.blk[i + 1] - sets.blk[i]);
+    // a row per wave where that still leaves CUs without work (one frame of 500 rows and 4 heads SEL16_TIME), else two, which read
+    // the means half as often (8 streams SEL32_TIME); few blocks: as many registers as those take
+#define SELECT(ROWS, PER) BY_TYPE(dtype, BY_DIM(head_dim, (block_select_kernel<T, D, ROWS, PER><<<xcd_grid(sets.tile[sets.n]), 1024, 0, s>>>(a, sets))))
+    if (tiles(32) >= 256) SELECT(32, 17);
+    else if (!tiles(16)) return hipSuccess;
+    else if (most <= 5 * 64) SELECT(16, 5);
+    else SELECT(16, 17);
+#undef SELECT
     return hipGetLastError();
 }
 

@@ -461,8 +461,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, 
 // A region is one (set, key head); entry e of it is place e % n_sel in the list of its query e / n_sel.  Where things lie:
 struct BinWork {
     int* list;     // entries by block, [regions][queries of the set * n_sel]
-    int4* tile;    // (block, first entry in the region's list, rows of the block = entries * group, first row of the tile)
-    int* tiles;    // tiles of a region
+    int4* tile;    // (block, first entry in the region's list, rows of the block = entries * group, first row of the tile); block -1: unused
 };
 // tiles that a region may need: its rows in 32s, and one more for every block's last
 __host__ __device__ inline int region_tiles(long long nq, int n_sel, int group, int blocks) {
@@ -555,7 +554,8 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
         }
         __syncthreads();
     }
-    if (tid == 0) w.tiles[blockIdx.x] = t0;
+    const int cap = region_tiles(nq, a.n_sel, group, blocks);
+    for (int i = t0 + tid; i < cap; i += 1024) tile[i] = make_int4(-1, 0, 0, 0);
 }
 
 // A wave per tile: one block's keys against 32 rows out of the queries that name it.
@@ -571,9 +571,9 @@ __global__ __launch_bounds__(256, 2) void attention_blocks_kernel(AttentionLaunc
     const int s = find_set_wave(sets.tile, sets.n, at, lane), kvh = a.k.heads, group = a.q.heads / kvh;
     const int q0 = sets.q_off[s], nq = sets.q_off[s + 1] - q0, k0 = sets.k_off[s], nk = sets.k_off[s + 1] - k0;
     const int cap = region_tiles(nq, a.n_sel, group, sets.blk[s + 1] - sets.blk[s]);
-    const int g = (at - sets.tile[s]) / cap, i = (at - sets.tile[s]) % cap;
-    if (i >= w.tiles[s * kvh + g]) return;
+    const int g = (at - sets.tile[s]) / cap;
     const int4 t = w.tile[at];
+    if (t.x < 0) return;
     const int first = t.x * a.block, n = min(a.block, nk - first);
     const T* kp = (const T*)a.k.p + g * a.k.head + (long long)(k0 + first) * a.k.row;
     const T* vp = (const T*)a.v.p + g * a.v.head + (long long)(k0 + first) * a.v.row;
@@ -636,8 +636,8 @@ DensePlan dense_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSets
     long long longest = 0;
     for (int s = 0; s < sets.n; s++) longest = std::max(longest, (long long)sets.k_off[s + 1] - sets.k_off[s]);
     const int bn = dtype == PPG_F32 || head_dim == 128 ? 32 : 64;
-    // a part has a tile for each of its waves at least
-    const long long most = std::max(1LL, longest / (4 * bn));
+    // a part has a tile for each of its waves
+    const long long most = std::max(1LL, (longest + 4 * bn - 1) / (4 * bn));
     return {false, (int)std::min<long long>(most, units ? (kFill + units - 1) / units : 1)};
 }
 
@@ -646,7 +646,7 @@ DensePlan dense_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSets
 struct BlocksPlan {
     bool binned;
     int parts;
-    size_t part_bytes, list_bytes, tile_bytes, tiles_bytes;   // of the binned form, in this order
+    size_t part_bytes, list_bytes, tile_bytes;   // of the binned form, in this order
 };
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 // Below this many list entries a query's blocks are read for itself: one launch instead of three
@@ -664,13 +664,12 @@ BlocksPlan blocks_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSe
         p.part_bytes = up256((size_t)nq * a.q.heads * a.n_sel * part);
         p.list_bytes = up256((size_t)nq * kvh * a.n_sel * sizeof(int));
         p.tile_bytes = up256((size_t)sets.tile[sets.n] * sizeof(int4));
-        p.tiles_bytes = up256((size_t)sets.n * kvh * sizeof(int));
         return p;
     }
     const long long per_q = (group + 31) / 32;
     for (int s = 0; s < sets.n; s++) sets.tile[s + 1] = sets.tile[s] + (int)((sets.q_off[s + 1] - sets.q_off[s]) * per_q * kvh);
     const int units = sets.tile[sets.n], bn = dtype == PPG_F32 || head_dim == 128 ? 32 : 64;
-    const long long most = std::max(1LL, (long long)a.n_sel * ((a.block + bn - 1) / bn) / 4);
+    const long long most = std::max(1LL, ((long long)a.n_sel * ((a.block + bn - 1) / bn) + 3) / 4);
     p.parts = (int)std::min<long long>(most, units ? (kFill + units - 1) / units : 1);
     if (p.parts > 1) p.part_bytes = (size_t)nq * a.q.heads * p.parts * part;
     return p;
@@ -707,7 +706,6 @@ template <class T, int D> hipError_t run(const AttentionLaunch& a, AttnSets& set
         BinWork w;
         w.list = (int*)((char*)a.work + p.part_bytes);
         w.tile = (int4*)((char*)w.list + p.list_bytes);
-        w.tiles = (int*)((char*)w.tile + p.tile_bytes);
         if (sets.tile[sets.n]) {
             bin_kernel<<<sets.n * a.k.heads, 1024, 0, s>>>(a, sets, w);
             if ((e = hipGetLastError()) != hipSuccess) return e;
@@ -736,7 +734,7 @@ template <class T> hipError_t run_dim(const AttentionLaunch& a, AttnSets& sets, 
 size_t attention_work(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets) {
     if (a.n_sel) {
         const BlocksPlan p = blocks_plan(dtype, head_dim, a, sets);
-        return p.part_bytes + p.list_bytes + p.tile_bytes + p.tiles_bytes;
+        return p.part_bytes + p.list_bytes + p.tile_bytes;
     }
     const DensePlan p = dense_plan(dtype, head_dim, a, sets);
     return p.parts == 1 ? 0 : ((size_t)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads * p.parts * (head_dim + 4) * sizeof(float);

@@ -12,6 +12,7 @@
 #include "attn_tile.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace ppg {
 
@@ -211,24 +212,26 @@ template <class T, int D, int BN> struct OwnKeys {
     using S = Shape<T, D>;
     static constexpr int SUB = BN / 32, VC = BN * S::CPR / 64, ROWB = D * (int)sizeof(T);
     u32x4 rk[SUB][S::NF], rv[VC];
-    unsigned long long gone;
+    int masked;                  // this lane's key of the tile (the first BN lanes)
+    unsigned long long gone;     // all of them, once settle() was called
     // keys j0 .. j0 + BN - 1 of the set at kp / vp, of which n exist (n >= 1: row n - 1 stands in for those behind it)
     __device__ __forceinline__ void load(const T* kp, const T* vp, long long k_row, long long v_row, const uint8_t* skip, int j0, int n, int lane) {
-        const int h = lane >> 5;
+        const int h = lane >> 5, j = j0 + (lane & (BN - 1));
+        masked = skip ? skip[min(j, n - 1)] : 0;   // first: loads come back in order, and this one is waited for first
+        if (j >= n) masked = 1;
 #pragma unroll
         for (int u = 0; u < SUB; u++) {
             const T* x = kp + (long long)min(j0 + u * 32 + (lane & 31), n - 1) * k_row;
 #pragma unroll
             for (int i = 0; i < S::NF; i++) rk[u][i] = *(const u32x4*)(x + S::chunk(i, h) * S::N);
         }
-        const int j = j0 + (lane & (BN - 1));
-        gone = __ballot(lane < BN && (j >= n || (skip && skip[min(j, n - 1)])));
 #pragma unroll
         for (int i = 0; i < VC; i++) {
             const int x = lane + 64 * i, r = x / S::CPR;
             rv[i] = *(const u32x4*)(vp + (long long)min(j0 + r, n - 1) * v_row + (x % S::CPR) * S::N);
         }
     }
+    __device__ __forceinline__ void settle(int lane) { gone = __ballot(lane < BN && masked); }
     __device__ __forceinline__ void values_to_lds(char* v, int lane) const {
 #pragma unroll
         for (int i = 0; i < VC; i++) {
@@ -294,6 +297,17 @@ template <int D> struct Part {
     float pad[2];
 };
 
+// The same for a selected block of a query, with 16-bit types: the mean of the values (o / l) in fp16, times a power of two that
+// brings the largest into [2^13, 2^14) where the values' own type reaches further than fp16.  That is off by 2^-11 of each
+// component (and 2^-38 of the largest), where the result is rounded to 2^-11 (fp16) or 2^-8 (bf16) anyway; it halves what is
+// written and read between the two kernels (8 streams: PARTH_TIME).
+template <int D> struct PartH {
+    _Float16 o[D];
+    float m, l, scale;   // o * scale is the mean
+    float pad;
+};
+template <class T, int D> using ListPart = std::conditional_t<IsF32<T>::v, Part<D>, PartH<D>>;
+
 // SEL: a unit's rows are the group of one query, its keys the blocks of that query's list.
 template <class T, int D, int BN, bool SEL>
 __global__ __launch_bounds__(256, 2) void attention_split_kernel(AttentionLaunch a, AttnSets sets, int parts) {
@@ -333,7 +347,7 @@ __global__ __launch_bounds__(256, 2) void attention_split_kernel(AttentionLaunch
             const bool ok = b >= 0 && b < blocks;
             const int first = ok ? b * a.block : 0, n = min(a.block, nk - first);
             keys.load(kp + first * a.k.row, vp + first * a.v.row, a.k.row, a.v.row, skip ? skip + first : nullptr, j, n, lane);
-            if (!ok) keys.gone = ~0ull;
+            if (!ok) keys.masked = 1;
         } else {
             keys.load(kp, vp, a.k.row, a.v.row, skip, t * BN, nk, lane);
         }
@@ -341,6 +355,7 @@ __global__ __launch_bounds__(256, 2) void attention_split_kernel(AttentionLaunch
     if (from + wave < to) load(from + wave);
     for (int t = from + wave; t < to; t += 4) {
         f32x16 sc[SUB];
+        keys.settle(lane);
         keys.scores(sc, qf, lane);
         keys.values_to_lds(lds.v[wave], lane);
         if (t + 4 < to) load(t + 4);
@@ -394,7 +409,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, 
     const long long n = ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads, at = (long long)blockIdx.x * (TEAMS / PG) + team / PG;
     const long long rh = min(at, n - 1);   // (a team behind the last does its work again and keeps it to itself)
     const float c = a.scale * kLog2e;
-    const Part<D>* w = (const Part<D>*)a.work + rh * parts;
+    using P = std::conditional_t<SEL, ListPart<T, D>, Part<D>>;
+    constexpr bool HALF = !__is_same(P, Part<D>);   // o is a mean there, a sum here
+    const P* w = (const P*)a.work + rh * parts;
     const long long q = sets.q_off[0] + rh / a.q.heads;
     const int head = (int)(rh % a.q.heads);
     int blocks = 0;
@@ -412,9 +429,16 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, 
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int p = min(p0 + i * PG, parts - 1);
-            x[i].o = *(const f32x4*)&w[p].o[d];
             x[i].m = w[p].m;
             x[i].l = w[p].l;
+            if constexpr (HALF) {
+                typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+                const f16x4 v = *(const f16x4*)&w[p].o[d];
+                const float f = w[p].scale * x[i].l;
+                x[i].o = f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]} * f;
+            } else {
+                x[i].o = *(const f32x4*)&w[p].o[d];
+            }
             on[i] = p0 + i * PG < parts;
             if constexpr (SEL) on[i] = on[i] && (unsigned)sel[p] < (unsigned)blocks;
         }
@@ -484,7 +508,8 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
     int4* tile = w.tile + sets.tile[s] + (long long)g * region_tiles(nq, a.n_sel, group, blocks);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int e0 = 0, t0 = 0;   // entries and tiles of the bins before this round's
-    int held[kBinHold];
+    int held[kBinHold], rank[kBinHold];
+    const bool once = n <= kBinHold * 1024;
     const int dq = 1024 / a.n_sel, dr = 1024 % a.n_sel;   // 1024 entries on, in queries and places
     auto load = [&](int from) {
         int q = (from + tid) / a.n_sel, r = (from + tid) % a.n_sel;
@@ -505,10 +530,10 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
         if (b0 == 0) load(0);
         __syncthreads();
         for (int from = 0; from < n; from += kBinHold * 1024) {
-            if (n > kBinHold * 1024) load(from);
+            if (!once) load(from);
 #pragma unroll
             for (int i = 0; i < kBinHold; i++)
-                if ((unsigned)(held[i] - b0) < (unsigned)nb && held[i] >= b0) atomicAdd(&cnt[held[i] - b0], 1);
+                if (held[i] >= b0 && held[i] - b0 < nb) rank[i] = atomicAdd(&cnt[held[i] - b0], 1);
         }
         __syncthreads();
         int es = 0, ts = 0;
@@ -547,10 +572,10 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
         }
         __syncthreads();
         for (int from = 0; from < n; from += kBinHold * 1024) {
-            if (n > kBinHold * 1024) load(from);
+            if (!once) load(from);
 #pragma unroll
             for (int i = 0; i < kBinHold; i++)
-                if ((unsigned)(held[i] - b0) < (unsigned)nb && held[i] >= b0) list[atomicAdd(&cnt[held[i] - b0], 1)] = from + i * 1024 + tid;
+                if (held[i] >= b0 && held[i] - b0 < nb) list[once ? cnt[held[i] - b0] + rank[i] : atomicAdd(&cnt[held[i] - b0], 1)] = from + i * 1024 + tid;
         }
         __syncthreads();
     }
@@ -560,14 +585,13 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
 
 // A wave per tile: one block's keys against 32 rows out of the queries that name it.
 template <class T, int D, int BN>
-__global__ __launch_bounds__(256, 2) void attention_blocks_kernel(AttentionLaunch a, AttnSets sets, BinWork w) {
+__global__ __launch_bounds__(64, 2) void attention_blocks_kernel(AttentionLaunch a, AttnSets sets, BinWork w) {
     using S = Shape<T, D>;
     constexpr int SUB = BN / 32, IMG = BN * D * (int)sizeof(T);
-    __shared__ alignas(16) char lds_v[4][IMG];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    __shared__ alignas(16) char lds_v[IMG];
+    const int lane = threadIdx.x, h = lane >> 5;
     // (in launch order: hardly two tiles read the same block, and a region's unused tiles would leave some XCDs without work)
-    const int at = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + wave);
-    if (at >= sets.tile[sets.n]) return;   // waves share nothing here: each may leave by itself
+    const int at = (int)blockIdx.x;
     const int s = find_set_wave(sets.tile, sets.n, at, lane), kvh = a.k.heads, group = a.q.heads / kvh;
     const int q0 = sets.q_off[s], nq = sets.q_off[s + 1] - q0, k0 = sets.k_off[s], nk = sets.k_off[s + 1] - k0;
     const int cap = region_tiles(nq, a.n_sel, group, sets.blk[s + 1] - sets.blk[s]);
@@ -591,22 +615,48 @@ __global__ __launch_bounds__(256, 2) void attention_blocks_kernel(AttentionLaunc
     run[0].clear();
     for (int j = 0; j < n; j += BN) {
         f32x16 sc[SUB];
+        keys.settle(lane);
         keys.scores(sc, qf, lane);
-        keys.values_to_lds(lds_v[wave], lane);
+        keys.values_to_lds(lds_v, lane);
         if (j + BN < n) keys.load(kp, vp, a.k.row, a.v.row, skip, j + BN, n, lane);
         run[0].template weights<SUB>(sc, c, slack);
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int u = 0; u < SUB; u++) add_values<T, D, 1, false>(run, *(f32x16(*)[1])&sc[u], lds_v[wave], u * 32, lane);
+        for (int u = 0; u < SUB; u++) add_values<T, D, 1, false>(run, *(f32x16(*)[1])&sc[u], lds_v, u * 32, lane);
         __builtin_amdgcn_wave_barrier();
     }
-    if (row >= t.z) return;
     const float l = run[0].sum();
-    Part<D>& to = ((Part<D>*)a.work)[((q - sets.q_off[0]) * a.q.heads + head) * a.n_sel + slot];
+    if (row >= t.z) return;   // (both lane halves of a row leave together)
+    ListPart<T, D>& to = ((ListPart<T, D>*)a.work)[((q - sets.q_off[0]) * a.q.heads + head) * a.n_sel + slot];
+    if constexpr (IsF32<T>::v) {
 #pragma unroll
-    for (int u = 0; u < D / 32; u++)
+        for (int u = 0; u < D / 32; u++)
 #pragma unroll
-        for (int b = 0; b < 4; b++) *(f32x4*)&to.o[u * 32 + 8 * b + 4 * h] = f32x4{run[0].o[u][4 * b], run[0].o[u][4 * b + 1], run[0].o[u][4 * b + 2], run[0].o[u][4 * b + 3]};
+            for (int b = 0; b < 4; b++) *(f32x4*)&to.o[u * 32 + 8 * b + 4 * h] = f32x4{run[0].o[u][4 * b], run[0].o[u][4 * b + 1], run[0].o[u][4 * b + 2], run[0].o[u][4 * b + 3]};
+    } else {
+        float f = inverse_sum(l), scale = 1.f;
+        if constexpr (__is_same(T, __bf16)) {
+            float most = 0.f;   // of the finite ones
+#pragma unroll
+            for (int u = 0; u < D / 32; u++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const float x = fabsf(run[0].o[u][r] * f);
+                    most = fmaxf(most, x < INFINITY ? x : 0.f);
+                }
+            const int e = max((int)(__float_as_uint(other_half(most, true)) >> 23), 14);   // biased exponent
+            scale = __uint_as_float((unsigned)(e - 13) << 23);
+            f *= __uint_as_float((unsigned)(267 - e) << 23);
+        }
+        typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int u = 0; u < D / 32; u++)
+#pragma unroll
+            for (int b = 0; b < 4; b++)
+                *(f16x4*)&to.o[u * 32 + 8 * b + 4 * h] = f16x4{(_Float16)(run[0].o[u][4 * b] * f), (_Float16)(run[0].o[u][4 * b + 1] * f),
+                                                              (_Float16)(run[0].o[u][4 * b + 2] * f), (_Float16)(run[0].o[u][4 * b + 3] * f)};
+        if (h == 0) to.scale = scale;
+    }
     if (h == 0) {
         to.m = run[0].m;
         to.l = l;
@@ -653,7 +703,7 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 constexpr long long kBinnedFrom = 512;
 BlocksPlan blocks_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets) {
     const long long nq = (long long)sets.q_off[sets.n] - sets.q_off[0], kvh = a.k.heads, group = a.q.heads / kvh;
-    const size_t part = (size_t)(head_dim + 4) * sizeof(float);
+    const size_t part = (size_t)(head_dim + 4) * sizeof(float), list_part = dtype == PPG_F32 ? part : (size_t)head_dim * 2 + 16;
     BlocksPlan p{};
     sets.tile[0] = 0;
     if (nq * kvh * a.n_sel >= kBinnedFrom) {
@@ -661,7 +711,7 @@ BlocksPlan blocks_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSe
         p.parts = a.n_sel;
         for (int s = 0; s < sets.n; s++)
             sets.tile[s + 1] = sets.tile[s] + (int)kvh * region_tiles(sets.q_off[s + 1] - sets.q_off[s], a.n_sel, (int)group, sets.blk[s + 1] - sets.blk[s]);
-        p.part_bytes = up256((size_t)nq * a.q.heads * a.n_sel * part);
+        p.part_bytes = up256((size_t)nq * a.q.heads * a.n_sel * list_part);
         p.list_bytes = up256((size_t)nq * kvh * a.n_sel * sizeof(int));
         p.tile_bytes = up256((size_t)sets.tile[sets.n] * sizeof(int4));
         return p;
@@ -709,7 +759,7 @@ template <class T, int D> hipError_t run(const AttentionLaunch& a, AttnSets& set
         if (sets.tile[sets.n]) {
             bin_kernel<<<sets.n * a.k.heads, 1024, 0, s>>>(a, sets, w);
             if ((e = hipGetLastError()) != hipSuccess) return e;
-            attention_blocks_kernel<T, D, OWN_BN><<<(unsigned)((sets.tile[sets.n] + 3) / 4), 256, 0, s>>>(a, sets, w);
+            attention_blocks_kernel<T, D, OWN_BN><<<(unsigned)sets.tile[sets.n], 64, 0, s>>>(a, sets, w);
             if ((e = hipGetLastError()) != hipSuccess) return e;
         }
         return join<T, D>(a, sets, p.parts, true, s);

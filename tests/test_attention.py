@@ -6,7 +6,10 @@ n keys and D components: a product q.k in 32 bits is off by at most (D + 4) 2^-2
 2^-23 of itself; the weights therefore by a factor 1 + 4 E with E the largest of those (twice for numerator and
 denominator, twice for the maximum that is subtracted).  Sums over the keys are taken in tiles of at least 32, so they add
 at most (n / 32 + 64) roundings.  With 16-bit types a weight is rounded once (u of the type; below fp16's smallest normal
-number 2^-25 absolutely, with a denominator of at least 1), and the result once more.  A stands for sum p |v|."""
+number 2^-25 absolutely, with a denominator of at least 1), and the result once more.  A stands for sum p |v|.  Selected
+blocks with 16-bit types: every block's mean passes through fp16 (scaled for bf16), which is off by 2^-11 of its components
+and 2^-25 for fp16, 2^-38 of its largest for bf16, both at most 2^-25 max |v|; the means' weights add up to 1, so that is
+2^-11 A + 2^-25 max |v| more (max |v| <= sum |v|)."""
 import ctypes as C
 import math
 
@@ -363,7 +366,7 @@ def _attend_ref(torch, q, k, v, scale, q_off, k_off, skip, sel=None, block=0, n_
     return out, lse, tol, a_abs, v_abs, ltol
 
 
-def _check_attend(torch, dtype, got, lse, ref):
+def _check_attend(torch, dtype, got, lse, ref, blocks=False):
     out, rl, tol, a_abs, v_abs, ltol = ref
     u = _u(dtype)
     t = tol + (0 if dtype == "fp32" else u * a_abs * 1.01) + u * out.abs() * 1.01
@@ -371,6 +374,8 @@ def _check_attend(torch, dtype, got, lse, ref):
         t = t + 2.0 ** -25 * (v_abs + 1)
     if dtype == "fp32":
         t = t + 2.0 ** -126
+    elif blocks:
+        t = t + 2.0 ** -11 * a_abs + 2.0 ** -25 * (v_abs.amax(-1, keepdim=True) + 1)
     err = (got.cpu().double() - out).abs()
     ok = (err <= t) | (out.isnan() & got.cpu().isnan())
     assert ok.all(), (float((err / t.clamp(min=1e-300))[~ok].max()), int((~ok).sum()))
@@ -571,7 +576,31 @@ def test_attention_selected_blocks(gpu, dtype, shape):
     out, lse = _run_attention(gpu, dtype, q.cuda(), k.cuda(), v.cuda(), scale, q_off, k_off, None if skip is None else skip.cuda(), sel.cuda(), block)
     a, b = q_off[0], q_off[-1]
     assert (out[:a] == 3).all() and (out[b:] == 3).all() and (lse[:a] == 3).all() and (lse[b:] == 3).all()
-    _check_attend(torch, dtype, out[a:b], lse[a:b], [x[a:b] for x in ref])
+    _check_attend(torch, dtype, out[a:b], lse[a:b], [x[a:b] for x in ref], blocks=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ("bf16", "fp32"))
+def test_selected_blocks_with_values_of_every_size(gpu, dtype):
+    """Values from 1e-30 to 1e30 (a size per block and per component), infinities and NaN among the keys attended to: what is
+    not finite stays in its component, the others keep their precision."""
+    pkg, ctx, torch = gpu
+    t = _t(torch, dtype)
+    g = torch.Generator().manual_seed(12)
+    q, k, v = _rand(torch, 74, 200, 2, 64).to(t), _rand(torch, 75, 1280, 2, 64).to(t), _rand(torch, 76, 1280, 2, 64)
+    v = v * 10.0 ** torch.randint(-30, 31, (20, 1, 1), generator=g).repeat_interleave(64, 0) * 10.0 ** (-torch.arange(64) / 16.0)
+    v[70, 0, 3], v[200, 1, 5], v[300, 0, 7] = math.inf, -math.inf, math.nan
+    v = v.to(t)
+    sel = torch.stack([torch.randperm(20, generator=g)[:5] for _ in range(400)]).view(200, 2, 5).to(torch.int32)
+    ref = _attend_ref(torch, q, k, v, 0.125, [0, 200], [0, 1280], None, sel, 64, 5)
+    out, lse = _run_attention(gpu, dtype, q.cuda(), k.cuda(), v.cuda(), 0.125, [0, 200], [0, 1280], sel=sel.cuda(), block=64)
+    got, want = out.cpu().double(), ref[0]
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf()) and want.isinf().any() and want.isnan().any()
+    fin = want.isfinite()
+    assert torch.equal(got[~fin & ~want.isnan()], want[~fin & ~want.isnan()])
+    part = 0 if dtype == "fp32" else 2.0 ** -11 * ref[3] + 2.0 ** -38 * ref[3].nan_to_num(0, 0, 0).amax(-1, keepdim=True)
+    tol = ref[2] + (0 if dtype == "fp32" else _u(dtype) * ref[3] * 1.01) + _u(dtype) * want.abs() * 1.01 + part + 2.0 ** -126
+    assert ((got - want).abs()[fin] <= tol[fin]).all()
 
 
 @pytest.mark.gpu
@@ -659,7 +688,7 @@ class _Chain:
         assert np.array_equal(sel.numpy(), _select_ref(self.rq.cpu().float().numpy(), self.mean.cpu().numpy(), self.count.cpu().numpy(), self.q_off,
                                                        self.k_off, 64, 4, 8))
         rq, rk, v, out = (x.cpu() for x in (self.rq, self.rk, self.v, self.out))
-        _check_attend(torch, "bf16", self.out, None, _attend_ref(torch, rq, rk, v, 0.125, self.q_off, self.k_off, None, sel, 64, 8))
+        _check_attend(torch, "bf16", self.out, None, _attend_ref(torch, rq, rk, v, 0.125, self.q_off, self.k_off, None, sel, 64, 8), blocks=True)
         _check_attend(torch, "bf16", self.own, None, _attend_ref(torch, rq, rq, out, 0.125, self.q_off, self.q_off, None))
 
     def results(self):

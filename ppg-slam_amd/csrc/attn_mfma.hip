@@ -394,23 +394,29 @@ __global__ __launch_bounds__(256, 2) void attention_split_kernel(AttentionLaunch
     }
 }
 
-// Joins the parts of every (row, head): D / 4 threads take four components each, PG such teams the parts of one (row, head) in
-// turn, four loads in flight; the teams' sums meet in LDS in their order.  SEL: part i belongs to place i of the query's list
-// and exists only if that names a block.
+// Joins the parts of every (row, head): a team's threads take 16 bytes of components each, PG such teams the parts of one
+// (row, head) in turn, four loads in flight; the teams' sums meet in LDS in their order.  SEL: part i belongs to place i of the
+// query's list and exists only if that names a block.
+template <class T, int D, bool SEL> struct JoinShape {
+    using P = std::conditional_t<SEL, ListPart<T, D>, Part<D>>;
+    static constexpr bool HALF = !__is_same(P, Part<D>);   // o is a mean there, a sum here
+    static constexpr int C = HALF ? 8 : 4, TEAM = D / C, TEAMS = 256 / TEAM;
+};
 template <class T, int D, bool SEL, int PG>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, AttnSets sets, int parts) {
-    constexpr int TEAM = D / 4, TEAMS = 256 / TEAM;
+    using J = JoinShape<T, D, SEL>;
+    using P = typename J::P;
+    constexpr int C = J::C, TEAM = J::TEAM, TEAMS = J::TEAMS;
+    typedef float vec __attribute__((ext_vector_type(C)));
     struct Sum {
-        f32x4 o;
+        vec o;
         float m, l;
     };
     __shared__ Sum met[PG > 1 ? 256 : 1];
-    const int team = threadIdx.x / TEAM, sub = team % PG, d = threadIdx.x % TEAM * 4;
+    const int team = threadIdx.x / TEAM, sub = team % PG, d = threadIdx.x % TEAM * C;
     const long long n = ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads, at = (long long)blockIdx.x * (TEAMS / PG) + team / PG;
     const long long rh = min(at, n - 1);   // (a team behind the last does its work again and keeps it to itself)
     const float c = a.scale * kLog2e;
-    using P = std::conditional_t<SEL, ListPart<T, D>, Part<D>>;
-    constexpr bool HALF = !__is_same(P, Part<D>);   // o is a mean there, a sum here
     const P* w = (const P*)a.work + rh * parts;
     const long long q = sets.q_off[0] + rh / a.q.heads;
     const int head = (int)(rh % a.q.heads);
@@ -422,7 +428,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, 
         sel = a.sel + (q * a.k.heads + head / (a.q.heads / a.k.heads)) * a.n_sel;
     }
     float m = -INFINITY, l = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    vec o = {};
     for (int p0 = sub; p0 < parts; p0 += 4 * PG) {
         Sum x[4];
         bool on[4];
@@ -431,13 +437,11 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, 
             const int p = min(p0 + i * PG, parts - 1);
             x[i].m = w[p].m;
             x[i].l = w[p].l;
-            if constexpr (HALF) {
-                typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-                const f16x4 v = *(const f16x4*)&w[p].o[d];
-                const float f = w[p].scale * x[i].l;
-                x[i].o = f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]} * f;
+            if constexpr (J::HALF) {
+                typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+                x[i].o = __builtin_convertvector(*(const half8*)&w[p].o[d], vec) * (w[p].scale * x[i].l);
             } else {
-                x[i].o = *(const f32x4*)&w[p].o[d];
+                x[i].o = *(const vec*)&w[p].o[d];
             }
             on[i] = p0 + i * PG < parts;
             if constexpr (SEL) on[i] = on[i] && (unsigned)sel[p] < (unsigned)blocks;
@@ -472,12 +476,10 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, 
     }
     if (at >= n) return;
     const float inv = inverse_sum(l);
-    T out[4];
+    struct alignas(C * sizeof(T)) Out { T v[C]; } out;
 #pragma unroll
-    for (int e = 0; e < 4; e++) out[e] = (T)(inv == 0.f ? 0.f : o[e] * inv);
-    T* to = (T*)a.out.p + q * a.out.row + head * a.out.head + d;
-    if constexpr (IsF32<T>::v) *(f32x4*)to = __builtin_bit_cast(f32x4, out);
-    else *(s16x4*)to = __builtin_bit_cast(s16x4, out);
+    for (int e = 0; e < C; e++) out.v[e] = (T)(inv == 0.f ? 0.f : o[e] * inv);
+    *(Out*)((T*)a.out.p + q * a.out.row + head * a.out.head + d) = out;
     if (a.lse && d == 0) a.lse[q * a.q.heads + head] = log_sum(m, l, c);
 }
 
@@ -487,19 +489,24 @@ struct BinWork {
     int* list;     // entries by block, [regions][queries of the set * n_sel]
     int4* tile;    // (block, first entry in the region's list, rows of the block = entries * group, first row of the tile); block -1: unused
 };
+// A region's blocks are counted by one work-group, or in kBinShares equal shares by as many where the entries are more than the
+// blocks.
+constexpr int kBinShares = 4;
+__host__ __device__ inline int bin_shares(long long nq, int n_sel, int blocks) { return nq * n_sel >= 2048 && nq * n_sel >= blocks ? kBinShares : 1; }
 // tiles that a region may need: its rows in 32s, and one more for every block's last
 __host__ __device__ inline int region_tiles(long long nq, int n_sel, int group, int blocks) {
     const long long e = nq * n_sel;
     return (int)(e * group / 32 + (e < blocks ? e : blocks));
 }
 
-// One work-group per region: counts per block, their running sum, and the entries put in their places.  Which entry of a block
-// comes first is left to the atomics: entries of a block never meet in a sum.
+// One work-group per share of a region's blocks: counts per block, their running sum, and the entries put in their places.  Which
+// entry of a block comes first is left to the atomics: entries of a block never meet in a sum.  A share's entries start
+// behind those of the blocks before it (every share counts them), its tiles where those blocks' could end at the latest.
 constexpr int kBins = 8192;    // blocks counted at a time (32 KB of LDS)
 constexpr int kBinHold = 16;   // entries per thread that stay in registers between the two passes
 __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets sets, BinWork w) {
     __shared__ int cnt[kBins];
-    __shared__ int sum_e[16], sum_t[16];
+    __shared__ int sum_e[16], sum_t[16], sum_b[16];
     const int kvh = a.k.heads, group = a.q.heads / kvh, s = blockIdx.x / kvh, g = blockIdx.x % kvh;
     const int q0 = sets.q_off[s], nq = sets.q_off[s + 1] - q0, blocks = sets.blk[s + 1] - sets.blk[s], n = nq * a.n_sel;
     const int* sel = a.sel + ((long long)q0 * kvh + g) * a.n_sel;
@@ -507,7 +514,10 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
     int* list = w.list + ((long long)(q0 - sets.q_off[0]) * kvh + (long long)g * nq) * a.n_sel;
     int4* tile = w.tile + sets.tile[s] + (long long)g * region_tiles(nq, a.n_sel, group, blocks);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int e0 = 0, t0 = 0;   // entries and tiles of the bins before this round's
+    const int shares = bin_shares(nq, a.n_sel, blocks), share = blockIdx.y;
+    if (share >= shares) return;
+    const int lo = (int)((long long)blocks * share / shares), hi = (int)((long long)blocks * (share + 1) / shares);
+    int e0 = 0, t0 = 0;   // where the entries and tiles of this round's bins go
     int held[kBinHold], rank[kBinHold];
     const bool once = n <= kBinHold * 1024;
     const int dq = 1024 / a.n_sel, dr = 1024 % a.n_sel;   // 1024 entries on, in queries and places
@@ -524,18 +534,29 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
             }
         }
     };
-    for (int b0 = 0; b0 < blocks; b0 += kBins) {
-        const int nb = min(kBins, blocks - b0), per = (nb + 1023) / 1024;
+    for (int b0 = lo; b0 < hi; b0 += kBins) {
+        const int nb = min(kBins, hi - b0), per = (nb + 1023) / 1024;
         for (int i = tid; i < nb; i += 1024) cnt[i] = 0;
-        if (b0 == 0) load(0);
+        int below = 0;
+        if (b0 == lo) load(0);
         __syncthreads();
         for (int from = 0; from < n; from += kBinHold * 1024) {
             if (!once) load(from);
 #pragma unroll
             for (int i = 0; i < kBinHold; i++)
+            {
                 if (held[i] >= b0 && held[i] - b0 < nb) rank[i] = atomicAdd(&cnt[held[i] - b0], 1);
+                below += held[i] >= 0 && held[i] < lo;
+            }
         }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) below += __shfl_xor(below, d);
+        if (lane == 0) sum_b[wave] = below;
         __syncthreads();
+        if (b0 == lo) {
+            for (int i = 0; i < 16; i++) e0 += sum_b[i];
+            if (lo) t0 = (int)((long long)e0 * group / 32) + lo;
+        }
         int es = 0, ts = 0;
         for (int i = tid * per; i < min(nb, (tid + 1) * per); i++) {
             es += cnt[i];
@@ -579,15 +600,17 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
         }
         __syncthreads();
     }
-    const int cap = region_tiles(nq, a.n_sel, group, blocks);
-    for (int i = t0 + tid; i < cap; i += 1024) tile[i] = make_int4(-1, 0, 0, 0);
+    // up to where the next share's tiles start
+    const int end = share + 1 < shares ? (int)((long long)e0 * group / 32) + hi : region_tiles(nq, a.n_sel, group, blocks);
+    for (int i = t0 + tid; i < end; i += 1024) tile[i] = make_int4(-1, 0, 0, 0);
 }
 
-// A wave per tile: one block's keys against 32 rows out of the queries that name it.
-template <class T, int D, int BN>
+// A wave per tile: one block's keys against 32 rows out of the queries that name it.  32 keys at a time: fewer registers, so that
+// three waves of a SIMD have loads in flight (64 at a time: 15 us more for 8 streams).
+template <class T, int D>
 __global__ __launch_bounds__(64, 2) void attention_blocks_kernel(AttentionLaunch a, AttnSets sets, BinWork w) {
     using S = Shape<T, D>;
-    constexpr int SUB = BN / 32, IMG = BN * D * (int)sizeof(T);
+    constexpr int BN = 32, SUB = BN / 32, IMG = BN * D * (int)sizeof(T);
     __shared__ alignas(16) char lds_v[IMG];
     const int lane = threadIdx.x, h = lane >> 5;
     // (in launch order: hardly two tiles read the same block, and a region's unused tiles would leave some XCDs without work)
@@ -725,21 +748,16 @@ BlocksPlan blocks_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSe
     return p;
 }
 
-template <class T, int D> hipError_t join(const AttentionLaunch& a, AttnSets& sets, int parts, bool by_list, hipStream_t s) {
-    constexpr int TEAMS = 256 / (D / 4), MANY = std::min(16, TEAMS);
+template <class T, int D, bool SEL> hipError_t join(const AttentionLaunch& a, AttnSets& sets, int parts, hipStream_t s) {
+    using J = JoinShape<T, D, SEL>;
+    constexpr int TEAMS = J::TEAMS, MANY = std::min(16, TEAMS);
     const long long n = ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads;
     // one team per (row, head) where those fill the chip, else several
-    const int pg = n * (D / 4) >= 65536 * 4 || parts < 8 ? 1 : parts < 32 ? 4 : MANY;
+    const int pg = n * J::TEAM >= 65536 * 2 || parts < 8 ? 1 : parts < 32 ? 4 : MANY;
     const unsigned grid = (unsigned)((n + TEAMS / pg - 1) / (TEAMS / pg));
-#define JOIN(SEL)                                                                                    \
-    do {                                                                                             \
-        if (pg == 1) attention_join_kernel<T, D, SEL, 1><<<grid, 256, 0, s>>>(a, sets, parts);       \
-        else if (pg == 4) attention_join_kernel<T, D, SEL, 4><<<grid, 256, 0, s>>>(a, sets, parts);  \
-        else attention_join_kernel<T, D, SEL, MANY><<<grid, 256, 0, s>>>(a, sets, parts);            \
-    } while (0)
-    if (by_list) JOIN(true);
-    else JOIN(false);
-#undef JOIN
+    if (pg == 1) attention_join_kernel<T, D, SEL, 1><<<grid, 256, 0, s>>>(a, sets, parts);
+    else if (pg == 4) attention_join_kernel<T, D, SEL, 4><<<grid, 256, 0, s>>>(a, sets, parts);
+    else attention_join_kernel<T, D, SEL, MANY><<<grid, 256, 0, s>>>(a, sets, parts);
     return hipGetLastError();
 }
 template <class T, int D> hipError_t run(const AttentionLaunch& a, AttnSets& sets, int dtype, hipStream_t s) {
@@ -751,18 +769,18 @@ template <class T, int D> hipError_t run(const AttentionLaunch& a, AttnSets& set
         if (!p.binned) {
             attention_split_kernel<T, D, OWN_BN, true><<<xcd_grid(sets.tile[sets.n] * p.parts), 256, 0, s>>>(a, sets, p.parts);
             e = hipGetLastError();
-            return e != hipSuccess || p.parts == 1 ? e : join<T, D>(a, sets, p.parts, false, s);
+            return e != hipSuccess || p.parts == 1 ? e : join<T, D, false>(a, sets, p.parts, s);
         }
         BinWork w;
         w.list = (int*)((char*)a.work + p.part_bytes);
         w.tile = (int4*)((char*)w.list + p.list_bytes);
         if (sets.tile[sets.n]) {
-            bin_kernel<<<sets.n * a.k.heads, 1024, 0, s>>>(a, sets, w);
+            bin_kernel<<<dim3(sets.n * a.k.heads, kBinShares), 1024, 0, s>>>(a, sets, w);
             if ((e = hipGetLastError()) != hipSuccess) return e;
-            attention_blocks_kernel<T, D, OWN_BN><<<(unsigned)sets.tile[sets.n], 64, 0, s>>>(a, sets, w);
+            attention_blocks_kernel<T, D><<<(unsigned)sets.tile[sets.n], 64, 0, s>>>(a, sets, w);
             if ((e = hipGetLastError()) != hipSuccess) return e;
         }
-        return join<T, D>(a, sets, p.parts, true, s);
+        return join<T, D, true>(a, sets, p.parts, s);
     }
     const DensePlan p = dense_plan(dtype, D, a, sets);
     if (!sets.tile[sets.n]) return hipSuccess;
@@ -773,7 +791,7 @@ template <class T, int D> hipError_t run(const AttentionLaunch& a, AttnSets& set
     }
     attention_split_kernel<T, D, OWN_BN, false><<<xcd_grid(sets.tile[sets.n] * p.parts), 256, 0, s>>>(a, sets, p.parts);
     e = hipGetLastError();
-    return e != hipSuccess || p.parts == 1 ? e : join<T, D>(a, sets, p.parts, false, s);
+    return e != hipSuccess || p.parts == 1 ? e : join<T, D, false>(a, sets, p.parts, s);
 }
 template <class T> hipError_t run_dim(const AttentionLaunch& a, AttnSets& sets, int dtype, int head_dim, hipStream_t s) {
     return head_dim == 32 ? run<T, 32>(a, sets, dtype, s) : head_dim == 64 ? run<T, 64>(a, sets, dtype, s) : run<T, 128>(a, sets, dtype, s);

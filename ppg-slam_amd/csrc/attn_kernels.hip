@@ -302,42 +302,44 @@ __global__ __launch_bounds__(1024, 4) void block_select_kernel(BlockSelectLaunch
     auto query = [&](int row, int h) { return (const T*)a.q.p + (long long)(q0 + min(row, nq - 1)) * a.q.row + ((long long)g * group + h) * a.q.head; };
     auto q_chunk = [&](int half, int r, int ch) { return lds.q[half] + r * (D * 2) + ((ch ^ (r & (D >= 64 ? 7 : 3))) << 4); };
 
+    f32x4 mx[D / 32][2];
+    bool alive = false;
+    auto load = [&](int b0, int t) {
+        const int n = min(CHUNK, nb - b0), b = t * 16 + (lane & 15), bb = b0 + min(b, n - 1);
+        const float* m = mean + bb * stride + (lane >> 4) * 8;
+#pragma unroll
+        for (int k = 0; k < D / 32; k++) {
+            mx[k][0] = *(const f32x4*)(m + k * 32);
+            mx[k][1] = *(const f32x4*)(m + k * 32 + 4);
+        }
+        alive = b < n && count[bb] > 0;
+    };
+    if (wave * 16 < nb) load(0, wave);   // (in flight while the queries are prepared)
+
     // a wave per RPW rows: the group's sum, its halves to LDS, its length
     Scored best[RPW];
     float eq[RPW];   // 2^-13 |q|, NaN: the plain way
 #pragma unroll
     for (int i = 0; i < RPW; i++) {
         const int r = wave * RPW + i;
-        double sq = 0;
+        float sq = 0.f;
         for (int d = lane; d < D; d += 64) {
             double x = 0;
             for (int h = 0; h < group; h++) x += (double)to_float(query(row0 + r, h)[d]);
             const __bf16 hi = (__bf16)(float)x, lo = (__bf16)(float)(x - (double)(float)hi);
             *(__bf16*)(q_chunk(0, r, d >> 3) + (d & 7) * 2) = hi;
             *(__bf16*)(q_chunk(1, r, d >> 3) + (d & 7) * 2) = lo;
-            sq += x * x;
+            sq = fmaf((float)x, (float)x, sq);
         }
-        sq = wave_sum_d(sq);
+        sq = wave_sum(sq);
         // (one so short that its components leave bf16's range has no such bound, unless it is zero)
-        eq[i] = sq < 1e36 && !(sq < 1e-24 && sq > 0) ? (float)sqrt(sq) * 1.22071e-4f : NAN;
+        eq[i] = sq < 1e36f && !(sq < 1e-24f && sq > 0.f) ? sqrtf(sq) * 1.2208e-4f : NAN;
         best[i] = Scored{0, 0x7fffffff};
     }
 
     for (int b0 = 0; b0 < nb; b0 += CHUNK) {
         const int n = min(CHUNK, nb - b0);
-        f32x4 mx[D / 32][2];
-        bool alive = false;
-        auto load = [&](int t) {
-            const int b = t * 16 + (lane & 15), bb = b0 + min(b, n - 1);
-            const float* m = mean + bb * stride + (lane >> 4) * 8;
-#pragma unroll
-            for (int k = 0; k < D / 32; k++) {
-                mx[k][0] = *(const f32x4*)(m + k * 32);
-                mx[k][1] = *(const f32x4*)(m + k * 32 + 4);
-            }
-            alive = b < n && count[bb] > 0;
-        };
-        if (wave * 16 < n) load(wave);
+        if (b0 && wave * 16 < n) load(b0, wave);
         __syncthreads();   // the queries are in LDS; the last stretch has been read
         for (int t = wave; t * 16 < n; t += kSelWaves) {
             f32x4 acc[RPW] = {};
@@ -353,7 +355,7 @@ __global__ __launch_bounds__(1024, 4) void block_select_kernel(BlockSelectLaunch
                     sm = fmaf(x, x, sm);
                 }
             const bool on = alive;
-            if ((t + kSelWaves) * 16 < n) load(t + kSelWaves);
+            if ((t + kSelWaves) * 16 < n) load(b0, t + kSelWaves);
 #pragma unroll
             for (int rt = 0; rt < RPW; rt++) {
 #pragma unroll

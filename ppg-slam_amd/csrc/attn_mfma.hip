@@ -51,28 +51,37 @@ template <class T, int D> __device__ __forceinline__ void store_out(const ppg_ro
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }
 __device__ __forceinline__ float log_sum(float m, float l, float c) { return l == 0.f ? -INFINITY : fmaf(m, c, __log2f(l)) * kLn2; }
 
+// Sums of one (row, part): D components, then m and l.  A part without keys has m = -inf, l = 0.
+template <int D> struct Part {
+    float o[D];
+    float m, l;
+    float pad[2];
+};
+
+// parts > 1: a work-group takes its share of the keys and leaves its sums.
 // Which keys are masked is read once, a bit each, kWindow words ahead, so that the loads of a tile do not wait for it.
 // UNIT (16-bit types): the matrix unit adds up the weights (a product with ones); the vector unit, which has the exponentials, is
 // the busier one (4 % of the time at 64 and at 128 components).  Those are the rounded weights, the same that meet the
 // values, but their sum is not good enough for a log: with lse the vector unit adds up the unrounded ones.
 constexpr int kWindow = 64;   // 64-key words of the mask in LDS at a time
-template <class T, int D, int BN, int QT, bool UNIT>
-__global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) void attention_wide_kernel(AttentionLaunch a, AttnSets sets) {
+template <class T, int D, int BN, bool UNIT>
+__global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) void attention_wide_kernel(AttentionLaunch a, AttnSets sets, int parts) {
     using S = Shape<T, D>;
-    constexpr int SUB = BN / 32, CH = BN * S::CPR / 256, ROWB = D * (int)sizeof(T), TILE = BN * ROWB, WG = 128 * QT, STEP = 256 / S::CPR;
+    constexpr int SUB = BN / 32, CH = BN * S::CPR / 256, ROWB = D * (int)sizeof(T), TILE = BN * ROWB, STEP = 256 / S::CPR;
     constexpr unsigned long long FULL = BN == 64 ? ~0ull : 0xffffffffull;
     static_assert(BN * S::CPR % 256 == 0, "tile loads are whole rounds of the work-group");
     __shared__ alignas(16) char lds_k[2][TILE], lds_v[2][TILE];
     __shared__ unsigned long long lds_dead[kWindow];
-    const int unit = xcd_unit(blockIdx.x, sets.tile[sets.n]);
-    if (unit >= sets.tile[sets.n]) return;
+    const int units = sets.tile[sets.n] * parts, whole = xcd_unit(blockIdx.x, units);
+    if (whole >= units) return;
+    const int unit = parts == 1 ? whole : whole / parts, part = parts == 1 ? 0 : whole % parts;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const int s = find_set_wave(sets.tile, sets.n, unit, lane);
     const int q0 = sets.q_off[s], k0 = sets.k_off[s], nk = sets.k_off[s + 1] - k0, kvh = a.k.heads, group = a.q.heads / kvh;
-    const int rows = (sets.q_off[s + 1] - q0) * group, tiles = (rows + WG - 1) / WG;
-    const int g = (unit - sets.tile[s]) / tiles, row = ((unit - sets.tile[s]) % tiles) * WG + wave * (32 * QT) + (lane & 31);
+    const int rows = (sets.q_off[s + 1] - q0) * group, tiles = (rows + 127) / 128;
+    const int g = (unit - sets.tile[s]) / tiles, row = ((unit - sets.tile[s]) % tiles) * 128 + wave * 32 + (lane & 31);
     const float c = a.scale * kLog2e, slack = 8.f / c;
-    const int nt = (nk + BN - 1) / BN;
+    const int all = (nk + BN - 1) / BN, from = (int)((long long)all * part / parts), to = (int)((long long)all * (part + 1) / parts);
 
     // tile loads: thread -> (row, chunk) and STEP rows on
     const int r0 = tid / S::CPR, ch0 = tid % S::CPR;
@@ -111,7 +120,7 @@ __global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) 
     auto window = [&](int t) {   // of the kWindow words from tile t's on
         for (int w = wave; w < kWindow; w += 4) {
             const long long j = (long long)t * BN + w * 64 + lane;
-            if (j - lane >= nk) break;
+            if (j - lane >= min((long long)nk, (long long)to * BN)) break;
             const unsigned long long m = __ballot(j >= nk || a.skip[k0 + (int)min(j, (long long)nk - 1)] != 0);
             if (lane == 0) lds_dead[w] = m;
         }
@@ -119,7 +128,8 @@ __global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) 
     auto dead_of = [&](int t) -> unsigned long long {
         unsigned long long m;
         if (a.skip) {
-            const unsigned long long x = lds_dead[(t * (BN / 32) / 2) % kWindow] >> (BN == 32 ? (t & 1) * 32 : 0);
+            const int i = t - from;
+            const unsigned long long x = lds_dead[(i * (BN / 32) / 2) % kWindow] >> (BN == 32 ? (i & 1) * 32 : 0);
             m = ((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)x);
         } else {
             const long long left = nk - (long long)t * BN;
@@ -130,81 +140,72 @@ __global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) 
     constexpr int PER_WINDOW = kWindow * 64 / BN;   // tiles
 
     unsigned long long dead = 0;   // of the tile being multiplied
-    if (nt) {
+    if (from < to) {
         if (a.skip) {
-            window(0);
+            window(from);
             __syncthreads();
         }
-        dead = dead_of(0);
-        fetch(0);
+        dead = dead_of(from);
+        fetch(from);
     }
-    u32x4 qf[QT][S::NF];
-#pragma unroll
-    for (int q = 0; q < QT; q++) load_query<T, D>(qf[q], a.q, row_place(row + 32 * q, rows, group, g, q0), h);
-    Running<T, D, UNIT> run[QT];
-#pragma unroll
-    for (int q = 0; q < QT; q++) run[q].clear();
-    if (nt) store(0, dead);
-    auto multiply = [&](int buf) {
-        f32x16 sc[SUB][QT];
-        __builtin_amdgcn_s_setprio(1);   // the matrix unit's share first: 4 % at 128 components, nothing at 64
-#pragma unroll
-        for (int u = 0; u < SUB; u++) {
-            const int r = u * 32 + (lane & 31);
-#pragma unroll
-            for (int q = 0; q < QT; q++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) sc[u][q][e] = 0.f;
-#pragma unroll
-            for (int i = 0; i < S::NF; i++) {
-                const u32x4 kf = *(const u32x4*)(lds_k[buf] + r * ROWB + ((S::chunk(i, h) ^ S::swz_k(r)) << 4));
-#pragma unroll
-                for (int q = 0; q < QT; q++) sc[u][q] = mfma_chunk<T>(kf, qf[q][i], sc[u][q]);
-            }
-            if (dead)
-#pragma unroll
-                for (int q = 0; q < QT; q++) mask_scores(sc[u][q], (unsigned)(dead >> (32 * u)), h);
-        }
-        __builtin_amdgcn_s_setprio(0);
-#pragma unroll
-        for (int q = 0; q < QT; q++) {
-            f32x16 one[SUB];
-#pragma unroll
-            for (int u = 0; u < SUB; u++) one[u] = sc[u][q];
-            run[q].template weights<SUB>(one, c, slack);
-#pragma unroll
-            for (int u = 0; u < SUB; u++) sc[u][q] = one[u];
-        }
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int u = 0; u < SUB; u++) add_values<T, D, QT, UNIT>(run, sc[u], lds_v[buf], u * 32, lane);
-        __builtin_amdgcn_s_setprio(0);
-    };
+    const RowPlace place = row_place(row, rows, group, g, q0);
+    u32x4 qf[S::NF];
+    load_query<T, D>(qf, a.q, place, h);
+    Running<T, D, UNIT> run;
+    run.clear();
+    if (from < to) store(from, dead);
     __syncthreads();
-    for (int t = 0; t < nt; t++) {
+    for (int t = from; t < to; t++) {
         const int buf = t & 1;
         unsigned long long next = 0;
-        if (t + 1 < nt) {
-            if (a.skip && (t + 1) % PER_WINDOW == 0) {   // (all words so far have been read, before the last barrier)
+        if (t + 1 < to) {
+            if (a.skip && (t + 1 - from) % PER_WINDOW == 0) {   // (all words so far have been read, before the last barrier)
                 window(t + 1);
                 __syncthreads();
             }
             next = dead_of(t + 1);
             fetch(t + 1);
         }
-        multiply(buf);
-        if (t + 1 < nt) store(t + 1, next);   // last read one tile ago, before the barrier below
+        f32x16 sc[SUB];
+        __builtin_amdgcn_s_setprio(1);   // the matrix unit's share first: 4 % at 128 components, nothing at 64
+#pragma unroll
+        for (int u = 0; u < SUB; u++) {
+            const int r = u * 32 + (lane & 31);
+#pragma unroll
+            for (int e = 0; e < 16; e++) sc[u][e] = 0.f;
+#pragma unroll
+            for (int i = 0; i < S::NF; i++) {
+                const u32x4 kf = *(const u32x4*)(lds_k[buf] + r * ROWB + ((S::chunk(i, h) ^ S::swz_k(r)) << 4));
+                sc[u] = mfma_chunk<T>(kf, qf[i], sc[u]);
+            }
+            if (dead) mask_scores(sc[u], (unsigned)(dead >> (32 * u)), h);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        run.template weights<SUB>(sc, c, slack);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int u = 0; u < SUB; u++) add_values(run, sc[u], lds_v[buf], u * 32, lane);
+        __builtin_amdgcn_s_setprio(0);
+        if (t + 1 < to) store(t + 1, next);   // last read one tile ago, before the barrier below
         dead = next;
         __syncthreads();
     }
+    const float l = run.sum();
+    if (row >= rows) return;
+    if (parts > 1) {
+        Part<D>& w = ((Part<D>*)a.work)[((place.q - sets.q_off[0]) * a.q.heads + place.head) * parts + part];
 #pragma unroll
-    for (int q = 0; q < QT; q++) {
-        if (row + 32 * q >= rows) return;
-        const RowPlace place = row_place(row + 32 * q, rows, group, g, q0);
-        const float l = run[q].sum();
-        store_out<T, D>(a.out, place, run[q].o, inverse_sum(l), h);
-        if (a.lse && h == 0) a.lse[place.q * a.q.heads + place.head] = log_sum(run[q].m, l, c);
+        for (int u = 0; u < D / 32; u++)
+#pragma unroll
+            for (int b = 0; b < 4; b++) *(f32x4*)&w.o[u * 32 + 8 * b + 4 * h] = f32x4{run.o[u][4 * b], run.o[u][4 * b + 1], run.o[u][4 * b + 2], run.o[u][4 * b + 3]};
+        if (h == 0) {
+            w.m = run.m;
+            w.l = l;
+        }
+        return;
     }
+    store_out<T, D>(a.out, place, run.o, inverse_sum(l), h);
+    if (a.lse && h == 0) a.lse[place.q * a.q.heads + place.head] = log_sum(run.m, l, c);
 }
 
 // A wave's own stretch of keys: operands straight from memory, values through an LDS image of its own.
@@ -290,13 +291,6 @@ template <class T, int D> __device__ __forceinline__ void meet(Meeting<T, D>& x,
     }
 }
 
-// Sums of one (row, part): D components, then m and l.  A part without keys has m = -inf, l = 0.
-template <int D> struct Part {
-    float o[D];
-    float m, l;
-    float pad[2];
-};
-
 // The same for a selected block of a query, with 16-bit types: the mean of the values (o / l) in fp16, times a power of two that
 // brings the largest into [2^13, 2^14) where the values' own type reaches further than fp16.  That is off by 2^-11 of each
 // component (and 2^-38 of the largest), where the result is rounded to 2^-11 (fp16) or 2^-8 (bf16) anyway; it halves what is
@@ -310,7 +304,7 @@ template <class T, int D> using ListPart = std::conditional_t<IsF32<T>::v, Part<
 
 // SEL: a unit's rows are the group of one query, its keys the blocks of that query's list.
 template <class T, int D, int BN, bool SEL>
-__global__ __launch_bounds__(256, 2) void attention_split_kernel(AttentionLaunch a, AttnSets sets, int parts) {
+__global__ __launch_bounds__(256, IsF32<T>::v && D == 128 ? 1 : 2) void attention_split_kernel(AttentionLaunch a, AttnSets sets, int parts) {
     using S = Shape<T, D>;
     constexpr int SUB = BN / 32, IMG = BN * D * (int)sizeof(T);
     __shared__ alignas(16) union {
@@ -331,8 +325,8 @@ __global__ __launch_bounds__(256, 2) void attention_split_kernel(AttentionLaunch
     u32x4 qf[S::NF];
     load_query<T, D>(qf, a.q, row_place(row0 + (lane & 31), rows, group, g, q0), h);
     const float c = a.scale * kLog2e, slack = 8.f / c;
-    Running<T, D> run[1];
-    run[0].clear();
+    Running<T, D> run;
+    run.clear();
     const T* kp = (const T*)a.k.p + g * a.k.head + (long long)k0 * a.k.row;
     const T* vp = (const T*)a.v.p + g * a.v.head + (long long)k0 * a.v.row;
     const uint8_t* skip = a.skip ? a.skip + k0 : nullptr;
@@ -359,14 +353,14 @@ __global__ __launch_bounds__(256, 2) void attention_split_kernel(AttentionLaunch
         keys.scores(sc, qf, lane);
         keys.values_to_lds(lds.v[wave], lane);
         if (t + 4 < to) load(t + 4);
-        run[0].template weights<SUB>(sc, c, slack);
+        run.template weights<SUB>(sc, c, slack);
         __builtin_amdgcn_wave_barrier();   // the image is this wave's own and LDS serves a wave in order
 #pragma unroll
-        for (int u = 0; u < SUB; u++) add_values<T, D, 1, false>(run, *(f32x16(*)[1])&sc[u], lds.v[wave], u * 32, lane);
+        for (int u = 0; u < SUB; u++) add_values(run, sc[u], lds.v[wave], u * 32, lane);
         __builtin_amdgcn_wave_barrier();
     }
     __syncthreads();
-    meet(lds.sums, run[0], c, wave, 4, lane);
+    meet(lds.sums, run, c, wave, 4, lane);
     // 32 rows x D components out, 4 per thread and round
     for (int i = threadIdx.x; i < 32 * (D / 4); i += 256) {
         const int r = i / (D / 4), d = (i % (D / 4)) * 4;
@@ -608,7 +602,7 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
 // A wave per tile: one block's keys against 32 rows out of the queries that name it.  32 keys at a time: fewer registers, so that
 // three waves of a SIMD have loads in flight (64 at a time: 15 us more for 8 streams).
 template <class T, int D>
-__global__ __launch_bounds__(64, 2) void attention_blocks_kernel(AttentionLaunch a, AttnSets sets, BinWork w) {
+__global__ __launch_bounds__(64, IsF32<T>::v && D == 128 ? 1 : 2) void attention_blocks_kernel(AttentionLaunch a, AttnSets sets, BinWork w) {
     using S = Shape<T, D>;
     constexpr int BN = 32, SUB = BN / 32, IMG = BN * D * (int)sizeof(T);
     __shared__ alignas(16) char lds_v[IMG];
@@ -634,28 +628,28 @@ __global__ __launch_bounds__(64, 2) void attention_blocks_kernel(AttentionLaunch
     u32x4 qf[S::NF];
     load_query<T, D>(qf, a.q, RowPlace{q, head}, h);
     const float c = a.scale * kLog2e, slack = 8.f / c;
-    Running<T, D> run[1];
-    run[0].clear();
+    Running<T, D> run;
+    run.clear();
     for (int j = 0; j < n; j += BN) {
         f32x16 sc[SUB];
         keys.settle(lane);
         keys.scores(sc, qf, lane);
         keys.values_to_lds(lds_v, lane);
         if (j + BN < n) keys.load(kp, vp, a.k.row, a.v.row, skip, j + BN, n, lane);
-        run[0].template weights<SUB>(sc, c, slack);
+        run.template weights<SUB>(sc, c, slack);
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int u = 0; u < SUB; u++) add_values<T, D, 1, false>(run, *(f32x16(*)[1])&sc[u], lds_v, u * 32, lane);
+        for (int u = 0; u < SUB; u++) add_values(run, sc[u], lds_v, u * 32, lane);
         __builtin_amdgcn_wave_barrier();
     }
-    const float l = run[0].sum();
+    const float l = run.sum();
     if (row >= t.z) return;   // (both lane halves of a row leave together)
     ListPart<T, D>& to = ((ListPart<T, D>*)a.work)[((q - sets.q_off[0]) * a.q.heads + head) * a.n_sel + slot];
     if constexpr (IsF32<T>::v) {
 #pragma unroll
         for (int u = 0; u < D / 32; u++)
 #pragma unroll
-            for (int b = 0; b < 4; b++) *(f32x4*)&to.o[u * 32 + 8 * b + 4 * h] = f32x4{run[0].o[u][4 * b], run[0].o[u][4 * b + 1], run[0].o[u][4 * b + 2], run[0].o[u][4 * b + 3]};
+            for (int b = 0; b < 4; b++) *(f32x4*)&to.o[u * 32 + 8 * b + 4 * h] = f32x4{run.o[u][4 * b], run.o[u][4 * b + 1], run.o[u][4 * b + 2], run.o[u][4 * b + 3]};
     } else {
         float f = inverse_sum(l), scale = 1.f;
         if constexpr (__is_same(T, __bf16)) {
@@ -664,7 +658,7 @@ __global__ __launch_bounds__(64, 2) void attention_blocks_kernel(AttentionLaunch
             for (int u = 0; u < D / 32; u++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    const float x = fabsf(run[0].o[u][r] * f);
+                    const float x = fabsf(run.o[u][r] * f);
                     most = fmaxf(most, x < INFINITY ? x : 0.f);
                 }
             const int e = max((int)(__float_as_uint(other_half(most, true)) >> 23), 14);   // biased exponent
@@ -676,12 +670,12 @@ __global__ __launch_bounds__(64, 2) void attention_blocks_kernel(AttentionLaunch
         for (int u = 0; u < D / 32; u++)
 #pragma unroll
             for (int b = 0; b < 4; b++)
-                *(f16x4*)&to.o[u * 32 + 8 * b + 4 * h] = f16x4{(_Float16)(run[0].o[u][4 * b] * f), (_Float16)(run[0].o[u][4 * b + 1] * f),
-                                                              (_Float16)(run[0].o[u][4 * b + 2] * f), (_Float16)(run[0].o[u][4 * b + 3] * f)};
+                *(f16x4*)&to.o[u * 32 + 8 * b + 4 * h] = f16x4{(_Float16)(run.o[u][4 * b] * f), (_Float16)(run.o[u][4 * b + 1] * f),
+                                                              (_Float16)(run.o[u][4 * b + 2] * f), (_Float16)(run.o[u][4 * b + 3] * f)};
         if (h == 0) to.scale = scale;
     }
     if (h == 0) {
-        to.m = run[0].m;
+        to.m = run.m;
         to.l = l;
     }
 }
@@ -694,6 +688,9 @@ struct DensePlan {
     int parts;
 };
 constexpr int kFill = 512;   // work-groups that fill the chip (two per CU)
+#ifndef WIDE_FEW
+#define WIDE_FEW 2
+#endif
 
 // units of `rows` rows of the call into sets.tile
 int count_tiles(const AttentionLaunch& a, AttnSets& sets, int rows) {
@@ -704,16 +701,20 @@ int count_tiles(const AttentionLaunch& a, AttnSets& sets, int rows) {
     return sets.tile[sets.n];
 }
 DensePlan dense_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets) {
-    if (count_tiles(a, sets, 128) >= kFill) return {true, 1};
-    const int units = count_tiles(a, sets, 32);
+    const bool f32 = dtype == PPG_F32;
     long long longest = 0;
     for (int s = 0; s < sets.n; s++) longest = std::max(longest, (long long)sets.k_off[s + 1] - sets.k_off[s]);
-    const int bn = dtype == PPG_F32 || head_dim == 128 ? 32 : 64;
+    const int few = count_tiles(a, sets, 32), many = count_tiles(a, sets, 128);
+    if (many >= kFill) return {true, 1};
+    // rows that fill 128 at least half: their keys are worth sharing, if every work-group still gets eight tiles of them
+    const long long wide_most = longest / (8 * (f32 ? 32 : 64));
+    if (many && few >= WIDE_FEW * many && many * wide_most >= kFill) return {true, (kFill + many - 1) / many};
+    count_tiles(a, sets, 32);
+    const int bn = f32 || head_dim == 128 ? 32 : 64;
     // a part has a tile for each of its waves
     const long long most = std::max(1LL, (longest + 4 * bn - 1) / (4 * bn));
-    return {false, (int)std::min<long long>(most, units ? (kFill + units - 1) / units : 1)};
+    return {false, (int)std::min<long long>(most, few ? (kFill + few - 1) / few : 1)};
 }
-
 
 // selected blocks
 struct BlocksPlan {
@@ -722,14 +723,17 @@ struct BlocksPlan {
     size_t part_bytes, list_bytes, tile_bytes;   // of the binned form, in this order
 };
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
-// Below this many list entries a query's blocks are read for itself: one launch instead of three
-constexpr long long kBinnedFrom = 512;
+// A query's blocks are read for itself (one launch instead of three) while that is no more than this many bytes of keys and values
+#ifndef BINNED_MB
+#define BINNED_MB 64
+#endif
+constexpr long long kBinnedFrom = (long long)BINNED_MB << 20;
 BlocksPlan blocks_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets) {
     const long long nq = (long long)sets.q_off[sets.n] - sets.q_off[0], kvh = a.k.heads, group = a.q.heads / kvh;
     const size_t part = (size_t)(head_dim + 4) * sizeof(float), list_part = dtype == PPG_F32 ? part : (size_t)head_dim * 2 + 16;
     BlocksPlan p{};
     sets.tile[0] = 0;
-    if (nq * kvh * a.n_sel >= kBinnedFrom) {
+    if (nq * kvh * a.n_sel * a.block * head_dim * (dtype == PPG_F32 ? 8 : 4) > kBinnedFrom) {
         p.binned = true;
         p.parts = a.n_sel;
         for (int s = 0; s < sets.n; s++)
@@ -785,9 +789,11 @@ template <class T, int D> hipError_t run(const AttentionLaunch& a, AttnSets& set
     const DensePlan p = dense_plan(dtype, D, a, sets);
     if (!sets.tile[sets.n]) return hipSuccess;
     if (p.wide) {
-        if (a.lse || IsF32<T>::v) attention_wide_kernel<T, D, WIDE_BN, 1, false><<<xcd_grid(sets.tile[sets.n]), 256, 0, s>>>(a, sets);
-        else attention_wide_kernel<T, D, WIDE_BN, 1, !IsF32<T>::v><<<xcd_grid(sets.tile[sets.n]), 256, 0, s>>>(a, sets);
-        return hipGetLastError();
+        const unsigned grid = xcd_grid(sets.tile[sets.n] * p.parts);
+        if (a.lse || IsF32<T>::v) attention_wide_kernel<T, D, WIDE_BN, false><<<grid, 256, 0, s>>>(a, sets, p.parts);
+        else attention_wide_kernel<T, D, WIDE_BN, !IsF32<T>::v><<<grid, 256, 0, s>>>(a, sets, p.parts);
+        e = hipGetLastError();
+        return e != hipSuccess || p.parts == 1 ? e : join<T, D, false>(a, sets, p.parts, s);
     }
     attention_split_kernel<T, D, OWN_BN, false><<<xcd_grid(sets.tile[sets.n] * p.parts), 256, 0, s>>>(a, sets, p.parts);
     e = hipGetLastError();

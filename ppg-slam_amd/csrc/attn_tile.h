@@ -145,10 +145,10 @@ template <class T, int D, bool UNIT = false> struct Running {
     }
 };
 
-// o += P V of 32 keys for QT groups of 32 queries; v: LDS image of the values, key0 the keys' first row in it.  The weights are
-// rounded to the values' type here, once.
-template <class T, int D, int QT, bool UNIT>
-__device__ __forceinline__ void add_values(Running<T, D, UNIT> (&run)[QT], const f32x16 (&p)[QT], const char* v, int key0, int lane) {
+// o += P V of 32 keys; v: LDS image of the values, key0 the keys' first row in it.  The weights are rounded to the values' type
+// here, once.
+template <class T, int D, bool UNIT>
+__device__ __forceinline__ void add_values(Running<T, D, UNIT>& run, const f32x16& p, const char* v, int key0, int lane) {
     using S = Shape<T, D>;
     const int h = lane >> 5;
     if constexpr (IsF32<T>::v) {
@@ -160,27 +160,21 @@ __device__ __forceinline__ void add_values(Running<T, D, UNIT> (&run)[QT], const
             for (int t = 0; t < D / 32; t++) {
                 const int d = t * 32 + (lane & 31);
                 const float a = *(const float*)(v + row * (D * 4) + ((((d >> 2) ^ S::swz_v(row)) << 4) | ((d & 3) << 2)));
-#pragma unroll
-                for (int q = 0; q < QT; q++) run[q].o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[q][r], run[q].o[t], 0, 0, 0);
+                run.o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[r], run.o[t], 0, 0, 0);
             }
         }
     } else {
         const int i = lane & 15, part = (lane >> 4) & 1;
 #pragma unroll
         for (int st = 0; st < 2; st++) {
-            u32x4 b[QT];
+            T pb[8];
 #pragma unroll
-            for (int q = 0; q < QT; q++) {
-                T pb[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) pb[e] = (T)p[q][8 * st + e];
-                b[q] = __builtin_bit_cast(u32x4, pb);
-            }
+            for (int e = 0; e < 8; e++) pb[e] = (T)p[8 * st + e];
+            const u32x4 b = __builtin_bit_cast(u32x4, pb);
             if constexpr (UNIT) {
                 const short one = __builtin_bit_cast(short, (T)1.f);
                 const s16x8 ones = {one, one, one, one, one, one, one, one};
-#pragma unroll
-                for (int q = 0; q < QT; q++) run[q].u = mfma_chunk<T>(__builtin_bit_cast(u32x4, ones), b[q], run[q].u);
+                run.u = mfma_chunk<T>(__builtin_bit_cast(u32x4, ones), b, run.u);
             }
             const int r0 = key0 + 16 * st + 4 * h + (i >> 2), r1 = r0 + 8;
 #pragma unroll
@@ -189,8 +183,7 @@ __device__ __forceinline__ void add_values(Running<T, D, UNIT> (&run)[QT], const
                 const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(v + r0 * (D * 2) + ((ch ^ S::swz_v(r0)) << 4) + in));
                 const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(v + r1 * (D * 2) + ((ch ^ S::swz_v(r1)) << 4) + in));
                 const s16x8 a = __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-                for (int q = 0; q < QT; q++) run[q].o[t] = mfma_chunk<T>(__builtin_bit_cast(u32x4, a), b[q], run[q].o[t]);
+                run.o[t] = mfma_chunk<T>(__builtin_bit_cast(u32x4, a), b, run.o[t]);
             }
         }
     }

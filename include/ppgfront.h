@@ -433,7 +433,7 @@ int ppg_block_select(ppg_ctx* ctx, const ppg_block_select_args* args, void* stre
  * meet the values, as the inputs of the matrix unit are. */
 typedef struct ppg_attention_args {
     int dtype, head_dim;
-    float scale;              /* > 0 */
+    float scale;              /* > 0, at most 1e37 */
     int n_sets;
     const int32_t *q_off, *k_off;
     ppg_rows q, k, v, out;

@@ -80,7 +80,7 @@ __global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) 
     const int q0 = sets.q_off[s], k0 = sets.k_off[s], nk = sets.k_off[s + 1] - k0, kvh = a.k.heads, group = a.q.heads / kvh;
     const int rows = (sets.q_off[s + 1] - q0) * group, tiles = (rows + 127) / 128;
     const int g = (unit - sets.tile[s]) / tiles, row = ((unit - sets.tile[s]) % tiles) * 128 + wave * 32 + (lane & 31);
-    const float c = a.scale * kLog2e, slack = 8.f / c;
+    const float c = a.scale * kLog2e, slack = rise_slack(c);
     const int all = (nk + BN - 1) / BN, from = (int)((long long)all * part / parts), to = (int)((long long)all * (part + 1) / parts);
 
     // tile loads: thread -> (row, chunk) and STEP rows on
@@ -101,7 +101,7 @@ __global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) 
         } else {   // rows behind the set are its last one
 #pragma unroll
             for (int i = 0; i < CH; i++) {
-                const long long r = min((int)j + r0 + STEP * i, nk - 1);
+                const long long r = min(j + r0 + STEP * i, (long long)nk - 1);
                 rk[i] = *(const u32x4*)(kp + r * a.k.row);
                 rv[i] = *(const u32x4*)(vp + r * a.v.row);
             }
@@ -324,7 +324,7 @@ __global__ __launch_bounds__(256, IsF32<T>::v && D == 128 ? 1 : 2) void attentio
     const int rows = SEL ? (at / per_q + 1) * group : all;
     u32x4 qf[S::NF];
     load_query<T, D>(qf, a.q, row_place(row0 + (lane & 31), rows, group, g, q0), h);
-    const float c = a.scale * kLog2e, slack = 8.f / c;
+    const float c = a.scale * kLog2e, slack = rise_slack(c);
     Running<T, D> run;
     run.clear();
     const T* kp = (const T*)a.k.p + g * a.k.head + (long long)k0 * a.k.row;
@@ -627,7 +627,7 @@ __global__ __launch_bounds__(64, IsF32<T>::v && D == 128 ? 1 : 2) void attention
     const int slot = entry % a.n_sel, head = g * group + (group == 1 ? 0 : rr % group);
     u32x4 qf[S::NF];
     load_query<T, D>(qf, a.q, RowPlace{q, head}, h);
-    const float c = a.scale * kLog2e, slack = 8.f / c;
+    const float c = a.scale * kLog2e, slack = rise_slack(c);
     Running<T, D> run;
     run.clear();
     for (int j = 0; j < n; j += BN) {
@@ -688,9 +688,6 @@ struct DensePlan {
     int parts;
 };
 constexpr int kFill = 512;   // work-groups that fill the chip (two per CU)
-#ifndef WIDE_FEW
-#define WIDE_FEW 2
-#endif
 
 // units of `rows` rows of the call into sets.tile
 int count_tiles(const AttentionLaunch& a, AttnSets& sets, int rows) {
@@ -706,14 +703,15 @@ DensePlan dense_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSets
     for (int s = 0; s < sets.n; s++) longest = std::max(longest, (long long)sets.k_off[s + 1] - sets.k_off[s]);
     const int few = count_tiles(a, sets, 32), many = count_tiles(a, sets, 128);
     if (many >= kFill) return {true, 1};
-    // rows that fill 128 at least half: their keys are worth sharing, if every work-group still gets eight tiles of them
-    const long long wide_most = longest / (8 * (f32 ? 32 : 64));
-    if (many && few >= WIDE_FEW * many && many * wide_most >= kFill) return {true, (kFill + many - 1) / many};
+    // More than 32 rows: their keys are worth sharing, if that still gives half the chip work of four tiles each (117 queries x 4
+    // heads of 128 on one key head against 219142 keys: 96 us, 280 us in 32s; 40 queries x 4 heads of 64 against 100000: 33 and 41).
+    const int wide_most = (int)std::min<long long>(longest / (4 * (f32 ? 32 : 64)), kFill);
+    if (many && few >= 2 * many && many * wide_most >= kFill / 2) return {true, std::min(wide_most, kFill / many)};
     count_tiles(a, sets, 32);
     const int bn = f32 || head_dim == 128 ? 32 : 64;
-    // a part has a tile for each of its waves
+    // a part has a tile for each of its waves; no more parts than run at once
     const long long most = std::max(1LL, (longest + 4 * bn - 1) / (4 * bn));
-    return {false, (int)std::min<long long>(most, few ? (kFill + few - 1) / few : 1)};
+    return {false, few ? (int)std::min<long long>(most, std::max(1, kFill / few)) : 1};
 }
 
 // selected blocks
@@ -723,17 +721,15 @@ struct BlocksPlan {
     size_t part_bytes, list_bytes, tile_bytes;   // of the binned form, in this order
 };
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
-// A query's blocks are read for itself (one launch instead of three) while that is no more than this many bytes of keys and values
-#ifndef BINNED_MB
-#define BINNED_MB 64
-#endif
-constexpr long long kBinnedFrom = (long long)BINNED_MB << 20;
+// A query's blocks are read for itself, in one launch instead of three, while that is no more than this many bytes of keys and
+// values (64 keys x 64 components bf16, 16 blocks, 4 heads: 40 queries, 42 MB: 16 us, turned round 22; 160, 168 MB: 28 and 22).
+constexpr long long kDirectBytes = 64LL << 20;
 BlocksPlan blocks_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets) {
     const long long nq = (long long)sets.q_off[sets.n] - sets.q_off[0], kvh = a.k.heads, group = a.q.heads / kvh;
     const size_t part = (size_t)(head_dim + 4) * sizeof(float), list_part = dtype == PPG_F32 ? part : (size_t)head_dim * 2 + 16;
     BlocksPlan p{};
     sets.tile[0] = 0;
-    if (nq * kvh * a.n_sel * a.block * head_dim * (dtype == PPG_F32 ? 8 : 4) > kBinnedFrom) {
+    if (nq * kvh * a.n_sel * a.block * head_dim * (dtype == PPG_F32 ? 8 : 4) > kDirectBytes) {
         p.binned = true;
         p.parts = a.n_sel;
         for (int s = 0; s < sets.n; s++)
@@ -747,7 +743,7 @@ BlocksPlan blocks_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSe
     for (int s = 0; s < sets.n; s++) sets.tile[s + 1] = sets.tile[s] + (int)((sets.q_off[s + 1] - sets.q_off[s]) * per_q * kvh);
     const int units = sets.tile[sets.n], bn = dtype == PPG_F32 || head_dim == 128 ? 32 : 64;
     const long long most = std::max(1LL, ((long long)a.n_sel * ((a.block + bn - 1) / bn) + 3) / 4);
-    p.parts = (int)std::min<long long>(most, units ? (kFill + units - 1) / units : 1);
+    p.parts = units ? (int)std::min<long long>(most, std::max(1, kFill / units)) : 1;
     if (p.parts > 1) p.part_bytes = (size_t)nq * a.q.heads * p.parts * part;
     return p;
 }

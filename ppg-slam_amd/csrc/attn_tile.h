@@ -77,6 +77,10 @@ __device__ __forceinline__ float other_half(float x, bool take_max) {
     return take_max ? fmaxf(lo, hi) : lo + hi;
 }
 
+// how far a product may pass m before the sums are rescaled: 2^8 in the weights (finite also for the smallest scales, where no
+// difference of products gets there)
+__device__ __forceinline__ float rise_slack(float c) { return fminf(8.f / c, 3e38f); }
+
 // Running softmax of the 32 queries of a wave, and their sums; m is the largest product seen (or up to 2^8 less in the
 // exponent: the sums are rescaled only when a product passes it by that much, which any type holds), c = scale * log2 e.
 //

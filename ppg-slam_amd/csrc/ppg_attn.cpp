@@ -38,6 +38,8 @@ const char* rows_fault(const ppg_rows& r, int dtype, int head_dim, long long n_r
     return nullptr;
 }
 
+constexpr long long kMostVectors = (1LL << 31) - (1 << 10);   // rows times heads of a call: tiles that pass a set's end stay countable
+
 bool known_type(int dtype) { return dtype == PPG_F32 || dtype == PPG_BF16 || dtype == PPG_F16; }
 bool known_dim(int d) { return d == 32 || d == 64 || d == 128; }
 bool known_block(int b) { return b == 32 || b == 64 || b == 128; }
@@ -74,15 +76,16 @@ int attention_checked(ppg_ctx* c, const ppg_attention_args* a, bool sizes_only, 
     if (!a) return fail(c, PPG_EINVAL, "%s: args is NULL", who);
     if (!known_type(a->dtype)) return fail(c, PPG_EINVAL, "%s: dtype %d is none of PPG_F32, PPG_BF16, PPG_F16", who, a->dtype);
     if (!known_dim(a->head_dim)) return fail(c, PPG_EINVAL, "%s: head_dim %d (32, 64 and 128 are built)", who, a->head_dim);
-    if (!(a->scale > 0.f) || !(a->scale < INFINITY)) return fail(c, PPG_EINVAL, "%s: scale must be positive and finite", who);
+    if (!(a->scale > 0.f) || !(a->scale <= 1e37f)) return fail(c, PPG_EINVAL, "%s: scale must be positive, at most 1e37", who);
     int rc = set_count(c, who, a->n_sets);
     if (rc) return rc;
     sets.n = a->n_sets;
     if ((rc = set_offsets(c, who, a->n_sets, a->q_off, "q_off", sets.q_off))) return rc;
     if ((rc = set_offsets(c, who, a->n_sets, a->k_off, "k_off", sets.k_off))) return rc;
     const long long nq = (long long)sets.q_off[sets.n] - sets.q_off[0], nk = (long long)sets.k_off[sets.n] - sets.k_off[0];
-    if (nq * a->q.heads >= (1LL << 31) || nk * a->k.heads >= (1LL << 31))
-        return fail(c, PPG_ECAP, "%s: rows times heads must stay below 2^31", who);
+    if (nq * a->q.heads >= kMostVectors || nk * a->k.heads >= kMostVectors)
+        return fail(c, PPG_ECAP, "%s: rows times heads must stay below 2^31 - 2^10", who);
+    if ((uintptr_t)a->lse % 4 || (uintptr_t)a->sel % 4) return fail(c, PPG_EINVAL, "%s: lse or sel is not at a multiple of 4", who);
     const ppg_rows* r[4] = {&a->q, &a->k, &a->v, &a->out};
     static const char* name[4] = {"q", "k", "v", "out"};
     for (int i = 0; i < 4; i++) {
@@ -153,7 +156,8 @@ int ppg_rotary(ppg_ctx* c, const ppg_rotary_args* a, void* stream) {
     if (a->rot_dim < 0 || a->rot_dim > a->head_dim || a->rot_dim % (2 * a->n_axes))
         return fail(c, PPG_EINVAL, "%s: rot_dim %d must be a multiple of %d, at most head_dim", who, a->rot_dim, 2 * a->n_axes);
     if (a->n_rows[0] < 0 || a->n_rows[1] < 0) return fail(c, PPG_EINVAL, "%s: n_rows is negative", who);
-    if (a->rot_dim && !a->freq && (a->n_rows[0] || a->n_rows[1])) return fail(c, PPG_EINVAL, "%s: freq is NULL", who);
+    if (a->rot_dim && (!a->freq || (uintptr_t)a->freq % 8) && (a->n_rows[0] || a->n_rows[1]))
+        return fail(c, PPG_EINVAL, "%s: freq is NULL or not at a multiple of 8", who);
     ppg::RotaryLaunch l;
     l.head_dim = a->head_dim; l.rot_dim = a->rot_dim; l.layout = a->layout; l.inverse = a->inverse != 0; l.n_axes = a->n_axes;
     l.freq = a->freq;
@@ -163,7 +167,8 @@ int ppg_rotary(ppg_ctx* c, const ppg_rotary_args* a, void* stream) {
         l.src[i] = a->src[i];
         l.dst[i] = a->dst[i];
         if (!a->n_rows[i]) continue;
-        if (a->rot_dim && !a->pos[i]) return fail(c, PPG_EINVAL, "%s: pos[%d] is NULL", who, i);
+        if (a->rot_dim && (!a->pos[i] || (uintptr_t)a->pos[i] % 4)) return fail(c, PPG_EINVAL, "%s: pos[%d] is NULL or not at a multiple of 4", who, i);
+        if ((long long)a->n_rows[i] * a->src[i].heads >= kMostVectors) return fail(c, PPG_ECAP, "%s: rows times heads must stay below 2^31 - 2^10", who);
         const char* fault = rows_fault(a->src[i], a->dtype, a->head_dim, a->n_rows[i], false);
         if (fault) return fail(c, PPG_EINVAL, "%s: src[%d]: %s", who, i, fault);
         if ((fault = rows_fault(a->dst[i], a->dtype, a->head_dim, a->n_rows[i], true))) return fail(c, PPG_EINVAL, "%s: dst[%d]: %s", who, i, fault);
@@ -192,7 +197,8 @@ int ppg_block_means(ppg_ctx* c, const ppg_block_means_args* a, void* stream) {
     const char* fault = rows_fault(a->k, a->dtype, a->head_dim, nk, false);
     if (fault) return fail(c, PPG_EINVAL, "%s: k: %s", who, fault);
     if (nk && (!a->mean || !a->count)) return fail(c, PPG_EINVAL, "%s: mean or count is NULL", who);
-    if ((uintptr_t)a->mean % 16) return fail(c, PPG_EINVAL, "%s: mean is not at a multiple of 16", who);
+    if ((uintptr_t)a->mean % 16 || (uintptr_t)a->count % 4) return fail(c, PPG_EINVAL, "%s: mean is not at a multiple of 16, or count of 4", who);
+    if (nk * a->k.heads >= kMostVectors) return fail(c, PPG_ECAP, "%s: rows times heads must stay below 2^31 - 2^10", who);
     block_offsets(sets, a->block);
     ppg::BlockMeansLaunch l;
     l.block = a->block; l.k = a->k; l.skip = a->skip; l.mean = a->mean; l.count = a->count;
@@ -221,7 +227,10 @@ int ppg_block_select(ppg_ctx* c, const ppg_block_select_args* a, void* stream) {
     if (fault) return fail(c, PPG_EINVAL, "%s: q: %s", who, fault);
     if (a->kv_heads < 1 || a->q.heads % a->kv_heads) return fail(c, PPG_EINVAL, "%s: kv_heads must divide the heads of q", who);
     if ((nq && !a->sel) || (nq && nk && (!a->mean || !a->count))) return fail(c, PPG_EINVAL, "%s: sel, mean or count is NULL", who);
-    if ((uintptr_t)a->mean % 16) return fail(c, PPG_EINVAL, "%s: mean is not at a multiple of 16", who);
+    if ((uintptr_t)a->mean % 16 || (uintptr_t)a->count % 4 || (uintptr_t)a->sel % 4)
+        return fail(c, PPG_EINVAL, "%s: mean is not at a multiple of 16, or count or sel of 4", who);
+    if (nq * a->q.heads >= kMostVectors || nk * a->kv_heads >= kMostVectors || nq * a->kv_heads * a->n_sel >= kMostVectors)
+        return fail(c, PPG_ECAP, "%s: rows times heads (and times n_sel) must stay below 2^31 - 2^10", who);
     block_offsets(sets, a->block);
     ppg::BlockSelectLaunch l;
     l.block = a->block; l.kv_heads = a->kv_heads; l.n_sel = a->n_sel; l.q = a->q; l.mean = a->mean; l.count = a->count; l.sel = a->sel;

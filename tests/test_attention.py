@@ -63,7 +63,9 @@ def test_valid_arguments_are_refused_only_for_the_missing_context(pkg):
     (dict(q=dict(heads=3, row=192), out=dict(heads=3, row=192)), "PPG_EINVAL", "divide"),
     (dict(block=48, n_sel=4, sel=4096), "PPG_EINVAL", "block 48"), (dict(block=64, n_sel=0, sel=4096), "PPG_EINVAL", "n_sel"),
     (dict(block=64, n_sel=65, sel=4096), "PPG_ECAP", "n_sel 65"), (dict(block=64, n_sel=4), "PPG_EINVAL", "sel is NULL"),
-    (dict(sel=4096), "PPG_EINVAL", "block 0"),
+    (dict(sel=4096), "PPG_EINVAL", "block 0"), (dict(scale=2e37), "PPG_EINVAL", "scale"), (dict(lse=4098), "PPG_EINVAL", "lse"),
+    (dict(block=64, n_sel=4, sel=4097), "PPG_EINVAL", "sel"), (dict(q_off=[0, 1 << 30]), "PPG_ECAP", "2^31"), (dict(k_off=[0, 2000000000]), "PPG_ECAP", "2^31"),
+    (dict(q_off=[0, 1 << 24], block=64, n_sel=64, sel=4096), "PPG_ECAP", "2^30"),
 ])
 def test_attention_refuses(pkg, change, code, word):
     kw = {}
@@ -87,6 +89,7 @@ def test_attention_refuses_offsets_that_are_missing(pkg):
     (dict(dtype=-1), "dtype"), (dict(head_dim=96), "head_dim"), (dict(layout=2), "layout"), (dict(n_axes=3), "n_axes"),
     (dict(rot_dim=66), "rot_dim"), (dict(rot_dim=-2), "rot_dim"), (dict(rot_dim=30, n_axes=2), "rot_dim"), (dict(freq=None), "freq"),
     (dict(n_rows=(-1,)), "n_rows"), (dict(pos=(None,)), "pos[0]"), (dict(dst="overlap"), "other strides"), (dict(dst="heads"), "heads"),
+    (dict(pos=(4098,)), "pos[0]"), (dict(freq=4100), "freq"), (dict(n_rows=((1 << 30),)), "2^31"),
 ])
 def test_rotary_refuses(pkg, change, word):
     f = dict(dtype=pkg.F16, head_dim=64, rot_dim=64, layout=0, n_axes=1, freq=4096, n_rows=(3,), pos=(4096,), src=(_rows(pkg),),
@@ -97,7 +100,7 @@ def test_rotary_refuses(pkg, change, word):
     if change.get("dst") == "heads":
         f["dst"] = (_rows(pkg, heads=4, p=8192),)
     rc, why = _refusal(pkg, "ppg_rotary", pkg.rotary_args(**f))
-    assert rc == pkg.PPG_EINVAL and word in why, why
+    assert rc == (pkg.PPG_ECAP if "2^" in word else pkg.PPG_EINVAL) and word in why, why
 
 
 @pytest.mark.parametrize("change, code, word", [
@@ -415,6 +418,8 @@ SHAPES = [
     (64, 2, 2, [130] + [129] * 127, [4500] + [40] * 127, 0.05), (128, 2, 2, [130] + [129] * 127, [4500] + list(range(127)), 0.3),
     (32, 4, 4, [100, 129, 1, 0] * 32, [65, 0, 127, 3] * 31 + [64, 63, 8200, 1], 0.0), (64, 12, 4, [90, 129] * 20, [33, 64] * 20, 0.5),
     (128, 8, 2, [300] * 22, [130, 1] * 11, 0.0),
+    # fewer rows against long sets: the same kernel with the keys in shares (the mask's window starts anywhere), rows of several tiles
+    (64, 4, 4, [300], [9001], 0.05), (128, 4, 4, [140, 70], [9000, 300], 0.5), (32, 8, 8, [129], [5001], 0.0), (64, 8, 2, [9], [30011], 0.02),
 ]
 
 

@@ -140,20 +140,20 @@ __global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) 
     constexpr int PER_WINDOW = kWindow * 64 / BN;   // tiles
 
     unsigned long long dead = 0;   // of the tile being multiplied
-    if (from < to) {
-        if (a.skip) {
-            window(from);
-            __syncthreads();
-        }
-        dead = dead_of(from);
-        fetch(from);
-    }
     const RowPlace place = row_place(row, rows, group, g, q0);
     u32x4 qf[S::NF];
     load_query<T, D>(qf, a.q, place, h);
     Running<T, D, UNIT> run;
     run.clear();
-    if (from < to) store(from, dead);
+    if (from < to) {
+        fetch(from);
+        if (a.skip) {
+            window(from);
+            __syncthreads();
+        }
+        dead = dead_of(from);
+        store(from, dead);
+    }
     __syncthreads();
     for (int t = from; t < to; t++) {
         const int buf = t & 1;

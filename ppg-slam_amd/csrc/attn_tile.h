@@ -46,12 +46,12 @@ template <class T, int D> struct Shape {
     // chunk i of the operand of the lane half h: 16-bit: the 8 components that one MFMA wants from it; 32-bit: the two
     // halves of a row belong to the two lane halves (any pairing of components serves, the same for both operands)
     static __device__ __forceinline__ int chunk(int i, int h) { return IsF32<T>::v ? h * NF + i : 2 * i + h; }
-    // LDS images keep a row's chunks permuted so that what one access touches lies in different banks: the eight rows that
-    // the lanes of a 16-byte read take the same chunk of, and the four rows by two chunks of a transposing read
-    static __device__ __forceinline__ int swz_k(int row) { return CPR >= 8 ? row & 7 : (row >> 1) & 3; }
+    // LDS images keep a row's chunks permuted so that what one access touches lies in different banks (64 of them, 256 bytes):
+    // the 16 rows of which 16 lanes take the same chunk, and the four rows by 64 bytes of a transposing read's 32 lanes
+    static __device__ __forceinline__ int swz_k(int row) { return CPR >= 16 ? row & 15 : CPR == 8 ? (row >> 1) & 7 : (row >> 2) & 3; }
     static __device__ __forceinline__ int swz_v(int row) {
         if (IsF32<T>::v) return swz_k(row);
-        return CPR >= 8 ? ((row & 3) << 1) | ((row >> 2) & 1) : row & 2;
+        return CPR >= 16 ? (row & 3) << 2 : CPR == 8 ? (row & 2) << 1 : 0;
     }
 };
 

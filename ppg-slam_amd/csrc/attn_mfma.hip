@@ -48,6 +48,30 @@ template <class T, int D> __device__ __forceinline__ void store_out(const ppg_ro
             else *(s16x4*)(y + t * 32 + 8 * b + 4 * h) = __builtin_bit_cast(s16x4, w);
         }
 }
+// The same for 16-bit numbers (E) by way of an LDS image of the wave's own (32 rows of D): a row is then stored by neighbouring
+// lanes, 16 bytes each, in one piece.  f: factor of this lane's row; to(r): where row r goes, or null.
+template <class E, int D, class To> __device__ __forceinline__ void store_rows(char* image, const f32x16 (&o)[D / 32], float f, int lane, To to) {
+    constexpr int CPR = D / 8;
+    const int h = lane >> 5, row = lane & 31;
+    auto place = [&](int r, int ch) { return image + r * (D * 2) + ((ch ^ (r & (CPR - 1))) << 4); };
+#pragma unroll
+    for (int t = 0; t < D / 32; t++)
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            E w[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = (E)(f == 0.f ? 0.f : o[t][b * 4 + e] * f);
+            *(s16x4*)(place(row, t * 4 + b) + 8 * h) = __builtin_bit_cast(s16x4, w);
+        }
+    __builtin_amdgcn_wave_barrier();   // (LDS serves a wave in order)
+#pragma unroll
+    for (int i = 0; i < 32 * CPR / 64; i++) {
+        const int r = (lane + 64 * i) / CPR, ch = (lane + 64 * i) % CPR;
+        E* y = (E*)to(r);
+        const u32x4 v = *(const u32x4*)place(r, ch);
+        if (y) *(u32x4*)(y + ch * 8) = v;
+    }
+}
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }
 __device__ __forceinline__ float log_sum(float m, float l, float c) { return l == 0.f ? -INFINITY : fmaf(m, c, __log2f(l)) * kLn2; }
 
@@ -191,6 +215,19 @@ __global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) 
         __syncthreads();
     }
     const float l = run.sum();
+    if constexpr (!IsF32<T>::v) {
+        if (parts == 1) {   // (the tiles' last reads are behind the last barrier)
+            static_assert(2 * TILE >= 128 * ROWB, "the key tiles' place holds the rows");
+            const int first = row - (lane & 31);
+            if (a.lse && h == 0 && row < rows) a.lse[place.q * a.q.heads + place.head] = log_sum(run.m, l, c);
+            store_rows<T, D>(lds_k[0] + wave * 32 * ROWB, run.o, inverse_sum(l), lane, [&](int r) -> void* {
+                if (first + r >= rows) return nullptr;
+                const RowPlace p = row_place(first + r, rows, group, g, q0);
+                return (T*)a.out.p + p.q * a.out.row + p.head * a.out.head;
+            });
+            return;
+        }
+    }
     if (row >= rows) return;
     if (parts > 1) {
         Part<D>& w = ((Part<D>*)a.work)[((place.q - sets.q_off[0]) * a.q.heads + place.head) * parts + part];
@@ -297,8 +334,7 @@ template <class T, int D> __device__ __forceinline__ void meet(Meeting<T, D>& x,
 // written and read between the two kernels (8 streams: PARTH_TIME).
 template <int D> struct PartH {
     _Float16 o[D];
-    float m, l, scale;   // o * scale is the mean
-    float pad;
+    float m, l, scale, pad;   // o * scale is the mean
 };
 template <class T, int D> using ListPart = std::conditional_t<IsF32<T>::v, Part<D>, PartH<D>>;
 
@@ -643,13 +679,18 @@ __global__ __launch_bounds__(64, IsF32<T>::v && D == 128 ? 1 : 2) void attention
         __builtin_amdgcn_wave_barrier();
     }
     const float l = run.sum();
-    if (row >= t.z) return;   // (both lane halves of a row leave together)
-    ListPart<T, D>& to = ((ListPart<T, D>*)a.work)[((q - sets.q_off[0]) * a.q.heads + head) * a.n_sel + slot];
+    using P = ListPart<T, D>;
+    P* to = row < t.z ? (P*)a.work + (((q - sets.q_off[0]) * a.q.heads + head) * a.n_sel + slot) : nullptr;
     if constexpr (IsF32<T>::v) {
+        if (!to) return;   // (both lane halves of a row leave together)
 #pragma unroll
         for (int u = 0; u < D / 32; u++)
 #pragma unroll
-            for (int b = 0; b < 4; b++) *(f32x4*)&to.o[u * 32 + 8 * b + 4 * h] = f32x4{run.o[u][4 * b], run.o[u][4 * b + 1], run.o[u][4 * b + 2], run.o[u][4 * b + 3]};
+            for (int b = 0; b < 4; b++) *(f32x4*)&to->o[u * 32 + 8 * b + 4 * h] = f32x4{run.o[u][4 * b], run.o[u][4 * b + 1], run.o[u][4 * b + 2], run.o[u][4 * b + 3]};
+        if (h == 0) {
+            to->m = run.m;
+            to->l = l;
+        }
     } else {
         float f = inverse_sum(l), scale = 1.f;
         if constexpr (__is_same(T, __bf16)) {
@@ -665,18 +706,11 @@ __global__ __launch_bounds__(64, IsF32<T>::v && D == 128 ? 1 : 2) void attention
             scale = __uint_as_float((unsigned)(e - 13) << 23);
             f *= __uint_as_float((unsigned)(267 - e) << 23);
         }
-        typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-#pragma unroll
-        for (int u = 0; u < D / 32; u++)
-#pragma unroll
-            for (int b = 0; b < 4; b++)
-                *(f16x4*)&to.o[u * 32 + 8 * b + 4 * h] = f16x4{(_Float16)(run.o[u][4 * b] * f), (_Float16)(run.o[u][4 * b + 1] * f),
-                                                              (_Float16)(run.o[u][4 * b + 2] * f), (_Float16)(run.o[u][4 * b + 3] * f)};
-        if (h == 0) to.scale = scale;
-    }
-    if (h == 0) {
-        to.m = run.m;
-        to.l = l;
+        if (to && h == 0) *(f32x4*)&to->m = f32x4{run.m, l, scale, 0.f};
+        const unsigned long long at_ = (unsigned long long)to;
+        store_rows<_Float16, D>(lds_v, run.o, f, lane, [&](int r) -> void* {
+            return (void*)(((unsigned long long)(unsigned)__shfl((int)(at_ >> 32), r) << 32) | (unsigned)__shfl((int)at_, r));
+        });
     }
 }
 

@@ -73,7 +73,7 @@ template <class E, int D, class To> __device__ __forceinline__ void store_rows(c
     }
 }
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }
-__device__ __forceinline__ float log_sum(float m, float l, float c) { return l == 0.f ? -INFINITY : fmaf(m, c, __log2f(l)) * kLn2; }
+template <class T> __device__ __forceinline__ float log_sum(float m, float l, float c) { return l == 0.f ? -INFINITY : fmaf(m, c, __log2f(l) - kLift<T>) * kLn2; }
 
 // Sums of one (row, part): D components, then m and l.  A part without keys has m = -inf, l = 0.
 template <int D> struct Part {
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) 
         if (parts == 1) {   // (the tiles' last reads are behind the last barrier)
             static_assert(2 * TILE >= 128 * ROWB, "the key tiles' place holds the rows");
             const int first = row - (lane & 31);
-            if (a.lse && h == 0 && row < rows) a.lse[place.q * a.q.heads + place.head] = log_sum(run.m, l, c);
+            if (a.lse && h == 0 && row < rows) a.lse[place.q * a.q.heads + place.head] = log_sum<T>(run.m, l, c);
             store_rows<T, D>(lds_k[0] + wave * 32 * ROWB, run.o, inverse_sum(l), lane, [&](int r) -> void* {
                 if (first + r >= rows) return nullptr;
                 const RowPlace p = row_place(first + r, rows, group, g, q0);
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) 
         return;
     }
     store_out<T, D>(a.out, place, run.o, inverse_sum(l), h);
-    if (a.lse && h == 0) a.lse[place.q * a.q.heads + place.head] = log_sum(run.m, l, c);
+    if (a.lse && h == 0) a.lse[place.q * a.q.heads + place.head] = log_sum<T>(run.m, l, c);
 }
 
 // A wave's own stretch of keys: operands straight from memory, values through an LDS image of its own.
@@ -328,15 +328,15 @@ template <class T, int D> __device__ __forceinline__ void meet(Meeting<T, D>& x,
     }
 }
 
-// The same for a selected block of a query, with 16-bit types: the mean of the values (o / l) in fp16, times a power of two that
-// brings the largest into [2^13, 2^14) where the values' own type reaches further than fp16.  That is off by 2^-11 of each
-// component (and 2^-38 of the largest), where the result is rounded to 2^-11 (fp16) or 2^-8 (bf16) anyway; it halves what is
-// written and read between the two kernels (8 streams: PARTH_TIME).
+// The same for a selected block of a query with bf16: the mean of the values (o / l) in fp16, times a power of two that brings the
+// largest into [2^13, 2^14).  That is off by 2^-11 of each component (and 2^-38 of the largest), where the result is rounded to
+// 2^-8 anyway; it halves what is written and read between the two kernels (8 streams: 208 -> 190 us when it came).
+// With fp16 the same rounding would be as large as the result's own: its parts stay in 32 bits.
 template <int D> struct PartH {
     _Float16 o[D];
     float m, l, scale, pad;   // o * scale is the mean
 };
-template <class T, int D> using ListPart = std::conditional_t<IsF32<T>::v, Part<D>, PartH<D>>;
+template <class T, int D> using ListPart = std::conditional_t<__is_same(T, __bf16), PartH<D>, Part<D>>;
 
 // SEL: a unit's rows are the group of one query, its keys the blocks of that query's list.
 template <class T, int D, int BN, bool SEL>
@@ -420,7 +420,7 @@ __global__ __launch_bounds__(256, IsF32<T>::v && D == 128 ? 1 : 2) void attentio
         T* to_ = (T*)a.out.p + p.q * a.out.row + p.head * a.out.head + d;
         if constexpr (IsF32<T>::v) *(f32x4*)to_ = __builtin_bit_cast(f32x4, out);
         else *(s16x4*)to_ = __builtin_bit_cast(s16x4, out);
-        if (a.lse && d == 0) a.lse[p.q * a.q.heads + p.head] = log_sum(m, l, c);
+        if (a.lse && d == 0) a.lse[p.q * a.q.heads + p.head] = log_sum<T>(m, l, c);
     }
 }
 
@@ -510,7 +510,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, 
 #pragma unroll
     for (int e = 0; e < C; e++) out.v[e] = (T)(inv == 0.f ? 0.f : o[e] * inv);
     *(Out*)((T*)a.out.p + q * a.out.row + head * a.out.head + d) = out;
-    if (a.lse && d == 0) a.lse[q * a.q.heads + head] = log_sum(m, l, c);
+    if (a.lse && d == 0) a.lse[q * a.q.heads + head] = log_sum<T>(m, l, c);
 }
 
 // ---- selected blocks, many queries ----
@@ -681,7 +681,7 @@ __global__ __launch_bounds__(64, IsF32<T>::v && D == 128 ? 1 : 2) void attention
     const float l = run.sum();
     using P = ListPart<T, D>;
     P* to = row < t.z ? (P*)a.work + (((q - sets.q_off[0]) * a.q.heads + head) * a.n_sel + slot) : nullptr;
-    if constexpr (IsF32<T>::v) {
+    if constexpr (!__is_same(T, __bf16)) {
         if (!to) return;   // (both lane halves of a row leave together)
 #pragma unroll
         for (int u = 0; u < D / 32; u++)
@@ -692,21 +692,17 @@ __global__ __launch_bounds__(64, IsF32<T>::v && D == 128 ? 1 : 2) void attention
             to->l = l;
         }
     } else {
-        float f = inverse_sum(l), scale = 1.f;
-        if constexpr (__is_same(T, __bf16)) {
-            float most = 0.f;   // of the finite ones
+        float f = inverse_sum(l), most = 0.f;   // of the finite ones
 #pragma unroll
-            for (int u = 0; u < D / 32; u++)
+        for (int u = 0; u < D / 32; u++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const float x = fabsf(run.o[u][r] * f);
-                    most = fmaxf(most, x < INFINITY ? x : 0.f);
-                }
-            const int e = max((int)(__float_as_uint(other_half(most, true)) >> 23), 14);   // biased exponent
-            scale = __uint_as_float((unsigned)(e - 13) << 23);
-            f *= __uint_as_float((unsigned)(267 - e) << 23);
-        }
-        if (to && h == 0) *(f32x4*)&to->m = f32x4{run.m, l, scale, 0.f};
+            for (int r = 0; r < 16; r++) {
+                const float x = fabsf(run.o[u][r] * f);
+                most = fmaxf(most, x < INFINITY ? x : 0.f);
+            }
+        const int e = max((int)(__float_as_uint(other_half(most, true)) >> 23), 14);   // biased exponent
+        f *= __uint_as_float((unsigned)(267 - e) << 23);
+        if (to && h == 0) *(f32x4*)&to->m = f32x4{run.m, l, __uint_as_float((unsigned)(e - 13) << 23), 0.f};
         const unsigned long long at_ = (unsigned long long)to;
         store_rows<_Float16, D>(lds_v, run.o, f, lane, [&](int r) -> void* {
             return (void*)(((unsigned long long)(unsigned)__shfl((int)(at_ >> 32), r) << 32) | (unsigned)__shfl((int)at_, r));
@@ -760,7 +756,7 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 constexpr long long kDirectBytes = 64LL << 20;
 BlocksPlan blocks_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets) {
     const long long nq = (long long)sets.q_off[sets.n] - sets.q_off[0], kvh = a.k.heads, group = a.q.heads / kvh;
-    const size_t part = (size_t)(head_dim + 4) * sizeof(float), list_part = dtype == PPG_F32 ? part : (size_t)head_dim * 2 + 16;
+    const size_t part = (size_t)(head_dim + 4) * sizeof(float), list_part = dtype == PPG_BF16 ? (size_t)head_dim * 2 + 16 : part;
     BlocksPlan p{};
     sets.tile[0] = 0;
     if (nq * kvh * a.n_sel * a.block * head_dim * (dtype == PPG_F32 ? 8 : 4) > kDirectBytes) {

@@ -81,6 +81,10 @@ __device__ __forceinline__ float other_half(float x, bool take_max) {
 // difference of products gets there)
 __device__ __forceinline__ float rise_slack(float c) { return fminf(8.f / c, 3e38f); }
 
+// Weights are 2^kLift times what the softmax says, in every sum alike: with fp16, whose smallest normal number is 2^-14, small ones
+// then keep their precision (and the largest, 2^8 over m, are 2^15).
+template <class T> constexpr float kLift = __is_same(T, _Float16) ? 7.f : 0.f;
+
 // Running softmax of the 32 queries of a wave, and their sums; m is the largest product seen (or up to 2^8 less in the
 // exponent: the sums are rescaled only when a product passes it by that much, which any type holds), c = scale * log2 e.
 //
@@ -132,7 +136,7 @@ template <class T, int D, bool UNIT = false> struct Running {
     }
     // weights in the place of the scores
     template <int SUB> __device__ __forceinline__ void weigh(f32x16 (&s)[SUB], float c) {
-        const float mc = m == -INFINITY ? 0.f : m * c;   // nothing so far: every weight below is exp2(-inf)
+        const float mc = (m == -INFINITY ? 0.f : m * c) - kLift<T>;   // (nothing so far: every weight below is exp2(-inf))
         float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int u = 0; u < SUB; u++)

@@ -7,9 +7,8 @@ n keys and D components: a product q.k in 32 bits is off by at most (D + 4) 2^-2
 denominator, twice for the maximum that is subtracted).  Sums over the keys are taken in tiles of at least 32, so they add
 at most (n / 32 + 64) roundings.  With 16-bit types a weight is rounded once (u of the type; below fp16's smallest normal
 number 2^-25 absolutely, with a denominator of at least 1), and the result once more.  A stands for sum p |v|.  Selected
-blocks with 16-bit types: every block's mean passes through fp16 (scaled for bf16), which is off by 2^-11 of its components
-and 2^-25 for fp16, 2^-38 of its largest for bf16, both at most 2^-25 max |v|; the means' weights add up to 1, so that is
-2^-11 A + 2^-25 max |v| more (max |v| <= sum |v|)."""
+blocks with bf16: every block's mean passes through fp16, scaled, which is off by 2^-11 of its components and 2^-38 of its
+largest (at most max |v|); the means' weights add up to 1, so that is 2^-11 A + 2^-38 max |v| more (max |v| <= sum |v|)."""
 import ctypes as C
 import math
 
@@ -377,8 +376,8 @@ def _check_attend(torch, dtype, got, lse, ref, blocks=False):
         t = t + 2.0 ** -25 * (v_abs + 1)
     if dtype == "fp32":
         t = t + 2.0 ** -126
-    elif blocks:
-        t = t + 2.0 ** -11 * a_abs + 2.0 ** -25 * (v_abs.amax(-1, keepdim=True) + 1)
+    if dtype == "bf16" and blocks:
+        t = t + 2.0 ** -11 * a_abs + 2.0 ** -38 * v_abs.amax(-1, keepdim=True)
     err = (got.cpu().double() - out).abs()
     ok = (err <= t) | (out.isnan() & got.cpu().isnan())
     assert ok.all(), (float((err / t.clamp(min=1e-300))[~ok].max()), int((~ok).sum()))

@@ -34,21 +34,19 @@ __device__ __forceinline__ void load_query(u32x4 (&f)[NF], const ppg_rows& q, co
     for (int i = 0; i < Shape<T, D>::NF; i++) f[i] = *(const u32x4*)(x + Shape<T, D>::chunk(i, h) * Shape<T, D>::N);
 }
 
-// this lane's components of its query: 4 consecutive ones per register group
-template <class T, int D> __device__ __forceinline__ void store_out(const ppg_rows& out, const RowPlace& p, const f32x16 (&o)[D / 32], float inv, int h) {
-    T* y = (T*)out.p + p.q * out.row + p.head * out.head;
+// Rows of 32-bit results: this lane's components of its own row, 4 consecutive ones per register group.
+template <int D> __device__ __forceinline__ void store_row(float* y, const f32x16 (&o)[D / 32], float f, int h) {
 #pragma unroll
     for (int t = 0; t < D / 32; t++)
 #pragma unroll
         for (int b = 0; b < 4; b++) {
-            T w[4];
+            f32x4 w;
 #pragma unroll
-            for (int e = 0; e < 4; e++) w[e] = (T)(inv == 0.f ? 0.f : o[t][b * 4 + e] * inv);
-            if constexpr (IsF32<T>::v) *(f32x4*)(y + t * 32 + 8 * b + 4 * h) = __builtin_bit_cast(f32x4, w);
-            else *(s16x4*)(y + t * 32 + 8 * b + 4 * h) = __builtin_bit_cast(s16x4, w);
+            for (int e = 0; e < 4; e++) w[e] = f == 0.f ? 0.f : o[t][b * 4 + e] * f;
+            *(f32x4*)(y + t * 32 + 8 * b + 4 * h) = w;
         }
 }
-// The same for 16-bit numbers (E) by way of an LDS image of the wave's own (32 rows of D): a row is then stored by neighbouring
+// Rows of 16-bit results (E), by way of an LDS image of the wave's own (32 rows of D): a row is then stored by neighbouring
 // lanes, 16 bytes each, in one piece.  f: factor of this lane's row; to(r): where row r goes, or null.
 template <class E, int D, class To> __device__ __forceinline__ void store_rows(char* image, const f32x16 (&o)[D / 32], float f, int lane, To to) {
     constexpr int CPR = D / 8;
@@ -82,6 +80,12 @@ template <int D> struct Part {
     float pad[2];
 };
 
+// Four waves of 32 rows each.  8192 x 8191 keys, 2 heads of 128, 4 sets: 300 us, 916 TFLOP/s, where a library product of 8192^3
+// reaches 1122; 64 streams of about 870, 4 heads of 64: 97 us, 517 TFLOP/s (with 8192 keys a set: 810).  Counters at 64
+// components: the vector unit (exponentials, maxima, conversions: 155 instructions for 64 keys) is busy for 61 % of the time,
+// the matrix unit for 47 %, at 2.0 GHz, the clock that the power limit leaves; what short sets lose is the work-group's start
+// (queries, first tiles) and the chip's last round.  Two waves of a SIMD in opposite phases, held there by barriers, measured
+// slower (315 and 1555 us instead of 303 and 1367): a single wave cannot keep the vector unit busy.
 // parts > 1: a work-group takes its share of the keys and leaves its sums.
 // Which keys are masked is read once, a bit each, kWindow words ahead, so that the loads of a tile do not wait for it.
 // UNIT (16-bit types): the matrix unit adds up the weights (a product with ones); the vector unit, which has the exponentials, is
@@ -215,37 +219,32 @@ __global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) 
         __syncthreads();
     }
     const float l = run.sum();
-    if constexpr (!IsF32<T>::v) {
-        if (parts == 1) {   // (the tiles' last reads are behind the last barrier)
-            static_assert(2 * TILE >= 128 * ROWB, "the key tiles' place holds the rows");
-            const int first = row - (lane & 31);
-            if (a.lse && h == 0 && row < rows) a.lse[place.q * a.q.heads + place.head] = log_sum<T>(run.m, l, c);
-            store_rows<T, D>(lds_k[0] + wave * 32 * ROWB, run.o, inverse_sum(l), lane, [&](int r) -> void* {
-                if (first + r >= rows) return nullptr;
-                const RowPlace p = row_place(first + r, rows, group, g, q0);
-                return (T*)a.out.p + p.q * a.out.row + p.head * a.out.head;
-            });
-            return;
-        }
-    }
-    if (row >= rows) return;
     if (parts > 1) {
+        if (row >= rows) return;
         Part<D>& w = ((Part<D>*)a.work)[((place.q - sets.q_off[0]) * a.q.heads + place.head) * parts + part];
-#pragma unroll
-        for (int u = 0; u < D / 32; u++)
-#pragma unroll
-            for (int b = 0; b < 4; b++) *(f32x4*)&w.o[u * 32 + 8 * b + 4 * h] = f32x4{run.o[u][4 * b], run.o[u][4 * b + 1], run.o[u][4 * b + 2], run.o[u][4 * b + 3]};
+        store_row<D>(w.o, run.o, 1.f, h);
         if (h == 0) {
             w.m = run.m;
             w.l = l;
         }
         return;
     }
-    store_out<T, D>(a.out, place, run.o, inverse_sum(l), h);
-    if (a.lse && h == 0) a.lse[place.q * a.q.heads + place.head] = log_sum<T>(run.m, l, c);
+    if (a.lse && h == 0 && row < rows) a.lse[place.q * a.q.heads + place.head] = log_sum<T>(run.m, l, c);
+    if constexpr (IsF32<T>::v) {
+        if (row < rows) store_row<D>((float*)a.out.p + place.q * a.out.row + place.head * a.out.head, run.o, inverse_sum(l), h);
+    } else {
+        static_assert(2 * TILE >= 128 * ROWB, "the key tiles' place holds the rows (their last reads are behind the last barrier)");
+        const int first = row - (lane & 31);
+        store_rows<T, D>(lds_k[0] + wave * 32 * ROWB, run.o, inverse_sum(l), lane, [&](int r) -> void* {
+            if (first + r >= rows) return nullptr;
+            const RowPlace p = row_place(first + r, rows, group, g, q0);
+            return (T*)a.out.p + p.q * a.out.row + p.head * a.out.head;
+        });
+    }
 }
 
 // A wave's own stretch of keys: operands straight from memory, values through an LDS image of its own.
+// One row against 400003 keys, 4 heads of 64: 410 MB in 87 us, 4.7 TB/s (a copy reaches 5.1).
 template <class T, int D, int BN> struct OwnKeys {
     using S = Shape<T, D>;
     static constexpr int SUB = BN / 32, VC = BN * S::CPR / 64, ROWB = D * (int)sizeof(T);
@@ -635,8 +634,10 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
     for (int i = t0 + tid; i < end; i += 1024) tile[i] = make_int4(-1, 0, 0, 0);
 }
 
+// Bound by memory: 8 streams of 1024 rows, 16 of 1025 blocks of 64 keys each, 4 heads of 64: 547 MB of inputs and results and 150 MB of
+// parts, written and read, in 160 us for the three kernels (13 turning the lists, 125 here, 18 joining).
 // A wave per tile: one block's keys against 32 rows out of the queries that name it.  32 keys at a time: fewer registers, so that
-// three waves of a SIMD have loads in flight (64 at a time: 15 us more for 8 streams).
+// three waves of a SIMD have loads in flight (64 at a time: 15 us more for 8 streams; two waves sharing a block: 10 % more).
 template <class T, int D>
 __global__ __launch_bounds__(64, IsF32<T>::v && D == 128 ? 1 : 2) void attention_blocks_kernel(AttentionLaunch a, AttnSets sets, BinWork w) {
     using S = Shape<T, D>;
@@ -683,10 +684,7 @@ __global__ __launch_bounds__(64, IsF32<T>::v && D == 128 ? 1 : 2) void attention
     P* to = row < t.z ? (P*)a.work + (((q - sets.q_off[0]) * a.q.heads + head) * a.n_sel + slot) : nullptr;
     if constexpr (!__is_same(T, __bf16)) {
         if (!to) return;   // (both lane halves of a row leave together)
-#pragma unroll
-        for (int u = 0; u < D / 32; u++)
-#pragma unroll
-            for (int b = 0; b < 4; b++) *(f32x4*)&to->o[u * 32 + 8 * b + 4 * h] = f32x4{run.o[u][4 * b], run.o[u][4 * b + 1], run.o[u][4 * b + 2], run.o[u][4 * b + 3]};
+        store_row<D>(to->o, run.o, 1.f, h);
         if (h == 0) {
             to->m = run.m;
             to->l = l;

@@ -519,9 +519,12 @@ struct BinWork {
     int4* tile;    // (block, first entry in the region's list, rows of the block = entries * group, first row of the tile); block -1: unused
 };
 // A region's blocks are counted by one work-group, or in kBinShares equal shares by as many where the entries are more than the
-// blocks.
+// blocks (region_tiles() then has room for every block's last tile) and every share has blocks (what a share without any would
+// have to know, the entries before it, it does not count).
 constexpr int kBinShares = 4;
-__host__ __device__ inline int bin_shares(long long nq, int n_sel, int blocks) { return nq * n_sel >= 2048 && nq * n_sel >= blocks ? kBinShares : 1; }
+__host__ __device__ inline int bin_shares(long long nq, int n_sel, int blocks) {
+    return nq * n_sel >= 2048 && nq * n_sel >= blocks && blocks >= 4 * kBinShares ? kBinShares : 1;
+}
 // tiles that a region may need: its rows in 32s, and one more for every block's last
 __host__ __device__ inline int region_tiles(long long nq, int n_sel, int group, int blocks) {
     const long long e = nq * n_sel;

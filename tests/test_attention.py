@@ -540,6 +540,9 @@ BLOCK_SHAPES = [
     (64, 4, 4, 64, 16, [1], [5000], 0.0), (64, 4, 4, 64, 1, [3], [10], 0.0), (32, 8, 2, 32, 7, [5, 0, 3], [300, 40, 0], 0.1), (128, 2, 2, 128, 33, [17], [9000], 0.05),
     (64, 4, 4, 64, 16, [300, 211], [3000, 65], 0.05), (64, 8, 1, 32, 5, [90], [640], 0.5), (128, 4, 2, 64, 64, [33], [4100], 0.0), (32, 2, 2, 128, 3, [400], [1000], 0.0),
     (64, 3, 1, 64, 4, [50], [700], 1.0), (64, 32, 2, 64, 4, [70], [1000], 0.1), (64, 4, 4, 64, 16, [700], [8000], 0.0),
+    # many entries on one to five blocks, groups of more than 32 heads, more entries and more blocks than a work-group holds at a time
+    (64, 4, 4, 128, 5, [1000, 999, 998, 997, 996], [30, 200, 300, 500, 640], 0.05), (32, 40, 1, 128, 16, [260], [5000], 0.0), (32, 40, 1, 64, 3, [3], [500], 0.1),
+    (64, 1, 1, 64, 16, [1100], [5000], 0.05), (128, 1, 1, 32, 16, [300], [300000], 0.0),
 ]
 
 

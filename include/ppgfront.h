@@ -352,7 +352,10 @@ int ppg_extend_map_matches(ppg_ctx* ctx, float nnratio, float th, const ppg_mapg
  * With more query heads than key heads, group = heads / kv_heads consecutive query heads share a key head.
  * An output shares no component with an input, except where that is said.
  * stream: as in ppg_match_nn_noalloc (NULL: the context's own stream, and the call returns when the results are in place;
- * else a hipStream_t to enqueue on without waiting); PPG_STREAM_DEFAULT is HIP's default stream. */
+ * what wrote the inputs on another stream must have finished by then; else a hipStream_t to enqueue on without waiting);
+ * PPG_STREAM_DEFAULT is HIP's default stream.
+ * Rows times heads (times n_sel, for lists) stay below 2^31 - 2^10 (attention over lists: 2^30), and the kernels' launches below
+ * 2^32 threads (for instance 2^28 rows to turn, 2^24 blocks to average); PPG_ECAP beyond. */
 #define PPG_STREAM_DEFAULT ((void*)1)
 #define PPG_F32 0
 #define PPG_BF16 1
@@ -429,7 +432,7 @@ int ppg_block_select(ppg_ctx* ctx, const ppg_block_select_args* args, void* stre
  * ppg_block_select writes them; numbers that name no block of the set are passed over, and a block listed twice counts
  * twice.  A row with nothing to attend to (or whose products are all -inf) gives 0, and -inf in lse.
  * lse (optional, [rows of q][heads]): log sum_j exp(scale * q . k_j).
- * Products and sums are held in 32 bits; with 16-bit inputs the softmax's weights are rounded to that type before they
+ * Products and sums are held in 32 bits, the sums undivided: |v| times the number of keys stays below 2^120.  With 16-bit inputs the softmax's weights are rounded to that type before they
  * meet the values, as the inputs of the matrix unit are. */
 typedef struct ppg_attention_args {
     int dtype, head_dim;

@@ -7,6 +7,9 @@
 
 namespace ppg {
 
+// HIP counts the threads of a launch in 32 bits
+inline bool launch_fits(long long groups, int threads) { return groups * threads < (1LL << 32); }
+
 // The sets of a call travel with the launch (kernel arguments): no copy to the device, nothing that a later call could
 // overwrite, and a captured graph keeps its own.
 struct AttnSets {
@@ -23,6 +26,7 @@ struct RotaryLaunch {
     const double* freq;
     ppg_rows src[2], dst[2];
 };
+bool rotary_fits(const RotaryLaunch& a);   // one launch holds it (likewise below)
 hipError_t launch_rotary(int dtype, const RotaryLaunch& a, hipStream_t s);
 
 struct BlockMeansLaunch {
@@ -32,6 +36,7 @@ struct BlockMeansLaunch {
     float* mean;
     int32_t* count;
 };
+bool block_means_fits(const AttnSets& sets);
 hipError_t launch_block_means(int dtype, int head_dim, const BlockMeansLaunch& a, AttnSets& sets, hipStream_t s);
 
 struct BlockSelectLaunch {
@@ -41,6 +46,7 @@ struct BlockSelectLaunch {
     const int32_t* count;
     int32_t* sel;
 };
+bool block_select_fits(const BlockSelectLaunch& a, AttnSets& sets);
 hipError_t launch_block_select(int dtype, int head_dim, const BlockSelectLaunch& a, AttnSets& sets, hipStream_t s);
 
 struct AttentionLaunch {
@@ -52,6 +58,7 @@ struct AttentionLaunch {
     const int32_t* sel;
     void* work;
 };
+constexpr size_t kNoWork = ~(size_t)0;   // "one launch does not hold it"
 size_t attention_work(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets);
 hipError_t launch_attention(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets, hipStream_t s);
 

@@ -590,6 +590,7 @@ __global__ __launch_bounds__(1024, 4) void block_select_kernel(BlockSelectLaunch
         else { constexpr int D = 128; CALL; }                 \
     } while (0)
 
+bool rotary_fits(const RotaryLaunch& a) { return launch_fits(((long long)a.n_rows[0] + 15) / 16 + ((long long)a.n_rows[1] + 15) / 16, 256); }
 hipError_t launch_rotary(int dtype, const RotaryLaunch& a, hipStream_t s) {
     const long long rows = (long long)a.n_rows[0] + a.n_rows[1];
     if (!rows) return hipSuccess;
@@ -613,6 +614,7 @@ hipError_t launch_rotary(int dtype, const RotaryLaunch& a, hipStream_t s) {
     return e;
 }
 
+bool block_means_fits(const AttnSets& sets) { return launch_fits(sets.blk[sets.n], 256); }
 hipError_t launch_block_means(int dtype, int head_dim, const BlockMeansLaunch& a, AttnSets& sets, hipStream_t s) {
     const int nb = sets.blk[sets.n];
     if (!nb) return hipSuccess;
@@ -620,20 +622,21 @@ hipError_t launch_block_means(int dtype, int head_dim, const BlockMeansLaunch& a
     return hipGetLastError();
 }
 
+static int select_tiles(const BlockSelectLaunch& a, AttnSets& sets, int rows) {
+    sets.tile[0] = 0;
+    for (int i = 0; i < sets.n; i++)
+        sets.tile[i + 1] = sets.tile[i] + (int)(((long long)sets.q_off[i + 1] - sets.q_off[i] + rows - 1) / rows * a.kv_heads);
+    return sets.tile[sets.n];
+}
+bool block_select_fits(const BlockSelectLaunch& a, AttnSets& sets) { return launch_fits(xcd_grid(select_tiles(a, sets, 32)), 1024); }
 hipError_t launch_block_select(int dtype, int head_dim, const BlockSelectLaunch& a, AttnSets& sets, hipStream_t s) {
-    auto tiles = [&](int rows) {
-        sets.tile[0] = 0;
-        for (int i = 0; i < sets.n; i++)
-            sets.tile[i + 1] = sets.tile[i] + (int)(((long long)sets.q_off[i + 1] - sets.q_off[i] + rows - 1) / rows * a.kv_heads);
-        return sets.tile[sets.n];
-    };
     int most = 0;
     for (int i = 0; i < sets.n; i++) most = std::max(most, sets.blk[i + 1] - sets.blk[i]);
     // a row per wave where that still leaves CUs without work (one frame of 500 rows, 4 heads, 313 blocks: 13 us, 23 us with two), else two, which read
     // the means half as often (8 streams of 1024 rows: 107 us, 149 us with one); few blocks: as many registers as those take
 #define SELECT(ROWS, PER) BY_TYPE(dtype, BY_DIM(head_dim, (block_select_kernel<T, D, ROWS, PER><<<xcd_grid(sets.tile[sets.n]), 1024, 0, s>>>(a, sets))))
-    if (tiles(32) >= 256) SELECT(32, 17);
-    else if (!tiles(16)) return hipSuccess;
+    if (select_tiles(a, sets, 32) >= 256) SELECT(32, 17);
+    else if (!select_tiles(a, sets, 16)) return hipSuccess;
     else if (most <= 5 * 64) SELECT(16, 5);
     else SELECT(16, 17);
 #undef SELECT

@@ -835,9 +835,14 @@ template <class T> hipError_t run_dim(const AttentionLaunch& a, AttnSets& sets, 
 size_t attention_work(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets) {
     if (a.n_sel) {
         const BlocksPlan p = blocks_plan(dtype, head_dim, a, sets);
+        // (a list's sums are joined by head_dim / 4 threads or half as many; what is not turned round is small)
+        const long long n = ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads;
+        if (p.binned && !(launch_fits(sets.tile[sets.n], 64) && launch_fits((long long)sets.n * a.k.heads * kBinShares, 1024) && launch_fits(n, head_dim / 4)))
+            return kNoWork;
         return p.part_bytes + p.list_bytes + p.tile_bytes;
     }
     const DensePlan p = dense_plan(dtype, head_dim, a, sets);
+    if (!launch_fits(xcd_grid(sets.tile[sets.n] * p.parts), 256)) return kNoWork;
     return p.parts == 1 ? 0 : ((size_t)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads * p.parts * (head_dim + 4) * sizeof(float);
 }
 hipError_t launch_attention(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets, hipStream_t s) {

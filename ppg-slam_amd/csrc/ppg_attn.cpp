@@ -31,8 +31,9 @@ const char* rows_fault(const ppg_rows& r, int dtype, int head_dim, long long n_r
     if (r.row < 0 || r.head < 0 || r.row > (1LL << 40) || r.head > (1LL << 40)) return "stride is negative or beyond 2^40";
     if (r.row * e % 16 || r.head * e % 16) return "a stride is not a multiple of 16 bytes";
     if (output && n_rows > 0) {
-        const bool rows_outer = (r.heads == 1 || r.head >= head_dim) && (n_rows == 1 || r.row >= (r.heads - 1) * r.head + head_dim);
-        const bool heads_outer = (n_rows == 1 || r.row >= head_dim) && (r.heads == 1 || r.head >= (n_rows - 1) * r.row + head_dim);
+        const __int128 row = r.row, head = r.head;
+        const bool rows_outer = (r.heads == 1 || head >= head_dim) && (n_rows == 1 || row >= (r.heads - 1) * head + head_dim);
+        const bool heads_outer = (n_rows == 1 || row >= head_dim) && (r.heads == 1 || head >= (n_rows - 1) * row + head_dim);
         if (!rows_outer && !heads_outer) return "strides of an output make its vectors overlap";
     }
     return nullptr;
@@ -62,6 +63,9 @@ void block_offsets(ppg::AttnSets& s, int block) {
     s.blk[0] = 0;
     for (int i = 0; i < s.n; i++) s.blk[i + 1] = s.blk[i] + (int)(((long long)s.k_off[i + 1] - s.k_off[i] + block - 1) / block);
 }
+
+// what the kernels' launches cannot count
+int too_large(ppg_ctx* c, const char* who) { return fail(c, PPG_ECAP, "%s: more rows or blocks than one launch holds (2^32 threads)", who); }
 
 hipStream_t stream_of(ppg_ctx* c, void* stream) { return stream == PPG_STREAM_DEFAULT ? nullptr : stream ? (hipStream_t)stream : c->post; }
 int finish(ppg_ctx* c, const char* who, hipError_t e, void* stream) {
@@ -176,6 +180,7 @@ int ppg_rotary(ppg_ctx* c, const ppg_rotary_args* a, void* stream) {
         if (a->src[i].p == a->dst[i].p && (a->src[i].row != a->dst[i].row || a->src[i].head != a->dst[i].head))
             return fail(c, PPG_EINVAL, "%s: dst[%d] is src[%d] with other strides", who, i, i);
     }
+    if (!ppg::rotary_fits(l)) return too_large(c, who);
     if (!c) return fail(c, PPG_EINVAL, "%s: ctx is NULL", who);
     DeviceScope dev(c->cfg.device_id);
     HIPCHK(c, dev.err);
@@ -200,6 +205,7 @@ int ppg_block_means(ppg_ctx* c, const ppg_block_means_args* a, void* stream) {
     if ((uintptr_t)a->mean % 16 || (uintptr_t)a->count % 4) return fail(c, PPG_EINVAL, "%s: mean is not at a multiple of 16, or count of 4", who);
     if (nk * a->k.heads >= kMostVectors) return fail(c, PPG_ECAP, "%s: rows times heads must stay below 2^31 - 2^10", who);
     block_offsets(sets, a->block);
+    if (!ppg::block_means_fits(sets)) return too_large(c, who);
     ppg::BlockMeansLaunch l;
     l.block = a->block; l.k = a->k; l.skip = a->skip; l.mean = a->mean; l.count = a->count;
     if (!c) return fail(c, PPG_EINVAL, "%s: ctx is NULL", who);
@@ -234,6 +240,7 @@ int ppg_block_select(ppg_ctx* c, const ppg_block_select_args* a, void* stream) {
     block_offsets(sets, a->block);
     ppg::BlockSelectLaunch l;
     l.block = a->block; l.kv_heads = a->kv_heads; l.n_sel = a->n_sel; l.q = a->q; l.mean = a->mean; l.count = a->count; l.sel = a->sel;
+    if (!ppg::block_select_fits(l, sets)) return too_large(c, who);
     if (!c) return fail(c, PPG_EINVAL, "%s: ctx is NULL", who);
     DeviceScope dev(c->cfg.device_id);
     HIPCHK(c, dev.err);
@@ -244,7 +251,8 @@ size_t ppg_attention_work(const ppg_attention_args* a) {
     ppg::AttentionLaunch l;
     ppg::AttnSets sets;
     if (!a || !a->q_off || !a->k_off || attention_checked(nullptr, a, true, l, sets)) return 0;
-    return ppg::attention_work(a->dtype, a->head_dim, l, sets);
+    const size_t need = ppg::attention_work(a->dtype, a->head_dim, l, sets);
+    return need == ppg::kNoWork ? 0 : need;
 }
 
 int ppg_attention(ppg_ctx* c, const ppg_attention_args* a, void* stream) {
@@ -253,6 +261,7 @@ int ppg_attention(ppg_ctx* c, const ppg_attention_args* a, void* stream) {
     const int rc = attention_checked(c, a, false, l, sets);
     if (rc) return rc;
     const size_t need = ppg::attention_work(a->dtype, a->head_dim, l, sets);
+    if (need == ppg::kNoWork) return too_large(c, "ppg_attention");
     if (need && (!a->work || a->work_bytes < need || (uintptr_t)a->work % 256))
         return fail(c, PPG_EINVAL, "ppg_attention: work must be %zu bytes (ppg_attention_work), 256-byte aligned", need);
     if (!c) return fail(c, PPG_EINVAL, "ppg_attention: ctx is NULL");

@@ -130,6 +130,24 @@ def test_block_select_refuses(pkg, change, code, word):
     assert rc == getattr(pkg, code) and word in why, why
 
 
+def test_what_one_launch_cannot_count_is_refused(pkg):
+    """2^32 threads or more, and strides whose products pass 64 bits."""
+    wide = dict(heads=65535, row=65535 * 64, head=64)
+    cases = [("ppg_rotary", pkg.rotary_args(dtype=pkg.BF16, head_dim=64, rot_dim=64, layout=0, n_axes=1, freq=4096, n_rows=(1 << 28,), pos=(4096,), src=(_rows(pkg, heads=1),), dst=(_rows(pkg, heads=1, p=8192),))),
+             ("ppg_block_means", pkg.block_means_args(dtype=pkg.F32, head_dim=64, block=32, k_off=pkg.offsets([0, 1 << 29]), k=_rows(pkg), mean=4096, count=4096)),
+             ("ppg_block_select", pkg.block_select_args(dtype=pkg.F32, head_dim=64, block=64, q_off=pkg.offsets([0, 1 << 27]), k_off=pkg.offsets([0, 9]), q=_rows(pkg, heads=1),
+                                                       kv_heads=1, mean=4096, count=4096, n_sel=4, sel=4096)),
+             ("ppg_attention", _attention(pkg, q_off=pkg.offsets([0] + [32640 + i for i in range(128)]), k_off=pkg.offsets([0] * 129), **{x: _rows(pkg, **wide) for x in ("q", "k", "v", "out")})),
+             ("ppg_attention", _attention(pkg, q_off=pkg.offsets([0, 1 << 27]), block=64, n_sel=3, sel=4096))]
+    for call, args in cases:
+        rc, why = _refusal(pkg, call, args)
+        assert rc == pkg.PPG_ECAP and "one launch" in why, (call, rc, why)
+    assert pkg.lib().ppg_attention_work(cases[-1][1]) == 0 and pkg.lib().ppg_attention_work(cases[-2][1]) == 0
+    # (2^23 rows at the rows' own distance would be 2^63 components away: the heads are not that far apart)
+    rc, why = _refusal(pkg, "ppg_attention", _attention(pkg, q_off=pkg.offsets([0, 1 << 23]), out=_rows(pkg, row=1 << 40, head=1 << 40)))
+    assert rc == pkg.PPG_EINVAL and "overlap" in why, (rc, why)
+
+
 def test_rotary_frequencies(pkg):
     n, base = 32, 10000.0
     plain = pkg.rotary_frequencies(n, base)

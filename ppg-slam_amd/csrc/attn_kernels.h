@@ -12,12 +12,23 @@ inline bool launch_fits(long long groups, int threads) { return groups * threads
 
 // The sets of a call travel with the launch (kernel arguments): no copy to the device, nothing that a later call could
 // overwrite, and a captured graph keeps its own.
+// What a work-group reads of them comes one round trip to memory after the other, so these are kept few: the number of units
+// stands in front, the lists that are searched end in INT_MAX, and what one set alone has is always at the same place.
 struct AttnSets {
     int n;
+    int units;   // tile[n]
     int q_off[PPG_ATTN_MAX_SETS + 1], k_off[PPG_ATTN_MAX_SETS + 1];
     int tile[PPG_ATTN_MAX_SETS + 1];   // first work-group tile of a set (what a tile is depends on the kernel)
     int blk[PPG_ATTN_MAX_SETS + 1];    // first key block of a set
 };
+// INT_MAX behind the last set
+inline void end_list(const AttnSets& sets, int (&list)[PPG_ATTN_MAX_SETS + 1]) {
+    for (int i = sets.n + 1; i <= PPG_ATTN_MAX_SETS; i++) list[i] = 0x7fffffff;
+}
+inline int end_tiles(AttnSets& sets) {
+    end_list(sets, sets.tile);
+    return sets.units = sets.tile[sets.n];
+}
 
 struct RotaryLaunch {
     int head_dim, rot_dim, layout, inverse, n_axes;

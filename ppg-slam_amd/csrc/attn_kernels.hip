@@ -134,8 +134,9 @@ __global__ __launch_bounds__(256) void block_means_kernel(BlockMeansLaunch a, At
     __shared__ double part[256][N];
     __shared__ unsigned char keep[128];
     __shared__ int kept[2];
-    const int b = blockIdx.x, s = find_set(sets.blk, sets.n, b), tid = threadIdx.x;
-    const int first = sets.k_off[s] + (b - sets.blk[s]) * a.block, n = min(a.block, sets.k_off[s + 1] - first);
+    const int b = blockIdx.x, tid = threadIdx.x;
+    const SetHere set = set_of(sets_here(sets), sets, sets.blk, b, tid & 63);
+    const int at = (b - set.blk0) * a.block, first = set.k0 + at, n = min(a.block, set.nk - at);
     if (tid < 128) {
         const bool on = tid < n && !(a.skip && a.skip[first + tid]);
         keep[tid] = on;
@@ -292,17 +293,19 @@ __global__ __launch_bounds__(1024, 4) void block_select_kernel(BlockSelectLaunch
     constexpr int CHUNK = PER * 64, RPW = ROWS / kSelWaves, N = 16 / (int)sizeof(T);
     constexpr int LPC = D / 16, CPP = 64 / LPC;   // lanes that share a candidate's product, candidates of a pass
     __shared__ alignas(16) SelectLds<D, ROWS, PER> lds;
-    const int unit = xcd_unit(blockIdx.x, sets.tile[sets.n]);
-    if (unit >= sets.tile[sets.n]) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, s = find_set_wave(sets.tile, sets.n, unit, lane);
-    const int q0 = sets.q_off[s], nq = sets.q_off[s + 1] - q0;
+    const SetsHere here = sets_here(sets);
+    const int unit = xcd_unit(blockIdx.x, here.units);
+    if (unit >= here.units) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const SetHere set = set_of(here, sets, sets.tile, unit, lane);
+    const int q0 = set.q0, nq = set.nq;
     // the heads in turn: work-groups that run at the same time then read whole rows of means between them, and with those all
     // channels of the L2
-    const int g = (unit - sets.tile[s]) % a.kv_heads, row0 = ((unit - sets.tile[s]) / a.kv_heads) * ROWS;
-    const int group = a.q.heads / a.kv_heads, nb = sets.blk[s + 1] - sets.blk[s];
-    const float* mean = a.mean + ((long long)sets.blk[s] * a.kv_heads + g) * D;
+    const int g = (unit - set.tile0) % a.kv_heads, row0 = ((unit - set.tile0) / a.kv_heads) * ROWS;
+    const int group = a.q.heads / a.kv_heads, nb = set.blocks;
+    const float* mean = a.mean + ((long long)set.blk0 * a.kv_heads + g) * D;
     const long long stride = (long long)a.kv_heads * D;
-    const int* count = a.count + sets.blk[s];
+    const int* count = a.count + set.blk0;
     auto query = [&](int row, int h) { return (const T*)a.q.p + (long long)(q0 + min(row, nq - 1)) * a.q.row + ((long long)g * group + h) * a.q.head; };
     auto q_chunk = [&](int half, int r, int ch) { return lds.q[half] + r * (D * 2) + ((ch ^ (r & (D >= 64 ? 7 : 3))) << 4); };
 
@@ -626,7 +629,7 @@ static int select_tiles(const BlockSelectLaunch& a, AttnSets& sets, int rows) {
     sets.tile[0] = 0;
     for (int i = 0; i < sets.n; i++)
         sets.tile[i + 1] = sets.tile[i] + (int)(((long long)sets.q_off[i + 1] - sets.q_off[i] + rows - 1) / rows * a.kv_heads);
-    return sets.tile[sets.n];
+    return end_tiles(sets);
 }
 bool block_select_fits(const BlockSelectLaunch& a, AttnSets& sets) { return launch_fits(xcd_grid(select_tiles(a, sets, 32)), 1024); }
 hipError_t launch_block_select(int dtype, int head_dim, const BlockSelectLaunch& a, AttnSets& sets, hipStream_t s) {
@@ -634,7 +637,7 @@ hipError_t launch_block_select(int dtype, int head_dim, const BlockSelectLaunch&
     for (int i = 0; i < sets.n; i++) most = std::max(most, sets.blk[i + 1] - sets.blk[i]);
     // a row per wave where that still leaves CUs without work (one frame of 500 rows, 4 heads, 313 blocks: 13 us, 23 us with two), else two, which read
     // the means half as often (8 streams of 1024 rows: 107 us, 149 us with one); few blocks: as many registers as those take
-#define SELECT(ROWS, PER) BY_TYPE(dtype, BY_DIM(head_dim, (block_select_kernel<T, D, ROWS, PER><<<xcd_grid(sets.tile[sets.n]), 1024, 0, s>>>(a, sets))))
+#define SELECT(ROWS, PER) BY_TYPE(dtype, BY_DIM(head_dim, (block_select_kernel<T, D, ROWS, PER><<<xcd_grid(sets.units), 1024, 0, s>>>(a, sets))))
     if (select_tiles(a, sets, 32) >= 256) SELECT(32, 17);
     else if (!select_tiles(a, sets, 16)) return hipSuccess;
     else if (most <= 5 * 64) SELECT(16, 5);

@@ -100,16 +100,17 @@ __global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) 
     static_assert(BN * S::CPR % 256 == 0, "tile loads are whole rounds of the work-group");
     __shared__ alignas(16) char lds_k[2][TILE], lds_v[2][TILE];
     __shared__ unsigned long long lds_dead[kWindow];
-    const int units = sets.tile[sets.n] * parts, whole = xcd_unit(blockIdx.x, units);
+    const SetsHere here = sets_here(sets);
+    const int units = here.units * parts, whole = xcd_unit(blockIdx.x, units);
     if (whole >= units) return;
     const int unit = parts == 1 ? whole : whole / parts, part = parts == 1 ? 0 : whole % parts;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    const int s = find_set_wave(sets.tile, sets.n, unit, lane);
-    const int q0 = sets.q_off[s], k0 = sets.k_off[s], nk = sets.k_off[s + 1] - k0, kvh = a.k.heads, group = a.q.heads / kvh;
-    const int rows = (sets.q_off[s + 1] - q0) * group, tiles = (rows + 127) / 128;
-    const int g = (unit - sets.tile[s]) / tiles, row = ((unit - sets.tile[s]) % tiles) * 128 + wave * 32 + (lane & 31);
+    const SetHere set = set_of(here, sets, sets.tile, unit, lane);
+    const int q0 = set.q0, k0 = set.k0, nk = set.nk, kvh = a.k.heads, group = a.q.heads / kvh;
+    const int rows = set.nq * group, tiles = (rows + 127) / 128;
+    const int g = (unit - set.tile0) / tiles, row = ((unit - set.tile0) % tiles) * 128 + wave * 32 + (lane & 31);
     const float c = a.scale * kLog2e, slack = rise_slack(c);
-    const int all = (nk + BN - 1) / BN, from = (int)((long long)all * part / parts), to = (int)((long long)all * (part + 1) / parts);
+    const int all = (nk + BN - 1) / BN, from = share_begin(all, part, parts), to = share_begin(all, part + 1, parts);
 
     // tile loads: thread -> (row, chunk) and STEP rows on
     const int r0 = tid / S::CPR, ch0 = tid % S::CPR;
@@ -288,43 +289,32 @@ template <class T, int D, int BN> struct OwnKeys {
     }
 };
 
-// The sums of the four waves of a work-group meet in LDS: [row][D] components and (m, l) per row, from wave 0 upwards.
-template <class T, int D> struct Meeting {
-    float o[32][D + 4];   // + 4: the 32 rows that a 16-byte access takes start in different banks
-    float m[32], l[32];
+// The sums of the four waves of a work-group meet in LDS; who stores a row's components adds them up, from wave 0 upwards.
+template <int D> struct Meeting {
+    float o[4][32][D + 4];   // + 4: the 32 rows that a 16-byte access takes start in different banks
+    float m[4][32], l[4][32];
 };
-template <class T, int D> __device__ __forceinline__ void meet(Meeting<T, D>& x, Running<T, D>& run, float c, int wave, int waves, int lane) {
+template <class T, int D> __device__ __forceinline__ void to_meeting(Meeting<D>& x, const Running<T, D>& run, int wave, int lane) {
     const int h = lane >> 5, col = lane & 31;
-    run.l = run.sum();
-    for (int w = 0; w < waves; w++) {
-        if (w == wave) {
-            float keep = 0.f, add = 1.f, l = run.l, m = run.m;
-            if (w) {
-                const float m0 = x.m[col];
-                m = fmaxf(m0, run.m);
-                keep = m0 == m ? 1.f : __builtin_amdgcn_exp2f((m0 - m) * c);
-                add = run.m == m ? 1.f : __builtin_amdgcn_exp2f((run.m - m) * c);
-                l = x.l[col] * keep + run.l * add;
-            }
-#pragma unroll
-            for (int t = 0; t < D / 32; t++)
-#pragma unroll
-                for (int b = 0; b < 4; b++) {
-                    f32x4* at = (f32x4*)&x.o[col][t * 32 + 8 * b + 4 * h];
-                    f32x4 y = {run.o[t][4 * b], run.o[t][4 * b + 1], run.o[t][4 * b + 2], run.o[t][4 * b + 3]};
-                    y *= add;
-                    if (w) y += *at * keep;
-                    *at = y;
-                }
-            // both halves of the wave have read m and l of the column before either writes them (one wave, in order)
-            __builtin_amdgcn_wave_barrier();
-            if (h == 0) {
-                x.m[col] = m;
-                x.l[col] = l;
-            }
-        }
-        __syncthreads();
+    store_row<D>(x.o[wave][col], run.o, 1.f, h);
+    const float l = run.sum();
+    if (h == 0) {
+        x.m[wave][col] = run.m;
+        x.l[wave][col] = l;
     }
+}
+// components d .. d + 3 of row r, its m and l
+template <int D> __device__ __forceinline__ f32x4 of_meeting(const Meeting<D>& x, int r, int d, float c, float& m, float& l) {
+    m = fmaxf(fmaxf(x.m[0][r], x.m[1][r]), fmaxf(x.m[2][r], x.m[3][r]));
+    l = 0.f;
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        const float f = x.m[w][r] == m ? 1.f : __builtin_amdgcn_exp2f((x.m[w][r] - m) * c);
+        l += x.l[w][r] * f;
+        y += *(const f32x4*)&x.o[w][r][d] * f;
+    }
+    return y;
 }
 
 // The same for a selected block of a query with bf16: the mean of the values (o / l) in fp16, times a power of two that brings the
@@ -344,17 +334,18 @@ __global__ __launch_bounds__(256, IsF32<T>::v && D == 128 ? 1 : 2) void attentio
     constexpr int SUB = BN / 32, IMG = BN * D * (int)sizeof(T);
     __shared__ alignas(16) union {
         char v[4][IMG];
-        Meeting<T, D> sums;
+        Meeting<D> sums;
     } lds;
-    const int units = sets.tile[sets.n] * parts, unit = xcd_unit(blockIdx.x, units);
+    const SetsHere here = sets_here(sets);
+    const int units = here.units * parts, unit = xcd_unit(blockIdx.x, units);
     if (unit >= units) return;
     const int part = unit % parts, tile = unit / parts;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const int s = find_set_wave(sets.tile, sets.n, tile, lane);
-    const int q0 = sets.q_off[s], k0 = sets.k_off[s], nk = sets.k_off[s + 1] - k0, kvh = a.k.heads, group = a.q.heads / kvh;
+    const SetHere set = set_of(here, sets, sets.tile, tile, lane);
+    const int q0 = set.q0, k0 = set.k0, nk = set.nk, kvh = a.k.heads, group = a.q.heads / kvh;
     // SEL: tiles of a query's group never hold rows of another query
-    const int nq = sets.q_off[s + 1] - q0, all = nq * group, per_q = (group + 31) / 32, tiles = SEL ? nq * per_q : (all + 31) / 32;
-    const int g = (tile - sets.tile[s]) / tiles, at = (tile - sets.tile[s]) % tiles;
+    const int nq = set.nq, all = nq * group, per_q = (group + 31) / 32, tiles = SEL ? nq * per_q : (all + 31) / 32;
+    const int g = (tile - set.tile0) / tiles, at = (tile - set.tile0) % tiles;
     const int row0 = SEL ? at / per_q * group + at % per_q * 32 : at * 32;
     const int rows = SEL ? (at / per_q + 1) * group : all;
     u32x4 qf[S::NF];
@@ -366,13 +357,13 @@ __global__ __launch_bounds__(256, IsF32<T>::v && D == 128 ? 1 : 2) void attentio
     const T* vp = (const T*)a.v.p + g * a.v.head + (long long)k0 * a.v.row;
     const uint8_t* skip = a.skip ? a.skip + k0 : nullptr;
     const int* sel = SEL ? a.sel + ((long long)(q0 + at / per_q) * kvh + g) * a.n_sel : nullptr;
-    const int per_block = SEL ? (a.block + BN - 1) / BN : 1, blocks = SEL ? (nk + a.block - 1) / a.block : 0;
-    const long long nt = SEL ? (nk ? (long long)a.n_sel * per_block : 0) : (nk + BN - 1) / BN;
-    const int from = (int)(nt * part / parts), to = (int)(nt * (part + 1) / parts);
+    const int per_shift = SEL && a.block > BN ? __builtin_ctz((unsigned)a.block / BN) : 0, blocks = SEL ? (nk + a.block - 1) / a.block : 0;
+    const int nt = SEL ? (nk ? a.n_sel << per_shift : 0) : (int)(((unsigned)nk + BN - 1) / BN);
+    const int from = share_begin(nt, part, parts), to = share_begin(nt, part + 1, parts);
     OwnKeys<T, D, BN> keys;
     auto load = [&](int t) {
         if constexpr (SEL) {
-            const int b = sel[t / per_block], j = t % per_block * BN;
+            const int b = sel[t >> per_shift], j = (t & ((1 << per_shift) - 1)) * BN;
             const bool ok = b >= 0 && b < blocks;
             const int first = ok ? b * a.block : 0, n = min(a.block, nk - first);
             keys.load(kp + first * a.k.row, vp + first * a.v.row, a.k.row, a.v.row, skip ? skip + first : nullptr, j, n, lane);
@@ -395,14 +386,15 @@ __global__ __launch_bounds__(256, IsF32<T>::v && D == 128 ? 1 : 2) void attentio
         __builtin_amdgcn_wave_barrier();
     }
     __syncthreads();
-    meet(lds.sums, run, c, wave, 4, lane);
+    to_meeting(lds.sums, run, wave, lane);
+    __syncthreads();
     // 32 rows x D components out, 4 per thread and round
     for (int i = threadIdx.x; i < 32 * (D / 4); i += 256) {
         const int r = i / (D / 4), d = (i % (D / 4)) * 4;
         if (row0 + r >= rows) continue;
-        const f32x4 y = *(const f32x4*)&lds.sums.o[r][d];
+        float m, l;
+        const f32x4 y = of_meeting(lds.sums, r, d, c, m, l);
         const RowPlace p = row_place(row0 + r, rows, group, g, q0);
-        const float m = lds.sums.m[r], l = lds.sums.l[r];
         if (parts > 1) {
             Part<D>& w = ((Part<D>*)a.work)[((p.q - sets.q_off[0]) * a.q.heads + p.head) * parts + part];
             *(f32x4*)&w.o[d] = y;
@@ -443,16 +435,22 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, 
     };
     __shared__ Sum met[PG > 1 ? 256 : 1];
     const int team = threadIdx.x / TEAM, sub = team % PG, d = threadIdx.x % TEAM * C;
-    const long long n = ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads, at = (long long)blockIdx.x * (TEAMS / PG) + team / PG;
-    const long long rh = min(at, n - 1);   // (a team behind the last does its work again and keeps it to itself)
+    const unsigned heads = a.q.heads, n = (unsigned)(sets.q_off[sets.n] - sets.q_off[0]) * heads, at = blockIdx.x * (TEAMS / PG) + team / PG;
+    const unsigned rh = min(at, n - 1);   // (a team behind the last does its work again and keeps it to itself)
     const float c = a.scale * kLog2e;
-    const P* w = (const P*)a.work + rh * parts;
-    const long long q = sets.q_off[0] + rh / a.q.heads;
-    const int head = (int)(rh % a.q.heads);
+    const P* w = (const P*)a.work + (long long)rh * parts;
+    const long long q = sets.q_off[0] + (int)(rh / heads);
+    const int head = (int)(rh % heads);
     int blocks = 0;
     const int* sel = nullptr;
     if constexpr (SEL) {
-        const int s = find_set(sets.q_off, sets.n, (int)q);
+        // the set of the work-group's first row, and on from there
+        int s = 0;
+        if (sets.n > 1) {
+            const unsigned first = min(blockIdx.x * (TEAMS / PG), n - 1);
+            s = find_set(sets.q_off, sets.q_off[0] + (int)(first / heads), threadIdx.x & 63);
+            while (q >= sets.q_off[s + 1]) s++;
+        }
         blocks = sets.blk[s + 1] - sets.blk[s];
         sel = a.sel + (q * a.k.heads + head / (a.q.heads / a.k.heads)) * a.n_sel;
     }
@@ -540,15 +538,17 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
     __shared__ int cnt[kBins];
     __shared__ int sum_e[16], sum_t[16], sum_b[16];
     const int kvh = a.k.heads, group = a.q.heads / kvh, s = blockIdx.x / kvh, g = blockIdx.x % kvh;
-    const int q0 = sets.q_off[s], nq = sets.q_off[s + 1] - q0, blocks = sets.blk[s + 1] - sets.blk[s], n = nq * a.n_sel;
+    const SetsHere here = sets_here(sets);
+    const SetHere set = here.n == 1 ? here.first : set_number(sets, s);
+    const int q0 = set.q0, nq = set.nq, blocks = set.blocks, n = nq * a.n_sel;
     const int* sel = a.sel + ((long long)q0 * kvh + g) * a.n_sel;
     const long long step = (long long)kvh * a.n_sel;
     int* list = w.list + ((long long)(q0 - sets.q_off[0]) * kvh + (long long)g * nq) * a.n_sel;
-    int4* tile = w.tile + sets.tile[s] + (long long)g * region_tiles(nq, a.n_sel, group, blocks);
+    int4* tile = w.tile + set.tile0 + (long long)g * region_tiles(nq, a.n_sel, group, blocks);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int shares = bin_shares(nq, a.n_sel, blocks), share = blockIdx.y;
     if (share >= shares) return;
-    const int lo = (int)((long long)blocks * share / shares), hi = (int)((long long)blocks * (share + 1) / shares);
+    const int lo = share_begin(blocks, share, shares), hi = share_begin(blocks, share + 1, shares);
     int e0 = 0, t0 = 0;   // where the entries and tiles of this round's bins go
     int held[kBinHold], rank[kBinHold];
     const bool once = n <= kBinHold * 1024;
@@ -649,11 +649,12 @@ __global__ __launch_bounds__(64, IsF32<T>::v && D == 128 ? 1 : 2) void attention
     const int lane = threadIdx.x, h = lane >> 5;
     // (in launch order: hardly two tiles read the same block, and a region's unused tiles would leave some XCDs without work)
     const int at = (int)blockIdx.x;
-    const int s = find_set_wave(sets.tile, sets.n, at, lane), kvh = a.k.heads, group = a.q.heads / kvh;
-    const int q0 = sets.q_off[s], nq = sets.q_off[s + 1] - q0, k0 = sets.k_off[s], nk = sets.k_off[s + 1] - k0;
-    const int cap = region_tiles(nq, a.n_sel, group, sets.blk[s + 1] - sets.blk[s]);
-    const int g = (at - sets.tile[s]) / cap;
     const int4 t = w.tile[at];
+    const SetsHere here = sets_here(sets);
+    const SetHere set = set_of(here, sets, sets.tile, at, lane);
+    const int q0 = set.q0, nq = set.nq, k0 = set.k0, nk = set.nk, kvh = a.k.heads, group = a.q.heads / kvh;
+    const int cap = region_tiles(nq, a.n_sel, group, set.blocks);
+    const int g = (at - set.tile0) / cap;
     if (t.x < 0) return;
     const int first = t.x * a.block, n = min(a.block, nk - first);
     const T* kp = (const T*)a.k.p + g * a.k.head + (long long)(k0 + first) * a.k.row;
@@ -726,7 +727,7 @@ int count_tiles(const AttentionLaunch& a, AttnSets& sets, int rows) {
     sets.tile[0] = 0;
     for (int s = 0; s < sets.n; s++)
         sets.tile[s + 1] = sets.tile[s] + (int)(((sets.q_off[s + 1] - (long long)sets.q_off[s]) * group + rows - 1) / rows * kvh);
-    return sets.tile[sets.n];
+    return end_tiles(sets);
 }
 DensePlan dense_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets) {
     const bool f32 = dtype == PPG_F32;
@@ -765,14 +766,16 @@ BlocksPlan blocks_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSe
         p.parts = a.n_sel;
         for (int s = 0; s < sets.n; s++)
             sets.tile[s + 1] = sets.tile[s] + (int)kvh * region_tiles(sets.q_off[s + 1] - sets.q_off[s], a.n_sel, (int)group, sets.blk[s + 1] - sets.blk[s]);
+        end_tiles(sets);
+        end_list(sets, sets.q_off);
         p.part_bytes = up256((size_t)nq * a.q.heads * a.n_sel * list_part);
         p.list_bytes = up256((size_t)nq * kvh * a.n_sel * sizeof(int));
-        p.tile_bytes = up256((size_t)sets.tile[sets.n] * sizeof(int4));
+        p.tile_bytes = up256((size_t)sets.units * sizeof(int4));
         return p;
     }
     const long long per_q = (group + 31) / 32;
     for (int s = 0; s < sets.n; s++) sets.tile[s + 1] = sets.tile[s] + (int)((sets.q_off[s + 1] - sets.q_off[s]) * per_q * kvh);
-    const int units = sets.tile[sets.n], bn = dtype == PPG_F32 || head_dim == 128 ? 32 : 64;
+    const int units = end_tiles(sets), bn = dtype == PPG_F32 || head_dim == 128 ? 32 : 64;
     const long long most = std::max(1LL, ((long long)a.n_sel * ((a.block + bn - 1) / bn) + 3) / 4);
     p.parts = units ? (int)std::min<long long>(most, std::max(1, kFill / units)) : 1;
     if (p.parts > 1) p.part_bytes = (size_t)nq * a.q.heads * p.parts * part;
@@ -796,33 +799,33 @@ template <class T, int D> hipError_t run(const AttentionLaunch& a, AttnSets& set
     hipError_t e;
     if (a.sel) {
         const BlocksPlan p = blocks_plan(dtype, D, a, sets);
-        if (!sets.tile[sets.n] && !p.binned) return hipSuccess;
+        if (!sets.units && !p.binned) return hipSuccess;
         if (!p.binned) {
-            attention_split_kernel<T, D, OWN_BN, true><<<xcd_grid(sets.tile[sets.n] * p.parts), 256, 0, s>>>(a, sets, p.parts);
+            attention_split_kernel<T, D, OWN_BN, true><<<xcd_grid(sets.units * p.parts), 256, 0, s>>>(a, sets, p.parts);
             e = hipGetLastError();
             return e != hipSuccess || p.parts == 1 ? e : join<T, D, false>(a, sets, p.parts, s);
         }
         BinWork w;
         w.list = (int*)((char*)a.work + p.part_bytes);
         w.tile = (int4*)((char*)w.list + p.list_bytes);
-        if (sets.tile[sets.n]) {
+        if (sets.units) {
             bin_kernel<<<dim3(sets.n * a.k.heads, kBinShares), 1024, 0, s>>>(a, sets, w);
             if ((e = hipGetLastError()) != hipSuccess) return e;
-            attention_blocks_kernel<T, D><<<(unsigned)sets.tile[sets.n], 64, 0, s>>>(a, sets, w);
+            attention_blocks_kernel<T, D><<<(unsigned)sets.units, 64, 0, s>>>(a, sets, w);
             if ((e = hipGetLastError()) != hipSuccess) return e;
         }
         return join<T, D, true>(a, sets, p.parts, s);
     }
     const DensePlan p = dense_plan(dtype, D, a, sets);
-    if (!sets.tile[sets.n]) return hipSuccess;
+    if (!sets.units) return hipSuccess;
     if (p.wide) {
-        const unsigned grid = xcd_grid(sets.tile[sets.n] * p.parts);
+        const unsigned grid = xcd_grid(sets.units * p.parts);
         if (a.lse || IsF32<T>::v) attention_wide_kernel<T, D, WIDE_BN, false><<<grid, 256, 0, s>>>(a, sets, p.parts);
         else attention_wide_kernel<T, D, WIDE_BN, !IsF32<T>::v><<<grid, 256, 0, s>>>(a, sets, p.parts);
         e = hipGetLastError();
         return e != hipSuccess || p.parts == 1 ? e : join<T, D, false>(a, sets, p.parts, s);
     }
-    attention_split_kernel<T, D, OWN_BN, false><<<xcd_grid(sets.tile[sets.n] * p.parts), 256, 0, s>>>(a, sets, p.parts);
+    attention_split_kernel<T, D, OWN_BN, false><<<xcd_grid(sets.units * p.parts), 256, 0, s>>>(a, sets, p.parts);
     e = hipGetLastError();
     return e != hipSuccess || p.parts == 1 ? e : join<T, D, false>(a, sets, p.parts, s);
 }
@@ -837,12 +840,12 @@ size_t attention_work(int dtype, int head_dim, const AttentionLaunch& a, AttnSet
         const BlocksPlan p = blocks_plan(dtype, head_dim, a, sets);
         // (a list's sums are joined by head_dim / 4 threads or half as many; what is not turned round is small)
         const long long n = ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads;
-        if (p.binned && !(launch_fits(sets.tile[sets.n], 64) && launch_fits((long long)sets.n * a.k.heads * kBinShares, 1024) && launch_fits(n, head_dim / 4)))
+        if (p.binned && !(launch_fits(sets.units, 64) && launch_fits((long long)sets.n * a.k.heads * kBinShares, 1024) && launch_fits(n, head_dim / 4)))
             return kNoWork;
         return p.part_bytes + p.list_bytes + p.tile_bytes;
     }
     const DensePlan p = dense_plan(dtype, head_dim, a, sets);
-    if (!launch_fits(xcd_grid(sets.tile[sets.n] * p.parts), 256)) return kNoWork;
+    if (!launch_fits(xcd_grid(sets.units * p.parts), 256)) return kNoWork;
     return p.parts == 1 ? 0 : ((size_t)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads * p.parts * (head_dim + 4) * sizeof(float);
 }
 hipError_t launch_attention(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets, hipStream_t s) {

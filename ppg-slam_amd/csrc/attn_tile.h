@@ -20,21 +20,31 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
-// the set whose [off[i], off[i+1]) holds x; off ascends, off[0] <= x < off[n]
-__device__ __forceinline__ int find_set(const int* off, int n, int x) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (off[mid] <= x) lo = mid;
-        else hi = mid;
-    }
-    return lo;
-}
-// the same for an x that all 64 lanes share, in one load instead of a chain of them
-__device__ __forceinline__ int find_set_wave(const int* off, int n, int x, int lane) {
+// The set whose [off[i], off[i+1]) holds x, the same for all 64 lanes; off ascends, off[0] <= x < off[n], INT_MAX behind off[n].
+__device__ __forceinline__ int find_set(const int* off, int x, int lane) {
     static_assert(PPG_ATTN_MAX_SETS == 128, "two sets per lane");
-    const int a = off[min(lane + 1, n)], b = off[min(lane + 65, n)];
-    return __popcll(__ballot(lane + 1 < n && a <= x)) + __popcll(__ballot(lane + 65 < n && b <= x));
+    return __popcll(__ballot(off[lane + 1] <= x)) + __popcll(__ballot(off[lane + 65] <= x));
+}
+// What a work-group needs to know of its set.
+struct SetHere {
+    int q0, nq, k0, nk, tile0, blk0, blocks;
+};
+__device__ __forceinline__ SetHere set_number(const AttnSets& sets, int s) {
+    const int q0 = sets.q_off[s], k0 = sets.k_off[s], blk0 = sets.blk[s];
+    return {q0, sets.q_off[s + 1] - q0, k0, sets.k_off[s + 1] - k0, sets.tile[s], blk0, sets.blk[s + 1] - blk0};
+}
+// Sets and units of a launch, and what one set alone has: all of it asked for before any of it is looked at.
+struct SetsHere {
+    int n, units;
+    SetHere first;
+};
+__device__ __forceinline__ SetsHere sets_here(const AttnSets& sets) {
+    int n = sets.n, units = sets.units, q0 = sets.q_off[0], q1 = sets.q_off[1], k0 = sets.k_off[0], k1 = sets.k_off[1], blocks = sets.blk[1];
+    asm volatile("" : "+s"(n), "+s"(units), "+s"(q0), "+s"(q1), "+s"(k0), "+s"(k1), "+s"(blocks));   // (the compiler would put the loads off)
+    return {n, units, {q0, q1 - q0, k0, k1 - k0, 0, 0, blocks}};
+}
+__device__ __forceinline__ SetHere set_of(const SetsHere& here, const AttnSets& sets, const int* off, int x, int lane) {
+    return here.n == 1 ? here.first : set_number(sets, find_set(off, x, lane));
 }
 
 template <class T> struct IsF32 { static constexpr bool v = false; };
@@ -210,6 +220,12 @@ __device__ __forceinline__ void mask_scores(f32x16& s, unsigned dead, int h) {
             s[4 * b + e] = __uint_as_float(__builtin_amdgcn_bitop3_b32(x, 0xff800000u, __float_as_uint(s[4 * b + e]), 0xca));   // x ? -inf : s
         }
     }
+}
+
+// where share i of n things begins, of `shares` equal ones (a division of 64 bits takes over a thousand cycles)
+__device__ __forceinline__ int share_begin(int n, int i, int shares) {
+    const unsigned each = (unsigned)n / (unsigned)shares, more = (unsigned)n - each * (unsigned)shares;
+    return (int)(each * (unsigned)i + min((unsigned)i, more));
 }
 
 // work-group L of a launch of n units: XCD L % 8 (launch order) serves a contiguous range of the units, so that the units that

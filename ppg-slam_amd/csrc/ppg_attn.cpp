@@ -62,6 +62,7 @@ int set_count(ppg_ctx* c, const char* who, int n_sets) {
 void block_offsets(ppg::AttnSets& s, int block) {
     s.blk[0] = 0;
     for (int i = 0; i < s.n; i++) s.blk[i + 1] = s.blk[i] + (int)(((long long)s.k_off[i + 1] - s.k_off[i] + block - 1) / block);
+    end_list(s, s.blk);
 }
 
 // what the kernels' launches cannot count

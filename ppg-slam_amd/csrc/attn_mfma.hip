@@ -34,6 +34,34 @@ __device__ __forceinline__ void load_query(u32x4 (&f)[NF], const ppg_rows& q, co
     for (int i = 0; i < Shape<T, D>::NF; i++) f[i] = *(const u32x4*)(x + Shape<T, D>::chunk(i, h) * Shape<T, D>::N);
 }
 
+// The same for a wave's 32 rows by way of an LDS image of its own, when its lanes know their rows' addresses (`mine`: of row
+// lane & 31): neighbouring lanes then load a row's neighbouring chunks, where a lane per row touches 32 or 64 lines with every load
+// (a frame pair's work-groups spent a quarter of their time on that).
+template <class T, int D, int NF = Shape<T, D>::NF> __device__ __forceinline__ void fetch_rows(u32x4 (&x)[NF], const T* mine, int lane) {
+    using S = Shape<T, D>;
+    const unsigned long long at = (unsigned long long)mine;
+#pragma unroll
+    for (int i = 0; i < S::NF; i++) {
+        const int c = lane + 64 * i, r = c / S::CPR;
+        const T* y = (const T*)(((unsigned long long)(unsigned)__shfl((int)(at >> 32), r) << 32) | (unsigned)__shfl((int)at, r));
+        x[i] = *(const u32x4*)(y + (c % S::CPR) * S::N);
+    }
+}
+template <class T, int D, int NF = Shape<T, D>::NF> __device__ __forceinline__ void rows_to_operand(u32x4 (&f)[NF], const u32x4 (&x)[NF], char* image, int lane) {
+    using S = Shape<T, D>;
+    constexpr int ROWB = D * (int)sizeof(T);
+    const int row = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < S::NF; i++) {
+        const int c = lane + 64 * i, r = c / S::CPR;
+        *(u32x4*)(image + r * ROWB + (((c % S::CPR) ^ S::swz_k(r)) << 4)) = x[i];
+    }
+    __builtin_amdgcn_wave_barrier();   // (LDS serves a wave in order)
+#pragma unroll
+    for (int i = 0; i < S::NF; i++) f[i] = *(const u32x4*)(image + row * ROWB + ((S::chunk(i, h) ^ S::swz_k(row)) << 4));
+    __builtin_amdgcn_wave_barrier();
+}
+
 // Rows of 32-bit results: this lane's components of its own row, 4 consecutive ones per register group.
 template <int D> __device__ __forceinline__ void store_row(float* y, const f32x16 (&o)[D / 32], float f, int h) {
 #pragma unroll
@@ -244,24 +272,23 @@ __global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) 
     }
 }
 
-// A wave's own stretch of keys: operands straight from memory, values through an LDS image of its own.
+// A wave's own stretch of keys: keys, then values, through an LDS image of its own.
 // One row against 400003 keys, 4 heads of 64: 410 MB in 87 us, 4.7 TB/s (a copy reaches 5.1).
 template <class T, int D, int BN> struct OwnKeys {
     using S = Shape<T, D>;
     static constexpr int SUB = BN / 32, VC = BN * S::CPR / 64, ROWB = D * (int)sizeof(T);
-    u32x4 rk[SUB][S::NF], rv[VC];
+    u32x4 rk[VC], rv[VC];
     int masked;                  // this lane's key of the tile (the first BN lanes)
     unsigned long long gone;     // all of them, once settle() was called
     // keys j0 .. j0 + BN - 1 of the set at kp / vp, of which n exist (n >= 1: row n - 1 stands in for those behind it)
     __device__ __forceinline__ void load(const T* kp, const T* vp, long long k_row, long long v_row, const uint8_t* skip, int j0, int n, int lane) {
-        const int h = lane >> 5, j = j0 + (lane & (BN - 1));
+        const int j = j0 + (lane & (BN - 1));
         masked = skip ? skip[min(j, n - 1)] : 0;   // first: loads come back in order, and this one is waited for first
         if (j >= n) masked = 1;
 #pragma unroll
-        for (int u = 0; u < SUB; u++) {
-            const T* x = kp + (long long)min(j0 + u * 32 + (lane & 31), n - 1) * k_row;
-#pragma unroll
-            for (int i = 0; i < S::NF; i++) rk[u][i] = *(const u32x4*)(x + S::chunk(i, h) * S::N);
+        for (int i = 0; i < VC; i++) {
+            const int x = lane + 64 * i, r = x / S::CPR;
+            rk[i] = *(const u32x4*)(kp + (long long)min(j0 + r, n - 1) * k_row + (x % S::CPR) * S::N);
         }
 #pragma unroll
         for (int i = 0; i < VC; i++) {
@@ -277,15 +304,27 @@ template <class T, int D, int BN> struct OwnKeys {
             *(u32x4*)(v + r * ROWB + ((ch ^ S::swz_v(r)) << 4)) = (gone >> r) & 1 ? u32x4{0, 0, 0, 0} : rv[i];
         }
     }
-    __device__ __forceinline__ void scores(f32x16 (&sc)[SUB], const u32x4 (&qf)[S::NF], int lane) const {
+    __device__ __forceinline__ void scores(f32x16 (&sc)[SUB], const u32x4 (&qf)[S::NF], char* image, int lane) const {
+        const int h = lane >> 5;
+#pragma unroll
+        for (int i = 0; i < VC; i++) {
+            const int x = lane + 64 * i, r = x / S::CPR, ch = x % S::CPR;
+            *(u32x4*)(image + r * ROWB + ((ch ^ S::swz_k(r)) << 4)) = rk[i];
+        }
+        __builtin_amdgcn_wave_barrier();   // the image is this wave's own and LDS serves a wave in order
 #pragma unroll
         for (int u = 0; u < SUB; u++) {
+            const int r = u * 32 + (lane & 31);
 #pragma unroll
             for (int e = 0; e < 16; e++) sc[u][e] = 0.f;
 #pragma unroll
-            for (int i = 0; i < S::NF; i++) sc[u] = mfma_chunk<T>(rk[u][i], qf[i], sc[u]);
-            if (gone) mask_scores(sc[u], (unsigned)(gone >> (32 * u)), lane >> 5);
+            for (int i = 0; i < S::NF; i++) {
+                const u32x4 kf = *(const u32x4*)(image + r * ROWB + ((S::chunk(i, h) ^ S::swz_k(r)) << 4));
+                sc[u] = mfma_chunk<T>(kf, qf[i], sc[u]);
+            }
+            if (gone) mask_scores(sc[u], (unsigned)(gone >> (32 * u)), h);
         }
+        __builtin_amdgcn_wave_barrier();
     }
 };
 
@@ -340,7 +379,7 @@ __global__ __launch_bounds__(256, IsF32<T>::v && D == 128 ? 1 : 2) void attentio
     const int units = here.units * parts, unit = xcd_unit(blockIdx.x, units);
     if (unit >= units) return;
     const int part = unit % parts, tile = unit / parts;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const SetHere set = set_of(here, sets, sets.tile, tile, lane);
     const int q0 = set.q0, k0 = set.k0, nk = set.nk, kvh = a.k.heads, group = a.q.heads / kvh;
     // SEL: tiles of a query's group never hold rows of another query
@@ -348,8 +387,9 @@ __global__ __launch_bounds__(256, IsF32<T>::v && D == 128 ? 1 : 2) void attentio
     const int g = (tile - set.tile0) / tiles, at = (tile - set.tile0) % tiles;
     const int row0 = SEL ? at / per_q * group + at % per_q * 32 : at * 32;
     const int rows = SEL ? (at / per_q + 1) * group : all;
-    u32x4 qf[S::NF];
-    load_query<T, D>(qf, a.q, row_place(row0 + (lane & 31), rows, group, g, q0), h);
+    const RowPlace place = row_place(row0 + (lane & 31), rows, group, g, q0);
+    u32x4 qx[S::NF], qf[S::NF];
+    fetch_rows<T, D>(qx, (const T*)a.q.p + place.q * a.q.row + place.head * a.q.head, lane);
     const float c = a.scale * kLog2e, slack = rise_slack(c);
     Running<T, D> run;
     run.clear();
@@ -373,14 +413,15 @@ __global__ __launch_bounds__(256, IsF32<T>::v && D == 128 ? 1 : 2) void attentio
         }
     };
     if (from + wave < to) load(from + wave);
+    rows_to_operand<T, D>(qf, qx, lds.v[wave], lane);
     for (int t = from + wave; t < to; t += 4) {
         f32x16 sc[SUB];
         keys.settle(lane);
-        keys.scores(sc, qf, lane);
+        keys.scores(sc, qf, lds.v[wave], lane);
         keys.values_to_lds(lds.v[wave], lane);
         if (t + 4 < to) load(t + 4);
         run.template weights<SUB>(sc, c, slack);
-        __builtin_amdgcn_wave_barrier();   // the image is this wave's own and LDS serves a wave in order
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int u = 0; u < SUB; u++) add_values(run, sc[u], lds.v[wave], u * 32, lane);
         __builtin_amdgcn_wave_barrier();
@@ -666,15 +707,16 @@ __global__ __launch_bounds__(64, IsF32<T>::v && D == 128 ? 1 : 2) void attention
     const int entry = w.list[((long long)(q0 - sets.q_off[0]) * kvh + (long long)g * nq) * a.n_sel + t.y + (group == 1 ? rr : rr / group)];
     const long long q = q0 + entry / a.n_sel;
     const int slot = entry % a.n_sel, head = g * group + (group == 1 ? 0 : rr % group);
-    u32x4 qf[S::NF];
-    load_query<T, D>(qf, a.q, RowPlace{q, head}, h);
+    u32x4 qx[S::NF], qf[S::NF];
+    fetch_rows<T, D>(qx, (const T*)a.q.p + q * a.q.row + head * a.q.head, lane);
+    rows_to_operand<T, D>(qf, qx, lds_v, lane);
     const float c = a.scale * kLog2e, slack = rise_slack(c);
     Running<T, D> run;
     run.clear();
     for (int j = 0; j < n; j += BN) {
         f32x16 sc[SUB];
         keys.settle(lane);
-        keys.scores(sc, qf, lane);
+        keys.scores(sc, qf, lds_v, lane);
         keys.values_to_lds(lds_v, lane);
         if (j + BN < n) keys.load(kp, vp, a.k.row, a.v.row, skip, j + BN, n, lane);
         run.template weights<SUB>(sc, c, slack);

@@ -439,7 +439,7 @@ __global__ __launch_bounds__(1024, 4) void block_select_kernel(BlockSelectLaunch
                 const bool on = high[p] >= t;
                 const unsigned long long m = __ballot(on);
                 if (on) {
-                    const int to = at + __popcll(m & ((1ull << lane) - 1));
+                    const int to = at + bits_below(m);
                     note.cand[to] = (unsigned short)(p * 64 + lane);
                     note.low[to] = low[p];
                     note.high[to] = high[p];
@@ -481,7 +481,7 @@ __global__ __launch_bounds__(1024, 4) void block_select_kernel(BlockSelectLaunch
                 for (int k = 0; k < 2; k++) {
                     in[k] = in[k] && hi[k] >= t;
                     const unsigned long long m = __ballot(in[k]);
-                    if (in[k]) note.cand[kept + __popcll(m & ((1ull << lane) - 1))] = (unsigned short)cand[k];
+                    if (in[k]) note.cand[kept + bits_below(m)] = (unsigned short)cand[k];
                     kept += __popcll(m);
                 }
                 __builtin_amdgcn_wave_barrier();
@@ -546,7 +546,7 @@ __global__ __launch_bounds__(1024, 4) void block_select_kernel(BlockSelectLaunch
             for (int k = 0; k < 3; k++) {
                 const bool take = all[k].idx != 0x7fffffff && order[k] < a.n_sel;
                 const unsigned long long m = __ballot(take);
-                const int place = to + __popcll(m & ((1ull << lane) - 1));
+                const int place = to + bits_below(m);
                 if (take) {
                     note.best_key[place] = all[k].key;
                     note.best_idx[place] = all[k].idx;

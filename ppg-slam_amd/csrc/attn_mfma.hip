@@ -131,12 +131,12 @@ __global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) 
     const SetsHere here = sets_here(sets);
     const int units = here.units * parts, whole = xcd_unit(blockIdx.x, units);
     if (whole >= units) return;
-    const int unit = parts == 1 ? whole : whole / parts, part = parts == 1 ? 0 : whole % parts;
+    const int unit = parts == 1 ? whole : quot24(whole, parts), part = parts == 1 ? 0 : rem24(whole, parts);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const SetHere set = set_of(here, sets, sets.tile, unit, lane);
-    const int q0 = set.q0, k0 = set.k0, nk = set.nk, kvh = a.k.heads, group = a.q.heads / kvh;
+    const int q0 = set.q0, k0 = set.k0, nk = set.nk, kvh = a.k.heads, group = quot24(a.q.heads, kvh);
     const int rows = set.nq * group, tiles = (rows + 127) / 128;
-    const int g = (unit - set.tile0) / tiles, row = ((unit - set.tile0) % tiles) * 128 + wave * 32 + (lane & 31);
+    const int g = quot24(unit - set.tile0, tiles), row = rem24(unit - set.tile0, tiles) * 128 + wave * 32 + (lane & 31);
     const float c = a.scale * kLog2e, slack = rise_slack(c);
     const int all = (nk + BN - 1) / BN, from = share_begin(all, part, parts), to = share_begin(all, part + 1, parts);
 
@@ -165,10 +165,11 @@ __global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) 
         }
     };
     auto store = [&](int t, unsigned long long dead) {   // masked values are zero
+        const Words w = words_of(dead);
 #pragma unroll
         for (int i = 0; i < CH; i++) {
             const int r = r0 + STEP * i;
-            const unsigned live = (dead >> r) & 1 ? 0u : ~0u;
+            const unsigned live = bit_of(w, r) ? 0u : ~0u;
             *(u32x4*)(lds_k[t & 1] + r * ROWB + ((ch0 ^ S::swz_k(r)) << 4)) = rk[i];
             *(u32x4*)(lds_v[t & 1] + r * ROWB + ((ch0 ^ S::swz_v(r)) << 4)) = rv[i] & u32x4{live, live, live, live};
         }
@@ -280,28 +281,53 @@ template <class T, int D, int BN> struct OwnKeys {
     u32x4 rk[VC], rv[VC];
     int masked;                  // this lane's key of the tile (the first BN lanes)
     unsigned long long gone;     // all of them, once settle() was called
-    // keys j0 .. j0 + BN - 1 of the set at kp / vp, of which n exist (n >= 1: row n - 1 stands in for those behind it)
-    __device__ __forceinline__ void load(const T* kp, const T* vp, long long k_row, long long v_row, const uint8_t* skip, int j0, int n, int lane) {
+    const T *kp, *vp;            // the set's first key and value, the same for the wave
+    const uint8_t* skip;
+    long long k_row, v_row;
+    unsigned k_at, v_at;         // this lane's place in a round of loads, in bytes, if it is `near` enough for 32 bits
+    bool near;
+    static constexpr int STEP = 64 / S::CPR;   // rows of a round
+    __device__ __forceinline__ void begin(const T* k, const T* v, long long k_row_, long long v_row_, const uint8_t* skip_, int lane) {
+        kp = k;
+        vp = v;
+        skip = skip_;
+        k_row = k_row_;
+        v_row = v_row_;
+        near = (k_row | v_row) < (1 << 24);
+        k_at = lane / S::CPR * (unsigned)k_row * sizeof(T) + lane % S::CPR * 16;
+        v_at = lane / S::CPR * (unsigned)v_row * sizeof(T) + lane % S::CPR * 16;
+    }
+    // keys first + j0 .. first + j0 + BN - 1, of which those below first + n exist (n >= 1: row n - 1 stands in for those behind it)
+    __device__ __forceinline__ void load(int first, int j0, int n, int lane) {
         const int j = j0 + (lane & (BN - 1));
-        masked = skip ? skip[min(j, n - 1)] : 0;   // first: loads come back in order, and this one is waited for first
+        masked = skip ? skip[first + min(j, n - 1)] : 0;   // first: loads come back in order, and this one is waited for first
         if (j >= n) masked = 1;
+        if (near && j0 + BN <= n) {   // the same for the wave; addresses are its own, but for one offset per lane
+            const char *x = (const char*)(kp + (long long)(first + j0) * k_row), *y = (const char*)(vp + (long long)(first + j0) * v_row);
 #pragma unroll
-        for (int i = 0; i < VC; i++) {
-            const int x = lane + 64 * i, r = x / S::CPR;
-            rk[i] = *(const u32x4*)(kp + (long long)min(j0 + r, n - 1) * k_row + (x % S::CPR) * S::N);
-        }
+            for (int i = 0; i < VC; i++) rk[i] = *(const u32x4*)(x + (long long)(STEP * i * sizeof(T)) * k_row + k_at);
 #pragma unroll
-        for (int i = 0; i < VC; i++) {
-            const int x = lane + 64 * i, r = x / S::CPR;
-            rv[i] = *(const u32x4*)(vp + (long long)min(j0 + r, n - 1) * v_row + (x % S::CPR) * S::N);
+            for (int i = 0; i < VC; i++) rv[i] = *(const u32x4*)(y + (long long)(STEP * i * sizeof(T)) * v_row + v_at);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VC; i++) {
+                const int x = lane + 64 * i, r = x / S::CPR;
+                rk[i] = *(const u32x4*)(kp + (long long)(first + min(j0 + r, n - 1)) * k_row + (x % S::CPR) * S::N);
+            }
+#pragma unroll
+            for (int i = 0; i < VC; i++) {
+                const int x = lane + 64 * i, r = x / S::CPR;
+                rv[i] = *(const u32x4*)(vp + (long long)(first + min(j0 + r, n - 1)) * v_row + (x % S::CPR) * S::N);
+            }
         }
     }
     __device__ __forceinline__ void settle(int lane) { gone = __ballot(lane < BN && masked); }
     __device__ __forceinline__ void values_to_lds(char* v, int lane) const {
+        const Words w = words_of(gone);
 #pragma unroll
         for (int i = 0; i < VC; i++) {
             const int x = lane + 64 * i, r = x / S::CPR, ch = x % S::CPR;
-            *(u32x4*)(v + r * ROWB + ((ch ^ S::swz_v(r)) << 4)) = (gone >> r) & 1 ? u32x4{0, 0, 0, 0} : rv[i];
+            *(u32x4*)(v + r * ROWB + ((ch ^ S::swz_v(r)) << 4)) = bit_of(w, r) ? u32x4{0, 0, 0, 0} : rv[i];
         }
     }
     __device__ __forceinline__ void scores(f32x16 (&sc)[SUB], const u32x4 (&qf)[S::NF], char* image, int lane) const {
@@ -378,13 +404,13 @@ __global__ __launch_bounds__(256, IsF32<T>::v && D == 128 ? 1 : 2) void attentio
     const SetsHere here = sets_here(sets);
     const int units = here.units * parts, unit = xcd_unit(blockIdx.x, units);
     if (unit >= units) return;
-    const int part = unit % parts, tile = unit / parts;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int part = rem24(unit, parts), tile = quot24(unit, parts);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const SetHere set = set_of(here, sets, sets.tile, tile, lane);
-    const int q0 = set.q0, k0 = set.k0, nk = set.nk, kvh = a.k.heads, group = a.q.heads / kvh;
+    const int q0 = set.q0, k0 = set.k0, nk = set.nk, kvh = a.k.heads, group = quot24(a.q.heads, kvh);
     // SEL: tiles of a query's group never hold rows of another query
     const int nq = set.nq, all = nq * group, per_q = (group + 31) / 32, tiles = SEL ? nq * per_q : (all + 31) / 32;
-    const int g = (tile - set.tile0) / tiles, at = (tile - set.tile0) % tiles;
+    const int g = quot24(tile - set.tile0, tiles), at = rem24(tile - set.tile0, tiles);
     const int row0 = SEL ? at / per_q * group + at % per_q * 32 : at * 32;
     const int rows = SEL ? (at / per_q + 1) * group : all;
     const RowPlace place = row_place(row0 + (lane & 31), rows, group, g, q0);
@@ -395,21 +421,21 @@ __global__ __launch_bounds__(256, IsF32<T>::v && D == 128 ? 1 : 2) void attentio
     run.clear();
     const T* kp = (const T*)a.k.p + g * a.k.head + (long long)k0 * a.k.row;
     const T* vp = (const T*)a.v.p + g * a.v.head + (long long)k0 * a.v.row;
-    const uint8_t* skip = a.skip ? a.skip + k0 : nullptr;
     const int* sel = SEL ? a.sel + ((long long)(q0 + at / per_q) * kvh + g) * a.n_sel : nullptr;
     const int per_shift = SEL && a.block > BN ? __builtin_ctz((unsigned)a.block / BN) : 0, blocks = SEL ? (nk + a.block - 1) / a.block : 0;
     const int nt = SEL ? (nk ? a.n_sel << per_shift : 0) : (int)(((unsigned)nk + BN - 1) / BN);
     const int from = share_begin(nt, part, parts), to = share_begin(nt, part + 1, parts);
     OwnKeys<T, D, BN> keys;
+    keys.begin(kp, vp, a.k.row, a.v.row, a.skip ? a.skip + k0 : nullptr, lane);
     auto load = [&](int t) {
         if constexpr (SEL) {
             const int b = sel[t >> per_shift], j = (t & ((1 << per_shift) - 1)) * BN;
             const bool ok = b >= 0 && b < blocks;
-            const int first = ok ? b * a.block : 0, n = min(a.block, nk - first);
-            keys.load(kp + first * a.k.row, vp + first * a.v.row, a.k.row, a.v.row, skip ? skip + first : nullptr, j, n, lane);
+            const int first = ok ? b * a.block : 0;
+            keys.load(first, j, min(a.block, nk - first), lane);
             if (!ok) keys.masked = 1;
         } else {
-            keys.load(kp, vp, a.k.row, a.v.row, skip, t * BN, nk, lane);
+            keys.load(0, t * BN, nk, lane);
         }
     };
     if (from + wave < to) load(from + wave);
@@ -437,7 +463,7 @@ __global__ __launch_bounds__(256, IsF32<T>::v && D == 128 ? 1 : 2) void attentio
         const f32x4 y = of_meeting(lds.sums, r, d, c, m, l);
         const RowPlace p = row_place(row0 + r, rows, group, g, q0);
         if (parts > 1) {
-            Part<D>& w = ((Part<D>*)a.work)[((p.q - sets.q_off[0]) * a.q.heads + p.head) * parts + part];
+            Part<D>& w = ((Part<D>*)a.work)[(long long)((int)(p.q - here.first.q0) * a.q.heads + p.head) * parts + part];
             *(f32x4*)&w.o[d] = y;
             if (d == 0) {
                 w.m = m;
@@ -552,11 +578,13 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, 
 }
 
 // ---- selected blocks, many queries ----
-// A region is one (set, key head); entry e of it is place e % n_sel in the list of its query e / n_sel.  Where things lie:
+// A region is one (set, key head); its entries are the places in the lists of its queries.  Where things lie:
 struct BinWork {
-    int* list;     // entries by block, [regions][queries of the set * n_sel]
-    int4* tile;    // (block, first entry in the region's list, rows of the block = entries * group, first row of the tile); block -1: unused
+    unsigned* list;   // entries by block, [regions][queries of the set * n_sel]: query of the set << entry_shift | place
+    int4* tile;       // (block, its first entry in the list, first of the tile's rows among entries * group, set << 22 | key head << 6 | rows of the tile); block -1: unused
 };
+__host__ __device__ inline int entry_shift(int n_sel) { return n_sel > 1 ? 32 - __builtin_clz((unsigned)n_sel - 1) : 0; }   // (queries * n_sel < 2^30)
+static_assert(PPG_ATTN_MAX_SETS <= 128, "seven bits for the set");
 // A region's blocks are counted by one work-group, or in kBinShares equal shares by as many where the entries are more than the
 // blocks (region_tiles() then has room for every block's last tile) and every share has blocks (what a share without any would
 // have to know, the entries before it, it does not count).
@@ -575,16 +603,18 @@ __host__ __device__ inline int region_tiles(long long nq, int n_sel, int group, 
 // behind those of the blocks before it (every share counts them), its tiles where those blocks' could end at the latest.
 constexpr int kBins = 8192;    // blocks counted at a time (32 KB of LDS)
 constexpr int kBinHold = 16;   // entries per thread that stay in registers between the two passes
+template <int W>               // entries that a load takes: 4 where n_sel is a multiple of that
 __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets sets, BinWork w) {
     __shared__ int cnt[kBins];
     __shared__ int sum_e[16], sum_t[16], sum_b[16];
-    const int kvh = a.k.heads, group = a.q.heads / kvh, s = blockIdx.x / kvh, g = blockIdx.x % kvh;
+    const int kvh = a.k.heads, group = quot24(a.q.heads, kvh), s = quot24(blockIdx.x, kvh), g = rem24(blockIdx.x, kvh);
     const SetsHere here = sets_here(sets);
     const SetHere set = here.n == 1 ? here.first : set_number(sets, s);
     const int q0 = set.q0, nq = set.nq, blocks = set.blocks, n = nq * a.n_sel;
     const int* sel = a.sel + ((long long)q0 * kvh + g) * a.n_sel;
-    const long long step = (long long)kvh * a.n_sel;
-    int* list = w.list + ((long long)(q0 - sets.q_off[0]) * kvh + (long long)g * nq) * a.n_sel;
+    const int step = kvh * a.n_sel, per_q = a.n_sel / W, shift = entry_shift(a.n_sel);
+    const int list0 = ((q0 - here.first.q0) * kvh + g * nq) * a.n_sel;   // of this region's entries
+    unsigned* list = w.list + list0;
     int4* tile = w.tile + set.tile0 + (long long)g * region_tiles(nq, a.n_sel, group, blocks);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int shares = bin_shares(nq, a.n_sel, blocks), share = blockIdx.y;
@@ -593,19 +623,30 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
     int e0 = 0, t0 = 0;   // where the entries and tiles of this round's bins go
     int held[kBinHold], rank[kBinHold];
     const bool once = n <= kBinHold * 1024;
-    const int dq = 1024 / a.n_sel, dr = 1024 % a.n_sel;   // 1024 entries on, in queries and places
-    auto load = [&](int from) {
-        int q = (from + tid) / a.n_sel, r = (from + tid) % a.n_sel;
+    const int dq = 1024 / per_q, dr = 1024 % per_q;   // 1024 times W entries on, in queries and places
+    // this thread's entries, W at a time, of the kBinHold * 1024 from `from` on: f(which, query, place, there is one)
+    auto each = [&](int from, auto f) {
+        int q = (from / W + tid) / per_q, r = (from / W + tid) % per_q;
 #pragma unroll
-        for (int i = 0; i < kBinHold; i++) {
-            held[i] = from + i * 1024 + tid < n ? sel[q * step + r] : -1;
+        for (int i = 0; i < kBinHold / W; i++) {
+            if (from + i * 1024 * W >= n) break;   // the same for all
+            f(i, q, r * W, from + (i * 1024 + tid) * W < n);
             q += dq;
             r += dr;
-            if (r >= a.n_sel) {
-                r -= a.n_sel;
+            if (r >= per_q) {
+                r -= per_q;
                 q++;
             }
         }
+    };
+    auto load = [&](int from) {
+#pragma unroll
+        for (int i = 0; i < kBinHold; i++) held[i] = -1;
+        each(from, [&](int i, int q, int r, bool on) {
+            if (!on) return;
+#pragma unroll
+            for (int w = 0; w < W; w++) held[i * W + w] = sel[q * step + r + w];
+        });
     };
     for (int b0 = lo; b0 < hi; b0 += kBins) {
         const int nb = min(kBins, hi - b0), per = (nb + 1023) / 1024;
@@ -616,8 +657,8 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
         for (int from = 0; from < n; from += kBinHold * 1024) {
             if (!once) load(from);
 #pragma unroll
-            for (int i = 0; i < kBinHold; i++)
-            {
+            for (int i = 0; i < kBinHold; i++) {
+                if (from + i / W * 1024 * W >= n) break;
                 if (held[i] >= b0 && held[i] - b0 < nb) rank[i] = atomicAdd(&cnt[held[i] - b0], 1);
                 below += held[i] >= 0 && held[i] < lo;
             }
@@ -660,16 +701,20 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
         }
         for (int i = tid * per; i < min(nb, (tid + 1) * per); i++) {
             const int c = cnt[i], rows = c * group;
-            for (int r = 0; r < rows; r += 32) tile[tb++] = make_int4(b0 + i, eb, rows, r);
+            for (int r = 0; r < rows; r += 32) tile[tb++] = make_int4(b0 + i, list0 + eb, r, s << 22 | g << 6 | min(32, rows - r));
             cnt[i] = eb;   // where the block's next entry goes
             eb += c;
         }
         __syncthreads();
         for (int from = 0; from < n; from += kBinHold * 1024) {
             if (!once) load(from);
+            each(from, [&](int i, int q, int r, bool) {
 #pragma unroll
-            for (int i = 0; i < kBinHold; i++)
-                if (held[i] >= b0 && held[i] - b0 < nb) list[once ? cnt[held[i] - b0] + rank[i] : atomicAdd(&cnt[held[i] - b0], 1)] = from + i * 1024 + tid;
+                for (int w = 0; w < W; w++) {
+                    const int b = held[i * W + w];
+                    if (b >= b0 && b - b0 < nb) list[once ? cnt[b - b0] + rank[i * W + w] : atomicAdd(&cnt[b - b0], 1)] = (unsigned)q << shift | (r + w);
+                }
+            });
         }
         __syncthreads();
     }
@@ -689,24 +734,22 @@ __global__ __launch_bounds__(64, IsF32<T>::v && D == 128 ? 1 : 2) void attention
     __shared__ alignas(16) char lds_v[IMG];
     const int lane = threadIdx.x, h = lane >> 5;
     // (in launch order: hardly two tiles read the same block, and a region's unused tiles would leave some XCDs without work)
-    const int at = (int)blockIdx.x;
-    const int4 t = w.tile[at];
+    const int4 t = w.tile[blockIdx.x];
     const SetsHere here = sets_here(sets);
-    const SetHere set = set_of(here, sets, sets.tile, at, lane);
-    const int q0 = set.q0, nq = set.nq, k0 = set.k0, nk = set.nk, kvh = a.k.heads, group = a.q.heads / kvh;
-    const int cap = region_tiles(nq, a.n_sel, group, set.blocks);
-    const int g = (at - set.tile0) / cap;
-    if (t.x < 0) return;
-    const int first = t.x * a.block, n = min(a.block, nk - first);
-    const T* kp = (const T*)a.k.p + g * a.k.head + (long long)(k0 + first) * a.k.row;
-    const T* vp = (const T*)a.v.p + g * a.v.head + (long long)(k0 + first) * a.v.row;
-    const uint8_t* skip = a.skip ? a.skip + k0 + first : nullptr;
+    const int block = __builtin_amdgcn_readfirstlane(t.x), region = __builtin_amdgcn_readfirstlane(t.w);
+    if (block < 0) return;
+    const SetHere set = here.n == 1 ? here.first : set_number(sets, region >> 22);
+    const int g = (region >> 6) & 0xffff, left = region & 63;   // (1..32 rows)
+    const int group = quot24(a.q.heads, a.k.heads), rr = t.z + min(lane & 31, left - 1);
+    const int in = group == 1 ? rr : rr / group;
+    const unsigned entry = w.list[t.y + in];   // before the keys, which are not waited for so soon
+    const int first = block * a.block, n = min(a.block, set.nk - first);
     OwnKeys<T, D, BN> keys;
-    keys.load(kp, vp, a.k.row, a.v.row, skip, 0, n, lane);
-    const int row = t.w + (lane & 31), rr = min(row, t.z - 1);
-    const int entry = w.list[((long long)(q0 - sets.q_off[0]) * kvh + (long long)g * nq) * a.n_sel + t.y + (group == 1 ? rr : rr / group)];
-    const long long q = q0 + entry / a.n_sel;
-    const int slot = entry % a.n_sel, head = g * group + (group == 1 ? 0 : rr % group);
+    keys.begin((const T*)a.k.p + g * a.k.head + (long long)set.k0 * a.k.row, (const T*)a.v.p + g * a.v.head + (long long)set.k0 * a.v.row, a.k.row,
+               a.v.row, a.skip ? a.skip + set.k0 : nullptr, lane);
+    keys.load(first, 0, n, lane);
+    const int shift = entry_shift(a.n_sel), slot = entry & ((1u << shift) - 1), head = g * group + (group == 1 ? 0 : rr - in * group);
+    const long long q = set.q0 + (int)(entry >> shift);
     u32x4 qx[S::NF], qf[S::NF];
     fetch_rows<T, D>(qx, (const T*)a.q.p + q * a.q.row + head * a.q.head, lane);
     rows_to_operand<T, D>(qf, qx, lds_v, lane);
@@ -718,7 +761,7 @@ __global__ __launch_bounds__(64, IsF32<T>::v && D == 128 ? 1 : 2) void attention
         keys.settle(lane);
         keys.scores(sc, qf, lds_v, lane);
         keys.values_to_lds(lds_v, lane);
-        if (j + BN < n) keys.load(kp, vp, a.k.row, a.v.row, skip, j + BN, n, lane);
+        if (j + BN < n) keys.load(first, j + BN, n, lane);
         run.template weights<SUB>(sc, c, slack);
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -727,7 +770,7 @@ __global__ __launch_bounds__(64, IsF32<T>::v && D == 128 ? 1 : 2) void attention
     }
     const float l = run.sum();
     using P = ListPart<T, D>;
-    P* to = row < t.z ? (P*)a.work + (((q - sets.q_off[0]) * a.q.heads + head) * a.n_sel + slot) : nullptr;
+    P* to = (lane & 31) < left ? (P*)a.work + ((int)(q - here.first.q0) * a.q.heads + head) * a.n_sel + slot : nullptr;
     if constexpr (!__is_same(T, __bf16)) {
         if (!to) return;   // (both lane halves of a row leave together)
         store_row<D>(to->o, run.o, 1.f, h);
@@ -848,10 +891,12 @@ template <class T, int D> hipError_t run(const AttentionLaunch& a, AttnSets& set
             return e != hipSuccess || p.parts == 1 ? e : join<T, D, false>(a, sets, p.parts, s);
         }
         BinWork w;
-        w.list = (int*)((char*)a.work + p.part_bytes);
+        w.list = (unsigned*)((char*)a.work + p.part_bytes);
         w.tile = (int4*)((char*)w.list + p.list_bytes);
         if (sets.units) {
-            bin_kernel<<<dim3(sets.n * a.k.heads, kBinShares), 1024, 0, s>>>(a, sets, w);
+            const dim3 grid(sets.n * a.k.heads, kBinShares);
+            if (a.n_sel % 4) bin_kernel<1><<<grid, 1024, 0, s>>>(a, sets, w);
+            else bin_kernel<4><<<grid, 1024, 0, s>>>(a, sets, w);
             if ((e = hipGetLastError()) != hipSuccess) return e;
             attention_blocks_kernel<T, D><<<(unsigned)sets.units, 64, 0, s>>>(a, sets, w);
             if ((e = hipGetLastError()) != hipSuccess) return e;

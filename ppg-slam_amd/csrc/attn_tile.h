@@ -47,6 +47,19 @@ __device__ __forceinline__ SetHere set_of(const SetsHere& here, const AttnSets& 
     return here.n == 1 ? here.first : set_number(sets, find_set(off, x, lane));
 }
 
+// Bit r of m, and how many of its bits lie below the lane's, without a 64-bit shift by what a lane holds: with the amount in the last
+// register of a wave's allocation such a shift has given wrong bits here (masks of a kernel that uses all 256).
+struct Words {
+    unsigned lo, hi;
+};
+__device__ __forceinline__ Words words_of(unsigned long long m) {   // m: the same for the wave
+    unsigned lo = (unsigned)m, hi = (unsigned)(m >> 32);
+    asm("" : "+s"(lo), "+s"(hi));   // (the compiler would make the two one 64-bit shift again)
+    return {lo, hi};
+}
+__device__ __forceinline__ bool bit_of(Words m, int r) { return (((r & 32) ? m.hi : m.lo) >> (r & 31)) & 1; }
+__device__ __forceinline__ int bits_below(unsigned long long m) { return __builtin_amdgcn_mbcnt_hi((unsigned)(m >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)m, 0)); }
+
 template <class T> struct IsF32 { static constexpr bool v = false; };
 template <> struct IsF32<float> { static constexpr bool v = true; };
 
@@ -222,8 +235,13 @@ __device__ __forceinline__ void mask_scores(f32x16& s, unsigned dead, int h) {
     }
 }
 
-// where share i of n things begins, of `shares` equal ones (a division of 64 bits takes over a thousand cycles)
+// Divisions are long chains of dependent instructions in a work-group's start.  24 bits (numbers of work-groups, heads, parts) have a
+// short one, which the compiler takes when it sees that there are no more.
+__device__ __forceinline__ int quot24(int a, int b) { return (int)(((unsigned)a & 0xffffff) / ((unsigned)b & 0xffffff)); }
+__device__ __forceinline__ int rem24(int a, int b) { return (int)(((unsigned)a & 0xffffff) % ((unsigned)b & 0xffffff)); }
+// where share i of n things begins, of `shares` equal ones
 __device__ __forceinline__ int share_begin(int n, int i, int shares) {
+    if (shares == 1) return i ? n : 0;
     const unsigned each = (unsigned)n / (unsigned)shares, more = (unsigned)n - each * (unsigned)shares;
     return (int)(each * (unsigned)i + min((unsigned)i, more));
 }

@@ -603,7 +603,6 @@ __host__ __device__ inline int region_tiles(long long nq, int n_sel, int group, 
 // behind those of the blocks before it (every share counts them), its tiles where those blocks' could end at the latest.
 constexpr int kBins = 8192;    // blocks counted at a time (32 KB of LDS)
 constexpr int kBinHold = 16;   // entries per thread that stay in registers between the two passes
-template <int W>               // entries that a load takes: 4 where n_sel is a multiple of that
 __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets sets, BinWork w) {
     __shared__ int cnt[kBins];
     __shared__ int sum_e[16], sum_t[16], sum_b[16];
@@ -612,7 +611,7 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
     const SetHere set = here.n == 1 ? here.first : set_number(sets, s);
     const int q0 = set.q0, nq = set.nq, blocks = set.blocks, n = nq * a.n_sel;
     const int* sel = a.sel + ((long long)q0 * kvh + g) * a.n_sel;
-    const int step = kvh * a.n_sel, per_q = a.n_sel / W, shift = entry_shift(a.n_sel);
+    const int step = kvh * a.n_sel, shift = entry_shift(a.n_sel);
     const int list0 = ((q0 - here.first.q0) * kvh + g * nq) * a.n_sel;   // of this region's entries
     unsigned* list = w.list + list0;
     int4* tile = w.tile + set.tile0 + (long long)g * region_tiles(nq, a.n_sel, group, blocks);
@@ -623,18 +622,19 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
     int e0 = 0, t0 = 0;   // where the entries and tiles of this round's bins go
     int held[kBinHold], rank[kBinHold];
     const bool once = n <= kBinHold * 1024;
-    const int dq = 1024 / per_q, dr = 1024 % per_q;   // 1024 times W entries on, in queries and places
-    // this thread's entries, W at a time, of the kBinHold * 1024 from `from` on: f(which, query, place, there is one)
+    const int dq = 1024 / a.n_sel, dr = 1024 % a.n_sel;   // 1024 entries on, in queries and places
+    // this thread's entries of the kBinHold * 1024 from `from` on (one at a time: neighbouring lanes take neighbouring entries, which
+    // name different blocks; four at a time 4 us more for 8 streams): f(which, query, place)
     auto each = [&](int from, auto f) {
-        int q = (from / W + tid) / per_q, r = (from / W + tid) % per_q;
+        int q = (from + tid) / a.n_sel, r = (from + tid) % a.n_sel;
 #pragma unroll
-        for (int i = 0; i < kBinHold / W; i++) {
-            if (from + i * 1024 * W >= n) break;   // the same for all
-            f(i, q, r * W, from + (i * 1024 + tid) * W < n);
+        for (int i = 0; i < kBinHold; i++) {
+            if (from + i * 1024 >= n) break;   // the same for all
+            f(i, q, r);
             q += dq;
             r += dr;
-            if (r >= per_q) {
-                r -= per_q;
+            if (r >= a.n_sel) {
+                r -= a.n_sel;
                 q++;
             }
         }
@@ -642,10 +642,8 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
     auto load = [&](int from) {
 #pragma unroll
         for (int i = 0; i < kBinHold; i++) held[i] = -1;
-        each(from, [&](int i, int q, int r, bool on) {
-            if (!on) return;
-#pragma unroll
-            for (int w = 0; w < W; w++) held[i * W + w] = sel[q * step + r + w];
+        each(from, [&](int i, int q, int r) {
+            if (from + i * 1024 + tid < n) held[i] = sel[q * step + r];
         });
     };
     for (int b0 = lo; b0 < hi; b0 += kBins) {
@@ -658,7 +656,7 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
             if (!once) load(from);
 #pragma unroll
             for (int i = 0; i < kBinHold; i++) {
-                if (from + i / W * 1024 * W >= n) break;
+                if (from + i * 1024 >= n) break;
                 if (held[i] >= b0 && held[i] - b0 < nb) rank[i] = atomicAdd(&cnt[held[i] - b0], 1);
                 below += held[i] >= 0 && held[i] < lo;
             }
@@ -708,12 +706,9 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
         __syncthreads();
         for (int from = 0; from < n; from += kBinHold * 1024) {
             if (!once) load(from);
-            each(from, [&](int i, int q, int r, bool) {
-#pragma unroll
-                for (int w = 0; w < W; w++) {
-                    const int b = held[i * W + w];
-                    if (b >= b0 && b - b0 < nb) list[once ? cnt[b - b0] + rank[i * W + w] : atomicAdd(&cnt[b - b0], 1)] = (unsigned)q << shift | (r + w);
-                }
+            each(from, [&](int i, int q, int r) {
+                const int b = held[i];
+                if (b >= b0 && b - b0 < nb) list[once ? cnt[b - b0] + rank[i] : atomicAdd(&cnt[b - b0], 1)] = (unsigned)q << shift | r;
             });
         }
         __syncthreads();
@@ -894,9 +889,7 @@ template <class T, int D> hipError_t run(const AttentionLaunch& a, AttnSets& set
         w.list = (unsigned*)((char*)a.work + p.part_bytes);
         w.tile = (int4*)((char*)w.list + p.list_bytes);
         if (sets.units) {
-            const dim3 grid(sets.n * a.k.heads, kBinShares);
-            if (a.n_sel % 4) bin_kernel<1><<<grid, 1024, 0, s>>>(a, sets, w);
-            else bin_kernel<4><<<grid, 1024, 0, s>>>(a, sets, w);
+            bin_kernel<<<dim3(sets.n * a.k.heads, kBinShares), 1024, 0, s>>>(a, sets, w);
             if ((e = hipGetLastError()) != hipSuccess) return e;
             attention_blocks_kernel<T, D><<<(unsigned)sets.units, 64, 0, s>>>(a, sets, w);
             if ((e = hipGetLastError()) != hipSuccess) return e;

@@ -128,14 +128,14 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryLaunch a, int tiles0)
 // One work-group per block.  The block's rows are taken 16 bytes at a time: a thread owns one chunk position and every
 // `lanes`-th row, sums in 64 bits (the sum of 128 numbers of 8 or 11 bits is exact while their exponents span less than 35 steps),
 // and the partial sums of a position meet in LDS.
-template <class T, int D>
-__global__ __launch_bounds__(256) void block_means_kernel(BlockMeansLaunch a, AttnSets sets) {
+template <class T, int D, class Sets>
+__global__ __launch_bounds__(256) void block_means_kernel(BlockMeansLaunch a, Sets sets) {
     constexpr int N = 16 / (int)sizeof(T), CPR = D / N;
     __shared__ double part[256][N];
     __shared__ unsigned char keep[128];
     __shared__ int kept[2];
     const int b = blockIdx.x, tid = threadIdx.x;
-    const SetHere set = set_of(sets_here(sets), sets, sets.blk, b, tid & 63);
+    const SetHere set = set_of_block(sets, b, tid & 63);
     const int at = (b - set.blk0) * a.block, first = set.k0 + at, n = min(a.block, set.nk - at);
     if (tid < 128) {
         const bool on = tid < n && !(a.skip && a.skip[first + tid]);
@@ -288,16 +288,16 @@ template <int D, int ROWS, int PER> struct SelectLds {
     float norm[PER * 64];                 // |mean|, -1 for a block that cannot be selected
     char q[2][ROWS * D * 2];           // the summed queries' upper and lower halves, chunks permuted against bank conflicts
 };
-template <class T, int D, int ROWS, int PER>
-__global__ __launch_bounds__(1024, 4) void block_select_kernel(BlockSelectLaunch a, AttnSets sets) {
+template <class T, int D, int ROWS, int PER, class Sets>
+__global__ __launch_bounds__(1024, 4) void block_select_kernel(BlockSelectLaunch a, Sets sets) {
     constexpr int CHUNK = PER * 64, RPW = ROWS / kSelWaves, N = 16 / (int)sizeof(T);
     constexpr int LPC = D / 16, CPP = 64 / LPC;   // lanes that share a candidate's product, candidates of a pass
     __shared__ alignas(16) SelectLds<D, ROWS, PER> lds;
-    const SetsHere here = sets_here(sets);
+    const Launch here = launch_of(sets);
     const int unit = xcd_unit(blockIdx.x, here.units);
     if (unit >= here.units) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const SetHere set = set_of(here, sets, sets.tile, unit, lane);
+    const SetHere set = set_of_tile(sets, unit, lane);
     const int q0 = set.q0, nq = set.nq;
     // the heads in turn: work-groups that run at the same time then read whole rows of means between them, and with those all
     // channels of the L2
@@ -621,8 +621,11 @@ bool block_means_fits(const AttnSets& sets) { return launch_fits(sets.blk[sets.n
 hipError_t launch_block_means(int dtype, int head_dim, const BlockMeansLaunch& a, AttnSets& sets, hipStream_t s) {
     const int nb = sets.blk[sets.n];
     if (!nb) return hipSuccess;
-    BY_TYPE(dtype, BY_DIM(head_dim, (block_means_kernel<T, D><<<nb, 256, 0, s>>>(a, sets))));
-    return hipGetLastError();
+    return with_sets(sets, [&](const auto& st) {
+        using Sets = std::decay_t<decltype(st)>;
+        BY_TYPE(dtype, BY_DIM(head_dim, (block_means_kernel<T, D, Sets><<<nb, 256, 0, s>>>(a, st))));
+        return hipGetLastError();
+    });
 }
 
 static int select_tiles(const BlockSelectLaunch& a, AttnSets& sets, int rows) {
@@ -637,13 +640,16 @@ hipError_t launch_block_select(int dtype, int head_dim, const BlockSelectLaunch&
     for (int i = 0; i < sets.n; i++) most = std::max(most, sets.blk[i + 1] - sets.blk[i]);
     // a row per wave where that still leaves CUs without work (one frame of 500 rows, 4 heads, 313 blocks: 13 us, 23 us with two), else two, which read
     // the means half as often (8 streams of 1024 rows: 107 us, 149 us with one); few blocks: as many registers as those take
-#define SELECT(ROWS, PER) BY_TYPE(dtype, BY_DIM(head_dim, (block_select_kernel<T, D, ROWS, PER><<<xcd_grid(sets.units), 1024, 0, s>>>(a, sets))))
+#define SELECT(ROWS, PER)                                                                                                                      \
+    return with_sets(sets, [&](const auto& st) {                                                                                               \
+        BY_TYPE(dtype, BY_DIM(head_dim, (block_select_kernel<T, D, ROWS, PER, std::decay_t<decltype(st)>><<<xcd_grid(sets.units), 1024, 0, s>>>(a, st)))); \
+        return hipGetLastError();                                                                                                              \
+    })
     if (select_tiles(a, sets, 32) >= 256) SELECT(32, 17);
     else if (!select_tiles(a, sets, 16)) return hipSuccess;
     else if (most <= 5 * 64) SELECT(16, 5);
     else SELECT(16, 17);
 #undef SELECT
-    return hipGetLastError();
 }
 
 }  // namespace ppg

@@ -120,20 +120,20 @@ template <int D> struct Part {
 // the busier one (4 % of the time at 64 and at 128 components).  Those are the rounded weights, the same that meet the
 // values, but their sum is not good enough for a log: with lse the vector unit adds up the unrounded ones.
 constexpr int kWindow = 64;   // 64-key words of the mask in LDS at a time
-template <class T, int D, int BN, bool UNIT>
-__global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) void attention_wide_kernel(AttentionLaunch a, AttnSets sets, int parts) {
+template <class T, int D, int BN, bool UNIT, class Sets>
+__global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) void attention_wide_kernel(AttentionLaunch a, Sets sets, int parts) {
     using S = Shape<T, D>;
     constexpr int SUB = BN / 32, CH = BN * S::CPR / 256, ROWB = D * (int)sizeof(T), TILE = BN * ROWB, STEP = 256 / S::CPR;
     constexpr unsigned long long FULL = BN == 64 ? ~0ull : 0xffffffffull;
     static_assert(BN * S::CPR % 256 == 0, "tile loads are whole rounds of the work-group");
     __shared__ alignas(16) char lds_k[2][TILE], lds_v[2][TILE];
     __shared__ unsigned long long lds_dead[kWindow];
-    const SetsHere here = sets_here(sets);
+    const Launch here = launch_of(sets);
     const int units = here.units * parts, whole = xcd_unit(blockIdx.x, units);
     if (whole >= units) return;
     const int unit = parts == 1 ? whole : quot24(whole, parts), part = parts == 1 ? 0 : rem24(whole, parts);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    const SetHere set = set_of(here, sets, sets.tile, unit, lane);
+    const SetHere set = set_of_tile(sets, unit, lane);
     const int q0 = set.q0, k0 = set.k0, nk = set.nk, kvh = a.k.heads, group = quot24(a.q.heads, kvh);
     const int rows = set.nq * group, tiles = (rows + 127) / 128;
     const int g = quot24(unit - set.tile0, tiles), row = rem24(unit - set.tile0, tiles) * 128 + wave * 32 + (lane & 31);
@@ -251,7 +251,7 @@ __global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) 
     const float l = run.sum();
     if (parts > 1) {
         if (row >= rows) return;
-        Part<D>& w = ((Part<D>*)a.work)[((place.q - sets.q_off[0]) * a.q.heads + place.head) * parts + part];
+        Part<D>& w = ((Part<D>*)a.work)[(long long)((int)(place.q - here.q0) * a.q.heads + place.head) * parts + part];
         store_row<D>(w.o, run.o, 1.f, h);
         if (h == 0) {
             w.m = run.m;
@@ -393,20 +393,20 @@ template <int D> struct PartH {
 template <class T, int D> using ListPart = std::conditional_t<__is_same(T, __bf16), PartH<D>, Part<D>>;
 
 // SEL: a unit's rows are the group of one query, its keys the blocks of that query's list.
-template <class T, int D, int BN, bool SEL>
-__global__ __launch_bounds__(256, IsF32<T>::v && D == 128 ? 1 : 2) void attention_split_kernel(AttentionLaunch a, AttnSets sets, int parts) {
+template <class T, int D, int BN, bool SEL, class Sets>
+__global__ __launch_bounds__(256, IsF32<T>::v && D == 128 ? 1 : 2) void attention_split_kernel(AttentionLaunch a, Sets sets, int parts) {
     using S = Shape<T, D>;
     constexpr int SUB = BN / 32, IMG = BN * D * (int)sizeof(T);
     __shared__ alignas(16) union {
         char v[4][IMG];
         Meeting<D> sums;
     } lds;
-    const SetsHere here = sets_here(sets);
+    const Launch here = launch_of(sets);
     const int units = here.units * parts, unit = xcd_unit(blockIdx.x, units);
     if (unit >= units) return;
     const int part = rem24(unit, parts), tile = quot24(unit, parts);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const SetHere set = set_of(here, sets, sets.tile, tile, lane);
+    const SetHere set = set_of_tile(sets, tile, lane);
     const int q0 = set.q0, k0 = set.k0, nk = set.nk, kvh = a.k.heads, group = quot24(a.q.heads, kvh);
     // SEL: tiles of a query's group never hold rows of another query
     const int nq = set.nq, all = nq * group, per_q = (group + 31) / 32, tiles = SEL ? nq * per_q : (all + 31) / 32;
@@ -463,7 +463,7 @@ __global__ __launch_bounds__(256, IsF32<T>::v && D == 128 ? 1 : 2) void attentio
         const f32x4 y = of_meeting(lds.sums, r, d, c, m, l);
         const RowPlace p = row_place(row0 + r, rows, group, g, q0);
         if (parts > 1) {
-            Part<D>& w = ((Part<D>*)a.work)[(long long)((int)(p.q - here.first.q0) * a.q.heads + p.head) * parts + part];
+            Part<D>& w = ((Part<D>*)a.work)[(long long)((int)(p.q - here.q0) * a.q.heads + p.head) * parts + part];
             *(f32x4*)&w.o[d] = y;
             if (d == 0) {
                 w.m = m;
@@ -490,8 +490,8 @@ template <class T, int D, bool SEL> struct JoinShape {
     static constexpr bool HALF = !__is_same(P, Part<D>);   // o is a mean there, a sum here
     static constexpr int C = HALF ? 8 : 4, TEAM = D / C, TEAMS = 256 / TEAM;
 };
-template <class T, int D, bool SEL, int PG>
-__global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, AttnSets sets, int parts) {
+template <class T, int D, bool SEL, int PG, class Sets>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, Sets sets, int parts) {
     using J = JoinShape<T, D, SEL>;
     using P = typename J::P;
     constexpr int C = J::C, TEAM = J::TEAM, TEAMS = J::TEAMS;
@@ -502,23 +502,24 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, 
     };
     __shared__ Sum met[PG > 1 ? 256 : 1];
     const int team = threadIdx.x / TEAM, sub = team % PG, d = threadIdx.x % TEAM * C;
-    const unsigned heads = a.q.heads, n = (unsigned)(sets.q_off[sets.n] - sets.q_off[0]) * heads, at = blockIdx.x * (TEAMS / PG) + team / PG;
+    const Launch here = launch_of(sets);
+    const unsigned heads = a.q.heads, n = (unsigned)(here.q1 - here.q0) * heads, at = blockIdx.x * (TEAMS / PG) + team / PG;
     const unsigned rh = min(at, n - 1);   // (a team behind the last does its work again and keeps it to itself)
     const float c = a.scale * kLog2e;
     const P* w = (const P*)a.work + (long long)rh * parts;
-    const long long q = sets.q_off[0] + (int)(rh / heads);
+    const long long q = here.q0 + (int)(rh / heads);
     const int head = (int)(rh % heads);
     int blocks = 0;
     const int* sel = nullptr;
     if constexpr (SEL) {
-        // the set of the work-group's first row, and on from there
-        int s = 0;
-        if (sets.n > 1) {
+        if constexpr (__is_same(Sets, OneSet)) {
+            blocks = sets.blocks;
+        } else {   // the set of the work-group's first row, and on from there
             const unsigned first = min(blockIdx.x * (TEAMS / PG), n - 1);
-            s = find_set(sets.q_off, sets.q_off[0] + (int)(first / heads), threadIdx.x & 63);
+            int s = find_set(sets.q_off, here.q0 + (int)(first / heads), threadIdx.x & 63);
             while (q >= sets.q_off[s + 1]) s++;
+            blocks = sets.blk[s + 1] - sets.blk[s];
         }
-        blocks = sets.blk[s + 1] - sets.blk[s];
         sel = a.sel + (q * a.k.heads + head / (a.q.heads / a.k.heads)) * a.n_sel;
     }
     float m = -INFINITY, l = 0.f;
@@ -603,16 +604,17 @@ __host__ __device__ inline int region_tiles(long long nq, int n_sel, int group, 
 // behind those of the blocks before it (every share counts them), its tiles where those blocks' could end at the latest.
 constexpr int kBins = 8192;    // blocks counted at a time (32 KB of LDS)
 constexpr int kBinHold = 16;   // entries per thread that stay in registers between the two passes
-__global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets sets, BinWork w) {
+template <class Sets>
+__global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, Sets sets, BinWork w) {
     __shared__ int cnt[kBins];
     __shared__ int sum_e[16], sum_t[16], sum_b[16];
     const int kvh = a.k.heads, group = quot24(a.q.heads, kvh), s = quot24(blockIdx.x, kvh), g = rem24(blockIdx.x, kvh);
-    const SetsHere here = sets_here(sets);
-    const SetHere set = here.n == 1 ? here.first : set_number(sets, s);
+    const Launch here = launch_of(sets);
+    const SetHere set = set_number(sets, s);
     const int q0 = set.q0, nq = set.nq, blocks = set.blocks, n = nq * a.n_sel;
     const int* sel = a.sel + ((long long)q0 * kvh + g) * a.n_sel;
     const int step = kvh * a.n_sel, shift = entry_shift(a.n_sel);
-    const int list0 = ((q0 - here.first.q0) * kvh + g * nq) * a.n_sel;   // of this region's entries
+    const int list0 = ((q0 - here.q0) * kvh + g * nq) * a.n_sel;   // of this region's entries
     unsigned* list = w.list + list0;
     int4* tile = w.tile + set.tile0 + (long long)g * region_tiles(nq, a.n_sel, group, blocks);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -722,18 +724,18 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, AttnSets s
 // parts, written and read, in 160 us for the three kernels (13 turning the lists, 125 here, 18 joining).
 // A wave per tile: one block's keys against 32 rows out of the queries that name it.  32 keys at a time: fewer registers, so that
 // three waves of a SIMD have loads in flight (64 at a time: 15 us more for 8 streams; two waves sharing a block: 10 % more).
-template <class T, int D>
-__global__ __launch_bounds__(64, IsF32<T>::v && D == 128 ? 1 : 2) void attention_blocks_kernel(AttentionLaunch a, AttnSets sets, BinWork w) {
+template <class T, int D, class Sets>
+__global__ __launch_bounds__(64, IsF32<T>::v && D == 128 ? 1 : 2) void attention_blocks_kernel(AttentionLaunch a, Sets sets, BinWork w) {
     using S = Shape<T, D>;
     constexpr int BN = 32, SUB = BN / 32, IMG = BN * D * (int)sizeof(T);
     __shared__ alignas(16) char lds_v[IMG];
     const int lane = threadIdx.x, h = lane >> 5;
     // (in launch order: hardly two tiles read the same block, and a region's unused tiles would leave some XCDs without work)
     const int4 t = w.tile[blockIdx.x];
-    const SetsHere here = sets_here(sets);
+    const Launch here = launch_of(sets);
     const int block = __builtin_amdgcn_readfirstlane(t.x), region = __builtin_amdgcn_readfirstlane(t.w);
     if (block < 0) return;
-    const SetHere set = here.n == 1 ? here.first : set_number(sets, region >> 22);
+    const SetHere set = set_number(sets, region >> 22);
     const int g = (region >> 6) & 0xffff, left = region & 63;   // (1..32 rows)
     const int group = quot24(a.q.heads, a.k.heads), rr = t.z + min(lane & 31, left - 1);
     const int in = group == 1 ? rr : rr / group;
@@ -765,7 +767,7 @@ __global__ __launch_bounds__(64, IsF32<T>::v && D == 128 ? 1 : 2) void attention
     }
     const float l = run.sum();
     using P = ListPart<T, D>;
-    P* to = (lane & 31) < left ? (P*)a.work + ((int)(q - here.first.q0) * a.q.heads + head) * a.n_sel + slot : nullptr;
+    P* to = (lane & 31) < left ? (P*)a.work + ((int)(q - here.q0) * a.q.heads + head) * a.n_sel + slot : nullptr;
     if constexpr (!__is_same(T, __bf16)) {
         if (!to) return;   // (both lane halves of a row leave together)
         store_row<D>(to->o, run.o, 1.f, h);
@@ -869,30 +871,45 @@ template <class T, int D, bool SEL> hipError_t join(const AttentionLaunch& a, At
     // one team per (row, head) where those fill the chip, else several
     const int pg = n * J::TEAM >= 65536 * 2 || parts < 8 ? 1 : parts < 32 ? 4 : MANY;
     const unsigned grid = (unsigned)((n + TEAMS / pg - 1) / (TEAMS / pg));
-    if (pg == 1) attention_join_kernel<T, D, SEL, 1><<<grid, 256, 0, s>>>(a, sets, parts);
-    else if (pg == 4) attention_join_kernel<T, D, SEL, 4><<<grid, 256, 0, s>>>(a, sets, parts);
-    else attention_join_kernel<T, D, SEL, MANY><<<grid, 256, 0, s>>>(a, sets, parts);
-    return hipGetLastError();
+    auto go = [&](const auto& st) {
+        using Sets = std::decay_t<decltype(st)>;
+        if (pg == 1) attention_join_kernel<T, D, SEL, 1, Sets><<<grid, 256, 0, s>>>(a, st, parts);
+        else if (pg == 4) attention_join_kernel<T, D, SEL, 4, Sets><<<grid, 256, 0, s>>>(a, st, parts);
+        else attention_join_kernel<T, D, SEL, MANY, Sets><<<grid, 256, 0, s>>>(a, st, parts);
+        return hipGetLastError();
+    };
+    if constexpr (SEL) return with_sets(sets, go);
+    else return go(OneSet(sets));
 }
 template <class T, int D> hipError_t run(const AttentionLaunch& a, AttnSets& sets, int dtype, hipStream_t s) {
     constexpr int WIDE_BN = IsF32<T>::v ? 32 : 64, OWN_BN = IsF32<T>::v || D == 128 ? 32 : 64;
     hipError_t e;
+    auto split = [&](auto sel, int parts) {
+        return with_sets(sets, [&](const auto& st) {
+            attention_split_kernel<T, D, OWN_BN, decltype(sel)::value, std::decay_t<decltype(st)>><<<xcd_grid(sets.units * parts), 256, 0, s>>>(a, st, parts);
+            return hipGetLastError();
+        });
+    };
     if (a.sel) {
         const BlocksPlan p = blocks_plan(dtype, D, a, sets);
         if (!sets.units && !p.binned) return hipSuccess;
         if (!p.binned) {
-            attention_split_kernel<T, D, OWN_BN, true><<<xcd_grid(sets.units * p.parts), 256, 0, s>>>(a, sets, p.parts);
-            e = hipGetLastError();
+            e = split(std::true_type(), p.parts);
             return e != hipSuccess || p.parts == 1 ? e : join<T, D, false>(a, sets, p.parts, s);
         }
         BinWork w;
         w.list = (unsigned*)((char*)a.work + p.part_bytes);
         w.tile = (int4*)((char*)w.list + p.list_bytes);
         if (sets.units) {
-            bin_kernel<<<dim3(sets.n * a.k.heads, kBinShares), 1024, 0, s>>>(a, sets, w);
-            if ((e = hipGetLastError()) != hipSuccess) return e;
-            attention_blocks_kernel<T, D><<<(unsigned)sets.units, 64, 0, s>>>(a, sets, w);
-            if ((e = hipGetLastError()) != hipSuccess) return e;
+            e = with_sets(sets, [&](const auto& st) {
+                using Sets = std::decay_t<decltype(st)>;
+                bin_kernel<Sets><<<dim3(sets.n * a.k.heads, kBinShares), 1024, 0, s>>>(a, st, w);
+                const hipError_t first = hipGetLastError();
+                if (first != hipSuccess) return first;
+                attention_blocks_kernel<T, D, Sets><<<(unsigned)sets.units, 64, 0, s>>>(a, st, w);
+                return hipGetLastError();
+            });
+            if (e != hipSuccess) return e;
         }
         return join<T, D, true>(a, sets, p.parts, s);
     }
@@ -900,13 +917,15 @@ template <class T, int D> hipError_t run(const AttentionLaunch& a, AttnSets& set
     if (!sets.units) return hipSuccess;
     if (p.wide) {
         const unsigned grid = xcd_grid(sets.units * p.parts);
-        if (a.lse || IsF32<T>::v) attention_wide_kernel<T, D, WIDE_BN, false><<<grid, 256, 0, s>>>(a, sets, p.parts);
-        else attention_wide_kernel<T, D, WIDE_BN, !IsF32<T>::v><<<grid, 256, 0, s>>>(a, sets, p.parts);
-        e = hipGetLastError();
+        e = with_sets(sets, [&](const auto& st) {
+            using Sets = std::decay_t<decltype(st)>;
+            if (a.lse || IsF32<T>::v) attention_wide_kernel<T, D, WIDE_BN, false, Sets><<<grid, 256, 0, s>>>(a, st, p.parts);
+            else attention_wide_kernel<T, D, WIDE_BN, !IsF32<T>::v, Sets><<<grid, 256, 0, s>>>(a, st, p.parts);
+            return hipGetLastError();
+        });
         return e != hipSuccess || p.parts == 1 ? e : join<T, D, false>(a, sets, p.parts, s);
     }
-    attention_split_kernel<T, D, OWN_BN, false><<<xcd_grid(sets.units * p.parts), 256, 0, s>>>(a, sets, p.parts);
-    e = hipGetLastError();
+    e = split(std::false_type(), p.parts);
     return e != hipSuccess || p.parts == 1 ? e : join<T, D, false>(a, sets, p.parts, s);
 }
 template <class T> hipError_t run_dim(const AttentionLaunch& a, AttnSets& sets, int dtype, int head_dim, hipStream_t s) {

@@ -20,11 +20,6 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
-// The set whose [off[i], off[i+1]) holds x, the same for all 64 lanes; off ascends, off[0] <= x < off[n], INT_MAX behind off[n].
-__device__ __forceinline__ int find_set(const int* off, int x, int lane) {
-    static_assert(PPG_ATTN_MAX_SETS == 128, "two sets per lane");
-    return __popcll(__ballot(off[lane + 1] <= x)) + __popcll(__ballot(off[lane + 65] <= x));
-}
 // What a work-group needs to know of its set.
 struct SetHere {
     int q0, nq, k0, nk, tile0, blk0, blocks;
@@ -33,19 +28,30 @@ __device__ __forceinline__ SetHere set_number(const AttnSets& sets, int s) {
     const int q0 = sets.q_off[s], k0 = sets.k_off[s], blk0 = sets.blk[s];
     return {q0, sets.q_off[s + 1] - q0, k0, sets.k_off[s + 1] - k0, sets.tile[s], blk0, sets.blk[s + 1] - blk0};
 }
-// Sets and units of a launch, and what one set alone has: all of it asked for before any of it is looked at.
-struct SetsHere {
-    int n, units;
-    SetHere first;
+// What a launch has for all: its units, first and behind the last query row.  Asked for before any of it is looked at.
+struct Launch {
+    int units, q0, q1;
 };
-__device__ __forceinline__ SetsHere sets_here(const AttnSets& sets) {
-    int n = sets.n, units = sets.units, q0 = sets.q_off[0], q1 = sets.q_off[1], k0 = sets.k_off[0], k1 = sets.k_off[1], blocks = sets.blk[1];
-    asm volatile("" : "+s"(n), "+s"(units), "+s"(q0), "+s"(q1), "+s"(k0), "+s"(k1), "+s"(blocks));   // (the compiler would put the loads off)
-    return {n, units, {q0, q1 - q0, k0, k1 - k0, 0, 0, blocks}};
+__device__ __forceinline__ Launch launch_of(const AttnSets& sets) {
+    int units = sets.units, n = sets.n, q0 = sets.q_off[0];
+    asm volatile("" : "+s"(units), "+s"(n), "+s"(q0));   // (the compiler would put the loads off)
+    return {units, q0, sets.q_off[n]};
 }
-__device__ __forceinline__ SetHere set_of(const SetsHere& here, const AttnSets& sets, const int* off, int x, int lane) {
-    return here.n == 1 ? here.first : set_number(sets, find_set(off, x, lane));
+__device__ __forceinline__ Launch launch_of(const OneSet& set) { return {set.units, set.q0, set.q1}; }
+// The set of tile, key block or query row x, the same for the wave; off ascends from off[0] <= x, INT_MAX behind the last set's end.
+__device__ __forceinline__ int find_set(const int* off, int x, int lane) {
+    static_assert(PPG_ATTN_MAX_SETS == 128, "two sets per lane");
+    return __popcll(__ballot(off[lane + 1] <= x)) + __popcll(__ballot(off[lane + 65] <= x));
 }
+__device__ __forceinline__ SetHere set_of_tile(const AttnSets& sets, int x, int lane) { return set_number(sets, find_set(sets.tile, x, lane)); }
+__device__ __forceinline__ SetHere set_of_block(const AttnSets& sets, int x, int lane) { return set_number(sets, find_set(sets.blk, x, lane)); }
+__device__ __forceinline__ SetHere set_number(const OneSet& set, int) {
+    int q0 = set.q0, q1 = set.q1, k0 = set.k0, k1 = set.k1, blocks = set.blocks;
+    asm volatile("" : "+s"(q0), "+s"(q1), "+s"(k0), "+s"(k1), "+s"(blocks));
+    return {q0, q1 - q0, k0, k1 - k0, 0, 0, blocks};
+}
+__device__ __forceinline__ SetHere set_of_tile(const OneSet& set, int, int) { return set_number(set, 0); }
+__device__ __forceinline__ SetHere set_of_block(const OneSet& set, int, int) { return set_number(set, 0); }
 
 // Bit r of m, and how many of its bits lie below the lane's, without a 64-bit shift by what a lane holds: with the amount in the last
 // register of a wave's allocation such a shift has given wrong bits here (masks of a kernel that uses all 256).

@@ -561,6 +561,8 @@ BLOCK_SHAPES = [
     # many entries on one to five blocks, groups of more than 32 heads, more entries and more blocks than a work-group holds at a time
     (64, 4, 4, 128, 5, [1000, 999, 998, 997, 996], [30, 200, 300, 500, 640], 0.05), (32, 40, 1, 128, 16, [260], [5000], 0.0), (32, 40, 1, 64, 3, [3], [500], 0.1),
     (64, 1, 1, 64, 16, [1100], [5000], 0.05), (128, 1, 1, 32, 16, [300], [300000], 0.0),
+    # many sets of few rows or none: several in the rows that one work-group joins
+    (64, 4, 2, 64, 6, [(7 * i) % 12 * (i % 5 > 0) for i in range(128)], [(37 * i) % 700 for i in range(128)], 0.05),
 ]
 
 

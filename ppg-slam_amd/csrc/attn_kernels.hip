@@ -268,7 +268,7 @@ __device__ __forceinline__ float key_float(unsigned k) {
 // blocks reach for sure, so only blocks with product + E >= t can be among them.  Mostly those are n_sel and that is the
 // answer; else they are scored in 64 bits and ranked exactly.  Rows for which that does not hold together (a product that is
 // not finite, or more than 128 left, as with many equal means) go the plain way.
-// 8 streams of 1024 rows against 65537 keys (1025 blocks), 4 heads of 64: 107 us, of which the products take half (the conversion of
+// 8 streams of 1024 rows against 65537 keys (1025 blocks), 4 heads of 64: 104 us, of which the products take half (the conversion of
 // the means to bf16 halves, repeated for every 32 rows, and the latency of the L2) and the choice the other half (some 600
 // vector instructions a row); all products in 64 bits on their matrix unit would be 61 us without any choice.
 constexpr int kSelWaves = 16;
@@ -639,7 +639,7 @@ hipError_t launch_block_select(int dtype, int head_dim, const BlockSelectLaunch&
     int most = 0;
     for (int i = 0; i < sets.n; i++) most = std::max(most, sets.blk[i + 1] - sets.blk[i]);
     // a row per wave where that still leaves CUs without work (one frame of 500 rows, 4 heads, 313 blocks: 13 us, 23 us with two), else two, which read
-    // the means half as often (8 streams of 1024 rows: 107 us, 149 us with one); few blocks: as many registers as those take
+    // the means half as often (8 streams of 1024 rows: 104 us, 149 us with one); few blocks: as many registers as those take
 #define SELECT(ROWS, PER)                                                                                                                      \
     return with_sets(sets, [&](const auto& st) {                                                                                               \
         BY_TYPE(dtype, BY_DIM(head_dim, (block_select_kernel<T, D, ROWS, PER, std::decay_t<decltype(st)>><<<xcd_grid(sets.units), 1024, 0, s>>>(a, st)))); \

@@ -274,7 +274,8 @@ __global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) 
 }
 
 // A wave's own stretch of keys: keys, then values, through an LDS image of its own.
-// One row against 400003 keys, 4 heads of 64: 410 MB in 87 us, 4.7 TB/s (a copy reaches 5.1).
+// One row against 400003 keys, 4 heads of 64: 410 MB in 79 us, 5.2 TB/s (a copy reaches 5.1, half of it written; with a
+// lane per row for the keys' loads, 85 us).
 template <class T, int D, int BN> struct OwnKeys {
     using S = Shape<T, D>;
     static constexpr int SUB = BN / 32, VC = BN * S::CPR / 64, ROWB = D * (int)sizeof(T);
@@ -721,7 +722,7 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, Sets sets,
 }
 
 // Bound by memory: 8 streams of 1024 rows, 16 of 1025 blocks of 64 keys each, 4 heads of 64: 547 MB of inputs and results and 150 MB of
-// parts, written and read, in 160 us for the three kernels (13 turning the lists, 125 here, 18 joining).
+// parts, written and read, in 158 us for the three kernels (13 turning the lists, 125 here, 19 joining).
 // A wave per tile: one block's keys against 32 rows out of the queries that name it.  32 keys at a time: fewer registers, so that
 // three waves of a SIMD have loads in flight (64 at a time: 15 us more for 8 streams; two waves sharing a block: 10 % more).
 template <class T, int D, class Sets>

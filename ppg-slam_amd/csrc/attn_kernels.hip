@@ -640,13 +640,16 @@ hipError_t launch_block_select(int dtype, int head_dim, const BlockSelectLaunch&
     for (int i = 0; i < sets.n; i++) most = std::max(most, sets.blk[i + 1] - sets.blk[i]);
     // a row per wave where that still leaves CUs without work (one frame of 500 rows, 4 heads, 313 blocks: 13 us, 23 us with two), else two, which read
     // the means half as often (8 streams of 1024 rows: 104 us, 149 us with one); few blocks: as many registers as those take
+    // (8 streams of about 250 rows, 8 heads, 172 blocks: 58 us, 65 us with room for 1088)
 #define SELECT(ROWS, PER)                                                                                                                      \
     return with_sets(sets, [&](const auto& st) {                                                                                               \
         BY_TYPE(dtype, BY_DIM(head_dim, (block_select_kernel<T, D, ROWS, PER, std::decay_t<decltype(st)>><<<xcd_grid(sets.units), 1024, 0, s>>>(a, st)))); \
         return hipGetLastError();                                                                                                              \
     })
-    if (select_tiles(a, sets, 32) >= 256) SELECT(32, 17);
-    else if (!select_tiles(a, sets, 16)) return hipSuccess;
+    if (select_tiles(a, sets, 32) >= 256) {
+        if (most <= 5 * 64) SELECT(32, 5);
+        else SELECT(32, 17);
+    } else if (!select_tiles(a, sets, 16)) return hipSuccess;
     else if (most <= 5 * 64) SELECT(16, 5);
     else SELECT(16, 17);
 #undef SELECT

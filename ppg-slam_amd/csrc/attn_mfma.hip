@@ -424,29 +424,37 @@ __global__ __launch_bounds__(256, IsF32<T>::v && D == 128 ? 1 : 2) void attentio
     const T* vp = (const T*)a.v.p + g * a.v.head + (long long)k0 * a.v.row;
     const int* sel = SEL ? a.sel + ((long long)(q0 + at / per_q) * kvh + g) * a.n_sel : nullptr;
     const int per_shift = SEL && a.block > BN ? __builtin_ctz((unsigned)a.block / BN) : 0, blocks = SEL ? (nk + a.block - 1) / a.block : 0;
-    const int nt = SEL ? (nk ? a.n_sel << per_shift : 0) : (int)(((unsigned)nk + BN - 1) / BN);
-    const int from = share_begin(nt, part, parts), to = share_begin(nt, part + 1, parts);
+    // SEL: a lane per place of the list, and those that name a block moved to the front; the waves take their tiles in turn.
+    // Whole sets: a stretch for every part, whose tiles the waves take in turn.
+    int listed = -1, named = 0;
+    if constexpr (SEL) {
+        static_assert(PPG_ATTN_MAX_SEL <= 64, "a lane per place");
+        listed = lane < a.n_sel ? sel[lane] : -1;
+        const unsigned long long ok = __ballot(listed >= 0 && listed < blocks);
+        named = __popcll(ok);
+        const int before = bits_below(ok), place = listed >= 0 && listed < blocks ? before : named + lane - before;
+        listed = __builtin_amdgcn_ds_permute(place << 2, listed);
+    }
+    const int nt = SEL ? named << per_shift : (int)(((unsigned)nk + BN - 1) / BN);
+    const int from = SEL ? part * 4 : share_begin(nt, part, parts), to = SEL ? nt : share_begin(nt, part + 1, parts), stride = SEL ? 4 * parts : 4;
     OwnKeys<T, D, BN> keys;
     keys.begin(kp, vp, a.k.row, a.v.row, a.skip ? a.skip + k0 : nullptr, lane);
     auto load = [&](int t) {
         if constexpr (SEL) {
-            const int b = sel[t >> per_shift], j = (t & ((1 << per_shift) - 1)) * BN;
-            const bool ok = b >= 0 && b < blocks;
-            const int first = ok ? b * a.block : 0;
+            const int first = __builtin_amdgcn_readlane(listed, t >> per_shift) * a.block, j = (t & ((1 << per_shift) - 1)) * BN;
             keys.load(first, j, min(a.block, nk - first), lane);
-            if (!ok) keys.masked = 1;
         } else {
             keys.load(0, t * BN, nk, lane);
         }
     };
     if (from + wave < to) load(from + wave);
     rows_to_operand<T, D>(qf, qx, lds.v[wave], lane);
-    for (int t = from + wave; t < to; t += 4) {
+    for (int t = from + wave; t < to; t += stride) {
         f32x16 sc[SUB];
         keys.settle(lane);
         keys.scores(sc, qf, lds.v[wave], lane);
         keys.values_to_lds(lds.v[wave], lane);
-        if (t + 4 < to) load(t + 4);
+        if (t + stride < to) load(t + stride);
         run.template weights<SUB>(sc, c, slack);
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -844,7 +852,13 @@ BlocksPlan blocks_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSe
     const size_t part = (size_t)(head_dim + 4) * sizeof(float), list_part = dtype == PPG_BF16 ? (size_t)head_dim * 2 + 16 : part;
     BlocksPlan p{};
     sets.tile[0] = 0;
-    if (nq * kvh * a.n_sel * a.block * head_dim * (dtype == PPG_F32 ? 8 : 4) > kDirectBytes) {
+    long long named = 0, longest = 1;   // (query, block)s at most, and of one query
+    for (int s = 0; s < sets.n; s++) {
+        const long long most = std::max(1, std::min(a.n_sel, sets.blk[s + 1] - sets.blk[s]));
+        named += (sets.q_off[s + 1] - (long long)sets.q_off[s]) * most;
+        longest = std::max(longest, most);
+    }
+    if (named * kvh * a.block * head_dim * (dtype == PPG_F32 ? 8 : 4) > kDirectBytes) {
         p.binned = true;
         p.parts = a.n_sel;
         for (int s = 0; s < sets.n; s++)
@@ -859,7 +873,7 @@ BlocksPlan blocks_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSe
     const long long per_q = (group + 31) / 32;
     for (int s = 0; s < sets.n; s++) sets.tile[s + 1] = sets.tile[s] + (int)((sets.q_off[s + 1] - sets.q_off[s]) * per_q * kvh);
     const int units = end_tiles(sets), bn = dtype == PPG_F32 || head_dim == 128 ? 32 : 64;
-    const long long most = std::max(1LL, ((long long)a.n_sel * ((a.block + bn - 1) / bn) + 3) / 4);
+    const long long most = std::max(1LL, (longest * ((a.block + bn - 1) / bn) + 3) / 4);
     p.parts = units ? (int)std::min<long long>(most, std::max(1, kFill / units)) : 1;
     if (p.parts > 1) p.part_bytes = (size_t)nq * a.q.heads * p.parts * part;
     return p;
@@ -938,10 +952,11 @@ template <class T> hipError_t run_dim(const AttentionLaunch& a, AttnSets& sets, 
 size_t attention_work(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets) {
     if (a.n_sel) {
         const BlocksPlan p = blocks_plan(dtype, head_dim, a, sets);
-        // (a list's sums are joined by head_dim / 4 threads or half as many; what is not turned round is small)
+        // (a list's sums are joined by head_dim / 4 threads or half as many)
         const long long n = ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads;
         if (p.binned && !(launch_fits(sets.units, 64) && launch_fits((long long)sets.n * a.k.heads * kBinShares, 1024) && launch_fits(n, head_dim / 4)))
             return kNoWork;
+        if (!p.binned && !launch_fits(xcd_grid(sets.units * p.parts), 256)) return kNoWork;
         return p.part_bytes + p.list_bytes + p.tile_bytes;
     }
     const DensePlan p = dense_plan(dtype, head_dim, a, sets);

@@ -138,6 +138,8 @@ def test_what_one_launch_cannot_count_is_refused(pkg):
              ("ppg_block_select", pkg.block_select_args(dtype=pkg.F32, head_dim=64, block=64, q_off=pkg.offsets([0, 1 << 27]), k_off=pkg.offsets([0, 9]), q=_rows(pkg, heads=1),
                                                        kv_heads=1, mean=4096, count=4096, n_sel=4, sel=4096)),
              ("ppg_attention", _attention(pkg, q_off=pkg.offsets([0] + [32640 + i for i in range(128)]), k_off=pkg.offsets([0] * 129), **{x: _rows(pkg, **wide) for x in ("q", "k", "v", "out")})),
+             ("ppg_attention", _attention(pkg, q_off=pkg.offsets([0, 16384]), k_off=pkg.offsets([0, 64]), block=32, n_sel=1, sel=4096, dtype=pkg.BF16, head_dim=32,
+                                          q=_rows(pkg, **wide), out=_rows(pkg, **wide), k=_rows(pkg, heads=1), v=_rows(pkg, heads=1))),
              ("ppg_attention", _attention(pkg, q_off=pkg.offsets([0, 1 << 27]), block=64, n_sel=3, sel=4096))]
     for call, args in cases:
         rc, why = _refusal(pkg, call, args)

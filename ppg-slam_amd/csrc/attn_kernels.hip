@@ -267,11 +267,14 @@ __device__ __forceinline__ float key_float(unsigned k) {
 // 2^-15).  They stay in LDS.  Then a wave takes a row: the n_sel-th largest of (product - E) is a bound t that the n_sel best
 // blocks reach for sure, so only blocks with product + E >= t can be among them.  Mostly those are n_sel and that is the
 // answer; else they are scored in 64 bits and ranked exactly.  Rows for which that does not hold together (a product that is
-// not finite, or more than 128 left, as with many equal means) go the plain way.
+// not finite, more than 128 left, as with many equal means, or a vector shorter than 1e-12 that is not zero) go the plain way.
 // 8 streams of 1024 rows against 65537 keys (1025 blocks), 4 heads of 64: 104 us, of which the products take half (the conversion of
 // the means to bf16 halves, repeated for every 32 rows, and the latency of the L2) and the choice the other half (some 600
 // vector instructions a row); all products in 64 bits on their matrix unit would be 61 us without any choice.
 constexpr int kSelWaves = 16;
+// A vector that is not zero has at least this for its squares' sum (they vanish in 32 bits below 2^-75): far below where the bound is
+// given up (1e-24), far above zero.
+constexpr float kNoSquare = 1e-30f;
 // A row's scores, and once its wave has them in registers, that wave's notes: the blocks left, their bounds, their exact keys.
 template <int PER> union SelectRow {
     float score[PER * 64 + 4];
@@ -337,6 +340,7 @@ __global__ __launch_bounds__(1024, 4) void block_select_kernel(BlockSelectLaunch
             *(__bf16*)(q_chunk(0, r, d >> 3) + (d & 7) * 2) = hi;
             *(__bf16*)(q_chunk(1, r, d >> 3) + (d & 7) * 2) = lo;
             sq = fmaf((float)x, (float)x, sq);
+            if (x != 0 && sq < kNoSquare) sq = kNoSquare;
         }
         sq = wave_sum(sq);
         // (one so short that its components leave bf16's range has no such bound, unless it is zero)
@@ -361,6 +365,14 @@ __global__ __launch_bounds__(1024, 4) void block_select_kernel(BlockSelectLaunch
                     ml[k][e] = (__bf16)(x - (float)mh[k][e]);
                     sm = fmaf(x, x, sm);
                 }
+            if (__any(sm < kNoSquare)) {   // hardly ever: the mean of a block without keys
+                bool any = false;
+#pragma unroll
+                for (int k = 0; k < D / 32; k++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) any |= mx[k][e / 4][e % 4] != 0.f;
+                if (any && sm < kNoSquare) sm = kNoSquare;
+            }
             const bool on = alive;
             if ((t + kSelWaves) * 16 < n) load(b0, t + kSelWaves);
 #pragma unroll

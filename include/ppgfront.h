@@ -431,7 +431,8 @@ int ppg_block_select(ppg_ctx* ctx, const ppg_block_select_args* args, void* stre
  * sel (optional, with block and n_sel): only the listed blocks of the set, [rows of q][kv_heads][n_sel] as
  * ppg_block_select writes them; numbers that name no block of the set are passed over, and a block listed twice counts
  * twice.  A row with nothing to attend to (or whose products are all -inf) gives 0, and -inf in lse.
- * lse (optional, [rows of q][heads]): log sum_j exp(scale * q . k_j).
+ * lse (optional, [rows of q][heads]): log sum_j exp(scale * q . k_j), infinite where 32 bits do not hold it; scale * q . k_j itself
+ * may pass them: the weights depend on differences.  A product q . k_j that passes them is infinite (+inf: NaN for its row).
  * Products and sums are held in 32 bits, the sums undivided: |v| times the number of keys stays below 2^120.  With 16-bit inputs the softmax's weights are rounded to that type before they
  * meet the values, as the inputs of the matrix unit are. */
 typedef struct ppg_attention_args {

@@ -99,7 +99,7 @@ template <class E, int D, class To> __device__ __forceinline__ void store_rows(c
     }
 }
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }
-template <class T> __device__ __forceinline__ float log_sum(float m, float l, float c) { return l == 0.f ? -INFINITY : fmaf(m, c, __log2f(l) - kLift<T>) * kLn2; }
+template <class T> __device__ __forceinline__ float log_sum(float m, float l, float scale) { return l == 0.f ? -INFINITY : fmaf(m, scale, (__log2f(l) - kLift<T>) * kLn2); }
 
 // Sums of one (row, part): D components, then m and l.  A part without keys has m = -inf, l = 0.
 template <int D> struct Part {
@@ -259,7 +259,7 @@ __global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) 
         }
         return;
     }
-    if (a.lse && h == 0 && row < rows) a.lse[place.q * a.q.heads + place.head] = log_sum<T>(run.m, l, c);
+    if (a.lse && h == 0 && row < rows) a.lse[place.q * a.q.heads + place.head] = log_sum<T>(run.m, l, a.scale);
     if constexpr (IsF32<T>::v) {
         if (row < rows) store_row<D>((float*)a.out.p + place.q * a.out.row + place.head * a.out.head, run.o, inverse_sum(l), h);
     } else {
@@ -487,7 +487,7 @@ __global__ __launch_bounds__(256, IsF32<T>::v && D == 128 ? 1 : 2) void attentio
         T* to_ = (T*)a.out.p + p.q * a.out.row + p.head * a.out.head + d;
         if constexpr (IsF32<T>::v) *(f32x4*)to_ = __builtin_bit_cast(f32x4, out);
         else *(s16x4*)to_ = __builtin_bit_cast(s16x4, out);
-        if (a.lse && d == 0) a.lse[p.q * a.q.heads + p.head] = log_sum<T>(m, l, c);
+        if (a.lse && d == 0) a.lse[p.q * a.q.heads + p.head] = log_sum<T>(m, l, a.scale);
     }
 }
 
@@ -584,7 +584,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, 
 #pragma unroll
     for (int e = 0; e < C; e++) out.v[e] = (T)(inv == 0.f ? 0.f : o[e] * inv);
     *(Out*)((T*)a.out.p + q * a.out.row + head * a.out.head + d) = out;
-    if (a.lse && d == 0) a.lse[q * a.q.heads + head] = log_sum<T>(m, l, c);
+    if (a.lse && d == 0) a.lse[q * a.q.heads + head] = log_sum<T>(m, l, a.scale);
 }
 
 // ---- selected blocks, many queries ----

@@ -114,6 +114,12 @@ __device__ __forceinline__ float rise_slack(float c) { return fminf(8.f / c, 3e3
 // then keep their precision (and the largest, 2^8 over m, are 2^15).
 template <class T> constexpr float kLift = __is_same(T, _Float16) ? 7.f : 0.f;
 
+// A weight's exponent is s c - m c, one instruction with m c computed once.  That m c is rounded: off by 2^-24 of itself, for all keys
+// alike, but not alike for two stretches of keys with maxima of their own, and where it passes 2^31 or 32 bits themselves the weights
+// under- or overflow altogether.  Beyond kFar (off by 2^-12 there) it is (s - m) c.  The test costs 1 % where the vector unit is the
+// bound (64 streams: 101 -> 102 us); taken where m rises, once a tile, it cost up to 70 registers.
+constexpr float kFar = 4096.f;
+
 // Running softmax of the 32 queries of a wave, and their sums; m is the largest product seen (or up to 2^8 less in the
 // exponent: the sums are rescaled only when a product passes it by that much, which any type holds), c = scale * log2 e.
 //
@@ -146,7 +152,7 @@ template <class T, int D, bool UNIT = false> struct Running {
     }
     // makes room for scores up to mt
     __device__ __forceinline__ void rise(float mt, float c, float slack) {
-        const bool up = mt > m + slack;
+        const bool up = mt - m > slack;   // (m + slack may round to more; -inf - -inf is no rise)
         if (__any(up)) {
             const float mn = up ? mt : m;
             const float alpha = mn == m ? 1.f : __builtin_amdgcn_exp2f((m - mn) * c);
@@ -165,8 +171,17 @@ template <class T, int D, bool UNIT = false> struct Running {
     }
     // weights in the place of the scores
     template <int SUB> __device__ __forceinline__ void weigh(f32x16 (&s)[SUB], float c) {
-        const float mc = (m == -INFINITY ? 0.f : m * c) - kLift<T>;   // (nothing so far: every weight below is exp2(-inf))
+        float mc = (m == -INFINITY ? 0.f : m * c) - kLift<T>;   // (nothing so far: every weight below is exp2(-inf))
         float sum[2] = {0.f, 0.f};
+        const bool far = fabsf(mc) > kFar;
+        if (__any(far)) {   // (in place, and nothing for queries that are not: their weights do not depend on which others are in the wave)
+            const float by = far ? m : 0.f;
+            mc = far ? -kLift<T> : mc;
+#pragma unroll
+            for (int u = 0; u < SUB; u++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[u][r] -= by;
+        }
 #pragma unroll
         for (int u = 0; u < SUB; u++)
 #pragma unroll

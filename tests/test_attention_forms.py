@@ -70,3 +70,76 @@ def test_block_select_of_very_short_vectors(gpu, dtype, what, size, q_off):
     got = _select(gpu, dtype, q.cuda(), mean, count, q_off, [0, 313 * 32], 32, 16)
     want = _select_ref(q.float().numpy(), mean.numpy(), count.numpy(), q_off, [0, 313 * 32], 32, 4, 16)
     assert np.array_equal(got, want), int((got != want).any(-1).sum())
+
+
+# ------------------------------------------------------------------------------------------------ products far from zero
+
+def _far_ref(torch, q, k, v, scale):
+    """One key head, every query head against all of k, v [n][64]: (out, lse, tolerance without the type's roundings, sum p|v|).
+    The products of these inputs are exact in 32 bits.  A weight's argument, its distance to a maximum that may be 8 binary orders
+    (5.6) off, is off by 2^-21 of itself and the exponential by 2^-22; a sum as in test_attention.py; twice, for the numerator and the
+    denominator."""
+    z = (q.double() @ k.double().t()) * scale
+    far = z - z.amax(-1, keepdim=True)
+    p = torch.exp(far)
+    total = p.sum(-1, keepdim=True)
+    w = p / total
+    t = w * (2.0 ** -20 * (7 + far.abs().clamp(max=1e4)) + 2 * (k.shape[0] / 32 + 64) * 2.0 ** -24)
+    out, a = w @ v.double(), w @ v.double().abs()
+    return out, (z.amax(-1, keepdim=True) + torch.log(total))[..., 0], t @ v.double().abs() + t.sum(-1, keepdim=True) * a, a
+
+
+# name -> (A, B, scale): products are +-A^2 + B x, x = 0..7
+FAR = {"2^28": (2.0 ** 14, 32.0, 0.11), "2^40": (2.0 ** 20, 2.0 ** 17, 1.0), "3e38": (5.5, 2.0 ** -3, 1e37), "6e38": (8.0, 2.0 ** -3, 1e37)}
+# form -> (queries, heads, kv_heads, keys, places of a list): what the rules in attn_mfma.hip make of them
+FAR_FORMS = {"rows": (3, 2, 2, 300, 0), "rows, shared keys": (2, 1, 1, 40000, 0), "tiles": (8300, 8, 1, 300, 0), "tiles, shared keys": (300, 4, 4, 9001, 0),
+             "list": (3, 2, 2, 900, 6), "lists turned round": (700, 4, 4, 1500, 9)}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("far", FAR)
+@pytest.mark.parametrize("form", FAR_FORMS)
+def test_attention_products_far_from_zero(gpu, dtype, far, form):
+    """scale * q.k of 2^24 to 2^40 and beyond what 32 bits hold, positive, negative and (the third of the query rows) near zero in
+    one call: softmax depends on differences, so no row is empty or NaN.  The maximum climbs along the keys."""
+    pkg, ctx, torch = gpu
+    A, B, scale = FAR[far]
+    if dtype == "fp16" and A > 65504:
+        pytest.skip("fp16 holds no such query")
+    nq, heads, kvh, n, places = FAR_FORMS[form]
+    t = _t(torch, dtype)
+    q, k = torch.zeros(nq, heads, 64), torch.zeros(n, kvh, 64)
+    q[0::3, :, 0], q[1::3, :, 0], q[2::3, :, 0] = A, -A, 0
+    q[:, :, 1] = B
+    k[:, :, 0] = A
+    k[:, :, 1] = (torch.arange(n) * 8 // n)[:, None].float()
+    k[:, :, 1] += ((torch.arange(n) * 7919 % 11) == 0)[:, None].float() * -1      # (some keys fall back by one)
+    v = _rand(torch, 211, n, kvh, 64).to(t)
+    q, k = q.to(t), k.to(t)
+    sel = None
+    keys = torch.arange(n)
+    if places:
+        blocks = (n + 63) // 64
+        sel = torch.arange(places, dtype=torch.int32)[None, None].repeat(nq, kvh, 1) * 2 % blocks
+        keys = torch.cat([torch.arange(i * 64, min(n, i * 64 + 64)) for i in sel[0, 0].tolist()])
+    for with_lse in (True, False):
+        out, lse = _run_attention(gpu, dtype, q.cuda(), k.cuda(), v.cuda(), scale, [0, nq], [0, n], sel=None if sel is None else sel.cuda(), block=64 if places else 0,
+                                  lse=with_lse)
+        for h in range(heads):
+            g = h // (heads // kvh)
+            ref, rl, tol, a = _far_ref(torch, q[:3, h], k[keys, g], v[keys, g], scale)
+            tol = tol + (0 if dtype == "fp32" else _u(dtype) * a * 1.01) + _u(dtype) * ref.abs() * 1.01
+            if dtype == "fp16":
+                tol = tol + 2.0 ** -25 * (v[keys, g].double().abs().sum(0) + 1)
+            got = out[:, h].cpu().double()
+            for r in range(3):
+                err = (got[r::3] - ref[min(r, nq - 1)]).abs()
+                assert (err <= tol[min(r, nq - 1)]).all(), (r, h, float(err.max()), got[r, :4].tolist() if r < nq else None)
+            if with_lse:
+                got_l = lse[:, h].cpu().double()
+                for r in range(min(3, nq)):
+                    want = float(rl[r])
+                    with np.errstate(over="ignore"):
+                        beyond = np.isinf(np.float32(want))
+                    assert ((got_l[r::3] == math.copysign(math.inf, want)) if beyond else ((got_l[r::3] - want).abs() <= 2.0 ** -21 * (abs(want) + 1))).all(), (r, h, want, got_l[r::3][:3])

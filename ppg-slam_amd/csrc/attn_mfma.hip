@@ -101,12 +101,15 @@ template <class E, int D, class To> __device__ __forceinline__ void store_rows(c
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }
 template <class T> __device__ __forceinline__ float log_sum(float m, float l, float scale) { return l == 0.f ? -INFINITY : fmaf(m, scale, (__log2f(l) - kLift<T>) * kLn2); }
 
-// Sums of one (row, part): D components, then m and l.  A part without keys has m = -inf, l = 0.
-template <int D> struct Part {
-    float o[D];
-    float m, l;
-    float pad[2];
+// Sums of every (row, part) between two kernels: D components each, so that they lie in whole lines (lists of 8 streams: 181 us, 198 with m and l
+// behind each vector), and behind all of them (m, l).  A part without keys has m = -inf, l = 0.
+template <int D> struct Parts {
+    float* o;
+    float2* ml;
+    __device__ __forceinline__ Parts(void* work, const Launch& here, int heads, int parts)
+        : o((float*)work), ml((float2*)(o + (long long)(here.q1 - here.q0) * heads * parts * D)) {}
 };
+inline size_t parts_bytes(long long n, int head_dim) { return (size_t)n * (head_dim + 2) * sizeof(float); }
 
 // Four waves of 32 rows each.  8192 x 8191 keys, 2 heads of 128, 4 sets: 300 us, 916 TFLOP/s, where a library product of 8192^3
 // reaches 1122; 64 streams of about 870, 4 heads of 64: 97 us, 517 TFLOP/s (with 8192 keys a set: 810).  Counters at 64
@@ -251,12 +254,10 @@ __global__ __launch_bounds__(256, D == 128 || (IsF32<T>::v && D == 64) ? 2 : 3) 
     const float l = run.sum();
     if (parts > 1) {
         if (row >= rows) return;
-        Part<D>& w = ((Part<D>*)a.work)[(long long)((int)(place.q - here.q0) * a.q.heads + place.head) * parts + part];
-        store_row<D>(w.o, run.o, 1.f, h);
-        if (h == 0) {
-            w.m = run.m;
-            w.l = l;
-        }
+        const Parts<D> to(a.work, here, a.q.heads, parts);
+        const long long at = (long long)((int)(place.q - here.q0) * a.q.heads + place.head) * parts + part;
+        store_row<D>(to.o + at * D, run.o, 1.f, h);
+        if (h == 0) to.ml[at] = make_float2(run.m, l);
         return;
     }
     if (a.lse && h == 0 && row < rows) a.lse[place.q * a.q.heads + place.head] = log_sum<T>(run.m, l, a.scale);
@@ -383,16 +384,6 @@ template <int D> __device__ __forceinline__ f32x4 of_meeting(const Meeting<D>& x
     return y;
 }
 
-// The same for a selected block of a query with bf16: the mean of the values (o / l) in fp16, times a power of two that brings the
-// largest into [2^13, 2^14).  That is off by 2^-11 of each component (and 2^-38 of the largest), where the result is rounded to
-// 2^-8 anyway; it halves what is written and read between the two kernels (8 streams: 208 -> 190 us when it came).
-// With fp16 the same rounding would be as large as the result's own: its parts stay in 32 bits.
-template <int D> struct PartH {
-    _Float16 o[D];
-    float m, l, scale, pad;   // o * scale is the mean
-};
-template <class T, int D> using ListPart = std::conditional_t<__is_same(T, __bf16), PartH<D>, Part<D>>;
-
 // SEL: a unit's rows are the group of one query, its keys the blocks of that query's list.
 template <class T, int D, int BN, bool SEL, class Sets>
 __global__ __launch_bounds__(256, IsF32<T>::v && D == 128 ? 1 : 2) void attention_split_kernel(AttentionLaunch a, Sets sets, int parts) {
@@ -472,12 +463,10 @@ __global__ __launch_bounds__(256, IsF32<T>::v && D == 128 ? 1 : 2) void attentio
         const f32x4 y = of_meeting(lds.sums, r, d, c, m, l);
         const RowPlace p = row_place(row0 + r, rows, group, g, q0);
         if (parts > 1) {
-            Part<D>& w = ((Part<D>*)a.work)[(long long)((int)(p.q - here.q0) * a.q.heads + p.head) * parts + part];
-            *(f32x4*)&w.o[d] = y;
-            if (d == 0) {
-                w.m = m;
-                w.l = l;
-            }
+            const Parts<D> to(a.work, here, a.q.heads, parts);
+            const long long at = (long long)((int)(p.q - here.q0) * a.q.heads + p.head) * parts + part;
+            *(f32x4*)(to.o + at * D + d) = y;
+            if (d == 0) to.ml[at] = make_float2(m, l);
             continue;
         }
         const float inv = inverse_sum(l);
@@ -494,15 +483,12 @@ __global__ __launch_bounds__(256, IsF32<T>::v && D == 128 ? 1 : 2) void attentio
 // Joins the parts of every (row, head): a team's threads take 16 bytes of components each, PG such teams the parts of one
 // (row, head) in turn, four loads in flight; the teams' sums meet in LDS in their order.  SEL: part i belongs to place i of the
 // query's list and exists only if that names a block.
-template <class T, int D, bool SEL> struct JoinShape {
-    using P = std::conditional_t<SEL, ListPart<T, D>, Part<D>>;
-    static constexpr bool HALF = !__is_same(P, Part<D>);   // o is a mean there, a sum here
-    static constexpr int C = HALF ? 8 : 4, TEAM = D / C, TEAMS = 256 / TEAM;
+template <int D> struct JoinShape {
+    static constexpr int C = 4, TEAM = D / C, TEAMS = 256 / TEAM;
 };
 template <class T, int D, bool SEL, int PG, class Sets>
 __global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, Sets sets, int parts) {
-    using J = JoinShape<T, D, SEL>;
-    using P = typename J::P;
+    using J = JoinShape<D>;
     constexpr int C = J::C, TEAM = J::TEAM, TEAMS = J::TEAMS;
     typedef float vec __attribute__((ext_vector_type(C)));
     struct Sum {
@@ -515,7 +501,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, 
     const unsigned heads = a.q.heads, n = (unsigned)(here.q1 - here.q0) * heads, at = blockIdx.x * (TEAMS / PG) + team / PG;
     const unsigned rh = min(at, n - 1);   // (a team behind the last does its work again and keeps it to itself)
     const float c = a.scale * kLog2e;
-    const P* w = (const P*)a.work + (long long)rh * parts;
+    const Parts<D> all(a.work, here, a.q.heads, parts);
+    const float* w = all.o + (long long)rh * parts * D + d;
+    const float2* ml = all.ml + (long long)rh * parts;
     const long long q = here.q0 + (int)(rh / heads);
     const int head = (int)(rh % heads);
     int blocks = 0;
@@ -539,14 +527,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionLaunch a, 
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int p = min(p0 + i * PG, parts - 1);
-            x[i].m = w[p].m;
-            x[i].l = w[p].l;
-            if constexpr (J::HALF) {
-                typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-                x[i].o = __builtin_convertvector(*(const half8*)&w[p].o[d], vec) * (w[p].scale * x[i].l);
-            } else {
-                x[i].o = *(const vec*)&w[p].o[d];
-            }
+            x[i].m = ml[p].x;
+            x[i].l = ml[p].y;
+            x[i].o = *(const vec*)(w + p * D);
             on[i] = p0 + i * PG < parts;
             if constexpr (SEL) on[i] = on[i] && (unsigned)sel[p] < (unsigned)blocks;
         }
@@ -729,8 +712,9 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, Sets sets,
     for (int i = t0 + tid; i < end; i += 1024) tile[i] = make_int4(-1, 0, 0, 0);
 }
 
-// Bound by memory: 8 streams of 1024 rows, 16 of 1025 blocks of 64 keys each, 4 heads of 64: 547 MB of inputs and results and 150 MB of
-// parts, written and read, in 158 us for the three kernels (13 turning the lists, 125 here, 19 joining).
+// Bound by memory: 8 streams of 1024 rows, 16 of 1025 blocks of 64 keys each, 4 heads of 64: 547 MB of inputs and results and 277 MB of
+// parts, written and read, in 181 us for the three kernels.  (Parts in fp16 were 20 us less, and lost what is left where the blocks'
+// values cancel.)
 // A wave per tile: one block's keys against 32 rows out of the queries that name it.  32 keys at a time: fewer registers, so that
 // three waves of a SIMD have loads in flight (64 at a time: 15 us more for 8 streams; two waves sharing a block: 10 % more).
 template <class T, int D, class Sets>
@@ -775,32 +759,11 @@ __global__ __launch_bounds__(64, IsF32<T>::v && D == 128 ? 1 : 2) void attention
         __builtin_amdgcn_wave_barrier();
     }
     const float l = run.sum();
-    using P = ListPart<T, D>;
-    P* to = (lane & 31) < left ? (P*)a.work + ((int)(q - here.q0) * a.q.heads + head) * a.n_sel + slot : nullptr;
-    if constexpr (!__is_same(T, __bf16)) {
-        if (!to) return;   // (both lane halves of a row leave together)
-        store_row<D>(to->o, run.o, 1.f, h);
-        if (h == 0) {
-            to->m = run.m;
-            to->l = l;
-        }
-    } else {
-        float f = inverse_sum(l), most = 0.f;   // of the finite ones
-#pragma unroll
-        for (int u = 0; u < D / 32; u++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const float x = fabsf(run.o[u][r] * f);
-                most = fmaxf(most, x < INFINITY ? x : 0.f);
-            }
-        const int e = max((int)(__float_as_uint(other_half(most, true)) >> 23), 14);   // biased exponent
-        f *= __uint_as_float((unsigned)(267 - e) << 23);
-        if (to && h == 0) *(f32x4*)&to->m = f32x4{run.m, l, __uint_as_float((unsigned)(e - 13) << 23), 0.f};
-        const unsigned long long at_ = (unsigned long long)to;
-        store_rows<_Float16, D>(lds_v, run.o, f, lane, [&](int r) -> void* {
-            return (void*)(((unsigned long long)(unsigned)__shfl((int)(at_ >> 32), r) << 32) | (unsigned)__shfl((int)at_, r));
-        });
-    }
+    if ((lane & 31) >= left) return;   // (both lane halves of a row leave together)
+    const Parts<D> to(a.work, here, a.q.heads, a.n_sel);
+    const int at = ((int)(q - here.q0) * a.q.heads + head) * a.n_sel + slot;
+    store_row<D>(to.o + (long long)at * D, run.o, 1.f, h);
+    if (h == 0) to.ml[at] = make_float2(run.m, l);
 }
 
 // ---- which kernel ----
@@ -849,7 +812,6 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 constexpr long long kDirectBytes = 64LL << 20;
 BlocksPlan blocks_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets) {
     const long long nq = (long long)sets.q_off[sets.n] - sets.q_off[0], kvh = a.k.heads, group = a.q.heads / kvh;
-    const size_t part = (size_t)(head_dim + 4) * sizeof(float), list_part = dtype == PPG_BF16 ? (size_t)head_dim * 2 + 16 : part;
     BlocksPlan p{};
     sets.tile[0] = 0;
     long long named = 0, longest = 1;   // (query, block)s at most, and of one query
@@ -865,7 +827,7 @@ BlocksPlan blocks_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSe
             sets.tile[s + 1] = sets.tile[s] + (int)kvh * region_tiles(sets.q_off[s + 1] - sets.q_off[s], a.n_sel, (int)group, sets.blk[s + 1] - sets.blk[s]);
         end_tiles(sets);
         end_list(sets, sets.q_off);
-        p.part_bytes = up256((size_t)nq * a.q.heads * a.n_sel * list_part);
+        p.part_bytes = up256(parts_bytes(nq * a.q.heads * a.n_sel, head_dim));
         p.list_bytes = up256((size_t)nq * kvh * a.n_sel * sizeof(int));
         p.tile_bytes = up256((size_t)sets.units * sizeof(int4));
         return p;
@@ -875,12 +837,12 @@ BlocksPlan blocks_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSe
     const int units = end_tiles(sets), bn = dtype == PPG_F32 || head_dim == 128 ? 32 : 64;
     const long long most = std::max(1LL, (longest * ((a.block + bn - 1) / bn) + 3) / 4);
     p.parts = units ? (int)std::min<long long>(most, std::max(1, kFill / units)) : 1;
-    if (p.parts > 1) p.part_bytes = (size_t)nq * a.q.heads * p.parts * part;
+    if (p.parts > 1) p.part_bytes = parts_bytes(nq * a.q.heads * p.parts, head_dim);
     return p;
 }
 
 template <class T, int D, bool SEL> hipError_t join(const AttentionLaunch& a, AttnSets& sets, int parts, hipStream_t s) {
-    using J = JoinShape<T, D, SEL>;
+    using J = JoinShape<D>;
     constexpr int TEAMS = J::TEAMS, MANY = std::min(16, TEAMS);
     const long long n = ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads;
     // one team per (row, head) where those fill the chip, else several
@@ -952,7 +914,7 @@ template <class T> hipError_t run_dim(const AttentionLaunch& a, AttnSets& sets, 
 size_t attention_work(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets) {
     if (a.n_sel) {
         const BlocksPlan p = blocks_plan(dtype, head_dim, a, sets);
-        // (a list's sums are joined by head_dim / 4 threads or half as many)
+        // (a list's sums are joined by head_dim / 4 threads)
         const long long n = ((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads;
         if (p.binned && !(launch_fits(sets.units, 64) && launch_fits((long long)sets.n * a.k.heads * kBinShares, 1024) && launch_fits(n, head_dim / 4)))
             return kNoWork;
@@ -961,7 +923,7 @@ size_t attention_work(int dtype, int head_dim, const AttentionLaunch& a, AttnSet
     }
     const DensePlan p = dense_plan(dtype, head_dim, a, sets);
     if (!launch_fits(xcd_grid(sets.units * p.parts), 256)) return kNoWork;
-    return p.parts == 1 ? 0 : ((size_t)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads * p.parts * (head_dim + 4) * sizeof(float);
+    return p.parts == 1 ? 0 : parts_bytes(((long long)sets.q_off[sets.n] - sets.q_off[0]) * a.q.heads * p.parts, head_dim);
 }
 hipError_t launch_attention(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets, hipStream_t s) {
     return dtype == PPG_F32    ? run_dim<float>(a, sets, dtype, head_dim, s)

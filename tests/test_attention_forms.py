@@ -1,7 +1,8 @@
 """Attention between descriptor sets where the sizes, layouts and values of test_attention.py do not lead: vectors so short that
 their squares vanish, products far from zero, sums that cancel, and the forms of the kernels that only large or strided calls take.
 
-References are in 64 bits; tolerances are those of test_attention.py unless a test derives its own."""
+References are in 64 bits; tolerances are those of test_attention.py unless a test derives its own.  (The room that those leave for
+block means in fp16 is not needed any more: what passes between two kernels of a call is in 32 bits.)"""
 import math
 
 import numpy as np
@@ -143,3 +144,30 @@ def test_attention_products_far_from_zero(gpu, dtype, far, form):
                     with np.errstate(over="ignore"):
                         beyond = np.isinf(np.float32(want))
                     assert ((got_l[r::3] == math.copysign(math.inf, want)) if beyond else ((got_l[r::3] - want).abs() <= 2.0 ** -21 * (abs(want) + 1))).all(), (r, h, want, got_l[r::3][:3])
+
+
+# ------------------------------------------------------------------------------------------------ sums that cancel
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("queries", (5, 900))
+def test_selected_blocks_whose_values_cancel(gpu, dtype, queries):
+    """Sums are held in 32 bits until the result is rounded, between the kernels too: with equal weights (a zero query) and blocks
+    whose values nearly cancel, what is left is right.  A weight of 1 is exact in every type, so the result is off by the 32-bit sums
+    ((keys / 32 + 64) 2^-24 of sum p|v|, for the numerator and the denominator) and one rounding."""
+    pkg, ctx, torch = gpu
+    t = _t(torch, dtype)
+    q, k = torch.zeros(queries, 4, 64, dtype=t), _rand(torch, 221, 640, 4, 64).to(t)
+    v = torch.full((640, 4, 64), 1000.0)
+    v[64:128] = -1000
+    v[320:384] = -1000
+    v[torch.arange(640) % 64 == 5] += torch.where(v[torch.arange(640) % 64 == 5] > 0, 4.0, 8.0)
+    v = v.to(t)
+    sel = torch.tensor([0, 1, 4, 5], dtype=torch.int32)[None, None].repeat(queries, 4, 1)
+    out, _ = _run_attention(gpu, dtype, q.cuda(), k.cuda(), v.cuda(), 0.125, [0, queries], [0, 640], sel=sel.cuda(), block=64)
+    keys = torch.cat([torch.arange(64 * i, 64 * i + 64) for i in (0, 1, 4, 5)])
+    want, a = v[keys].double().mean(0)[:1], v[keys].double().abs().mean(0)[:1]
+    tol = 2 * (256 / 32 + 64) * 2.0 ** -24 * a + _u(dtype) * want.abs() * 1.01
+    assert float(want.abs().min()) > 4 * float(tol.max())
+    err = (out.cpu().double() - want[:, :1]).abs()
+    assert (err <= tol[:, :1]).all(), (float(err.max()), float(tol.max()))

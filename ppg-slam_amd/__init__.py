@@ -80,16 +80,21 @@ class AttentionArgs(C.Structure):
 
 def offsets(values):
     """Set offsets as the argument structures take them (n_sets + 1 host integers)."""
-    return np.ascontiguousarray(values, np.int32)
+    a = np.asarray(values)
+    if a.ndim != 1 or not a.size or a.dtype.kind not in "iu" or a.min() < -(1 << 31) or a.max() >= 1 << 31:
+        raise ValueError("offsets: a row of n_sets + 1 whole numbers of 32 bits is needed")
+    return np.ascontiguousarray(a, np.int32)
 
 
 def _args(kind, q_off, k_off, fields):
     a = kind(**fields)
-    a._keep = (q_off, k_off)   # the structure holds addresses only
-    for name, off in (("q_off", q_off), ("k_off", k_off)):
-        if off is not None:
-            setattr(a, name, off.ctypes.data)
-            a.n_sets = len(off) - 1
+    given = {name: offsets(off) for name, off in (("q_off", q_off), ("k_off", k_off)) if off is not None}
+    if len({len(off) for off in given.values()}) > 1:
+        raise ValueError("q_off and k_off are of different numbers of sets")
+    a._keep = given   # the structure holds addresses only
+    for name, off in given.items():
+        setattr(a, name, off.ctypes.data)
+        a.n_sets = len(off) - 1
     return a
 
 

@@ -171,3 +171,31 @@ def test_selected_blocks_whose_values_cancel(gpu, dtype, queries):
     assert float(want.abs().min()) > 4 * float(tol.max())
     err = (out.cpu().double() - want[:, :1]).abs()
     assert (err <= tol[:, :1]).all(), (float(err.max()), float(tol.max()))
+
+
+# ------------------------------------------------------------------------------------------------ the Python argument helpers
+
+def test_offsets_that_do_not_belong_together_are_refused(pkg):
+    """The entry points read n_sets + 1 of both lists: two of different lengths must not reach them."""
+    for a, b in (([0, 5], [0, 7, 9]), ([0, 5, 6], [0, 7])):
+        with pytest.raises(ValueError, match="sets"):
+            _attention(pkg, q_off=pkg.offsets(a), k_off=pkg.offsets(b))
+        with pytest.raises(ValueError, match="sets"):
+            pkg.block_select_args(pkg.offsets(a), pkg.offsets(b), dtype=pkg.F32, head_dim=64, block=64, q=_rows(pkg), kv_heads=2, n_sel=4)
+
+
+@pytest.mark.parametrize("values", ([0, 1 << 31], np.array([0, (1 << 32) + 5]), [0, 2.5], np.array([0.0, 3.0]), [], [[0, 5]]), ids=str)
+def test_offsets_that_32_bits_do_not_hold_are_refused(pkg, values):
+    with pytest.raises(ValueError, match="offsets"):
+        pkg.offsets(values)
+
+
+@pytest.mark.parametrize("kind", (np.int64, np.int16, np.uint32))
+def test_offsets_of_other_types_mean_the_same(pkg, kind):
+    """Straight into the helpers, without offsets(): not read as if they were 32-bit numbers."""
+    a = _attention(pkg, q_off=np.array([0, 5], kind), k_off=np.array([0, 7], kind))
+    assert _refusal(pkg, "ppg_attention", a)[1] == "ppg_attention: ctx is NULL" and a.n_sets == 1
+    a = _attention(pkg, q_off=np.array([0, 5, 3], kind), k_off=np.array([0, 7, 9, 0][:3], kind))
+    assert "q_off[2] = 3" in _refusal(pkg, "ppg_attention", a)[1]
+    a = _attention(pkg, q_off=np.array([0, 99, 5, 99], kind)[::2], k_off=[0, 7])      # every second number of an array
+    assert _refusal(pkg, "ppg_attention", a)[1] == "ppg_attention: ctx is NULL"

@@ -433,8 +433,10 @@ int ppg_block_select(ppg_ctx* ctx, const ppg_block_select_args* args, void* stre
  * twice.  A row with nothing to attend to (or whose products are all -inf) gives 0, and -inf in lse.
  * lse (optional, [rows of q][heads]): log sum_j exp(scale * q . k_j), infinite where 32 bits do not hold it; scale * q . k_j itself
  * may pass them: the weights depend on differences.  A product q . k_j that passes them is infinite (+inf: NaN for its row).
- * Products and sums are held in 32 bits, the sums undivided: |v| times the number of keys stays below 2^120.  With 16-bit inputs the softmax's weights are rounded to that type before they
- * meet the values, as the inputs of the matrix unit are. */
+ * Products and sums are held in 32 bits, the sums undivided: |v| times the number of keys stays below 2^120.  With 16-bit
+ * inputs the softmax's weights are rounded to that type before they meet the values, as the inputs of the matrix unit are; they
+ * are divided by the sum of the unrounded weights when lse is asked for, and by that of the rounded ones where that is quicker
+ * when it is not, so out may differ between the two by as much as the weights' rounding. */
 typedef struct ppg_attention_args {
     int dtype, head_dim;
     float scale;              /* > 0, at most 1e37 */

@@ -270,7 +270,9 @@ __device__ __forceinline__ float key_float(unsigned k) {
 // not finite, more than 128 left, as with many equal means, or a vector shorter than 1e-12 that is not zero) go the plain way.
 // 8 streams of 1024 rows against 65537 keys (1025 blocks), 4 heads of 64: 104 us, of which the products take half (the conversion of
 // the means to bf16 halves, repeated for every 32 rows, and the latency of the L2) and the choice the other half (some 600
-// vector instructions a row); all products in 64 bits on their matrix unit would be 61 us without any choice.
+// vector instructions a row); all products in 64 bits on their matrix unit would be 61 us without any choice.  128 components,
+// 960 blocks: 232 us.  1024 threads leave a wave 128 registers, and every form spills: 15 vector registers at 64 components and 1088 blocks, 64 at
+// 128 (there in the loop over the rows), and scalar ones, most of them in the plain way's loop.
 constexpr int kSelWaves = 16;
 // A vector that is not zero has at least this for its squares' sum (they vanish in 32 bits below 2^-75): far below where the bound is
 // given up (1e-24), far above zero.
@@ -651,8 +653,9 @@ hipError_t launch_block_select(int dtype, int head_dim, const BlockSelectLaunch&
     int most = 0;
     for (int i = 0; i < sets.n; i++) most = std::max(most, sets.blk[i + 1] - sets.blk[i]);
     // a row per wave where that still leaves CUs without work (one frame of 500 rows, 4 heads, 313 blocks: 13 us, 23 us with two), else two, which read
-    // the means half as often (8 streams of 1024 rows: 104 us, 149 us with one); few blocks: as many registers as those take
-    // (8 streams of about 250 rows, 8 heads, 172 blocks: 58 us, 65 us with room for 1088)
+    // the means half as often (8 streams of 1024 rows: 104 us, 149 us with one); few blocks: as many registers as those take, up to
+    // 320 (8 streams of 1024 rows, 4 heads of 64 bf16, with room for 320 : for 1088: 172 blocks 62 : 73 us, 320 blocks 69 : 79; beyond, in
+    // several stretches, 321 blocks 136 : 80, 640 blocks 173 : 93; one frame 320 blocks 13.1 : 15.2, 321 blocks 20.6 : 15.1)
 #define SELECT(ROWS, PER)                                                                                                                      \
     return with_sets(sets, [&](const auto& st) {                                                                                               \
         BY_TYPE(dtype, BY_DIM(head_dim, (block_select_kernel<T, D, ROWS, PER, std::decay_t<decltype(st)>><<<xcd_grid(sets.units), 1024, 0, s>>>(a, st)))); \

@@ -111,12 +111,14 @@ template <int D> struct Parts {
 };
 inline size_t parts_bytes(long long n, int head_dim) { return (size_t)n * (head_dim + 2) * sizeof(float); }
 
-// Four waves of 32 rows each.  8192 x 8191 keys, 2 heads of 128, 4 sets: 300 us, 916 TFLOP/s, where a library product of 8192^3
-// reaches 1122; 64 streams of about 870, 4 heads of 64: 97 us, 517 TFLOP/s (with 8192 keys a set: 810).  Counters at 64
+// Four waves of 32 rows each.  8192 x 8191 keys, 2 heads of 128, 4 sets: 303 us, 907 TFLOP/s, where a library product of 8192^3
+// reaches 1122; 64 streams of about 870, 4 heads of 64: 102 us, 490 TFLOP/s (with 8192 keys a set: 810).  Counters at 64
 // components: the vector unit (exponentials, maxima, conversions: 155 instructions for 64 keys) is busy for 61 % of the time,
 // the matrix unit for 47 %, at 2.0 GHz, the clock that the power limit leaves; what short sets lose is the work-group's start
 // (queries, first tiles) and the chip's last round.  Two waves of a SIMD in opposite phases, held there by barriers, measured
 // slower (315 and 1555 us instead of 303 and 1367): a single wave cannot keep the vector unit busy.
+// 32-bit types (the matrix unit reaches 154 TFLOP/s): 64 components 124 TFLOP/s (4 sets of 4096 a side, 4 heads; 64 sets of 870: 103),
+// 32 components 115, 128 components 103 (84 for short sets): there two waves a SIMD spill 38 registers, some inside the loop.
 // parts > 1: a work-group takes its share of the keys and leaves its sums.
 // Which keys are masked is read once, a bit each, kWindow words ahead, so that the loads of a tile do not wait for it.
 // UNIT (16-bit types): the matrix unit adds up the weights (a product with ones); the vector unit, which has the exponentials, is
@@ -594,6 +596,7 @@ __host__ __device__ inline int region_tiles(long long nq, int n_sel, int group, 
 // One work-group per share of a region's blocks: counts per block, their running sum, and the entries put in their places.  Which
 // entry of a block comes first is left to the atomics: entries of a block never meet in a sum.  A share's entries start
 // behind those of the blocks before it (every share counts them), its tiles where those blocks' could end at the latest.
+// (The form for one set spills 26 registers, the other none.  One frame of 500 queries x 16: 9 us from 16 work-groups; 8 streams: 13 us.)
 constexpr int kBins = 8192;    // blocks counted at a time (32 KB of LDS)
 constexpr int kBinHold = 16;   // entries per thread that stay in registers between the two passes
 template <class Sets>
@@ -713,7 +716,7 @@ __global__ __launch_bounds__(1024) void bin_kernel(AttentionLaunch a, Sets sets,
 }
 
 // Bound by memory: 8 streams of 1024 rows, 16 of 1025 blocks of 64 keys each, 4 heads of 64: 547 MB of inputs and results and 277 MB of
-// parts, written and read, in 181 us for the three kernels.  (Parts in fp16 were 20 us less, and lost what is left where the blocks'
+// parts, written and read, in 181 us for the three kernels (13 turning the lists, 134 here, 33 joining).  (Parts in fp16 were 20 us less, and lost what is left where the blocks'
 // values cancel.)
 // A wave per tile: one block's keys against 32 rows out of the queries that name it.  32 keys at a time: fewer registers, so that
 // three waves of a SIMD have loads in flight (64 at a time: 15 us more for 8 streams; two waves sharing a block: 10 % more).
@@ -808,7 +811,9 @@ struct BlocksPlan {
 };
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 // A query's blocks are read for itself, in one launch instead of three, while that is no more than this many bytes of keys and
-// values (64 keys x 64 components bf16, 16 blocks, 4 heads: 40 queries, 42 MB: 16 us, turned round 22; 160, 168 MB: 28 and 22).
+// values.  16 of 313 blocks, 4 heads, direct against turned round in us, at 64 MB and where the second overtakes: 64 keys x 64
+// components bf16 11.6 : 16.8, 175 MB; x 128 14.6 : 18.4, 150 MB; x 32 10.6 : 16.4, 125 MB; fp32 x 64 19.4 : 25.3, 95 MB; x 128
+// 30.6 : 34.1, 75 MB; 32 keys x 64 bf16 14.0 : 16.5, 75 MB: below it for all of these.
 constexpr long long kDirectBytes = 64LL << 20;
 BlocksPlan blocks_plan(int dtype, int head_dim, const AttentionLaunch& a, AttnSets& sets) {
     const long long nq = (long long)sets.q_off[sets.n] - sets.q_off[0], kvh = a.k.heads, group = a.q.heads / kvh;

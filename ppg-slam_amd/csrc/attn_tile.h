@@ -116,8 +116,8 @@ template <class T> constexpr float kLift = __is_same(T, _Float16) ? 7.f : 0.f;
 
 // A weight's exponent is s c - m c, one instruction with m c computed once.  That m c is rounded: off by 2^-24 of itself, for all keys
 // alike, but not alike for two stretches of keys with maxima of their own, and where it passes 2^31 or 32 bits themselves the weights
-// under- or overflow altogether.  Beyond kFar (off by 2^-12 there) it is (s - m) c.  The test costs 1 % where the vector unit is the
-// bound (64 streams: 101 -> 102 us); taken where m rises, once a tile, it cost up to 70 registers.
+// under- or overflow altogether.  Beyond kFar (off by 2^-12 there) it is (s - m) c.  The test, once a tile, costs 1 % where the vector
+// unit is the bound (64 streams: 101 -> 102 us); a flag set where m rises, and kept, cost up to 70 registers.
 constexpr float kFar = 4096.f;
 
 // Running softmax of the 32 queries of a wave, and their sums; m is the largest product seen (or up to 2^8 less in the
